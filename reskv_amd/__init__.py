@@ -11,7 +11,7 @@ first use of an operator.
 from .config import KernelPlan, ResKVKernelConfig
 
 __version__ = "0.1.0"
-__all__ = ["ResKVKernelConfig", "KernelPlan", "ResKVForCausalLM", "compress", "attention"]
+__all__ = ["ResKVKernelConfig", "KernelPlan", "ResKVForCausalLM", "compress", "attention", "packed_attention"]
 
 
 def __getattr__(name):
@@ -23,6 +23,10 @@ def __getattr__(name):
         from ._attention import attention
 
         return attention
+    if name == "packed_attention":
+        from .packed import packed_attention
+
+        return packed_attention
     if name == "ResKVForCausalLM":
         from .models.llama import ResKVForCausalLM
 

@@ -69,6 +69,14 @@ SIGNATURES = {
     "reskv_merge_recent_qk": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _f, _vp, _vp]),
     "reskv_decode_dense": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _f, _i, _vp, _vp, _vp, _vp, _i64,
                                 _vp]),
+    # include/reskv_serving.h: packed prompts and the paged 4-bit cache
+    "reskv_packed_workspace_bytes": (_i64, [_i, _i64, _i, _i, _i64]),
+    "reskv_packed_attention": (_i, [_vp] * 6 + [_i, _i64, _i64, _i, _i, _vp, _f, _i64, _i, _vp, _i64, _vp]),
+    "reskv_int4_append": (_i, [_vp, _i64, _i, _i, _vp, _i, _i, _vp, _vp, _vp, _vp, _i64, _vp, _vp]),
+    "reskv_int4_gather": (_i, [_vp, _i64, _i, _i, _vp, _i, _i, _vp, _vp, _vp, _vp, _i64, _i, _vp]),
+    "reskv_int4_workspace_bytes": (_i64, [_i, _i, _i, _i64]),
+    "reskv_int4_attention": (_i, [_vp, _vp, _i64, _i, _vp, _i, _vp, _i, _i, _i, _f, _i64, _vp, _vp, _i64, _vp]),
+    "reskv_copy_pages": (_i, [_vp, _i, _i64, _i64, _vp, _vp, _i, _vp]),
     # include/reskv_llama.h: fused steps of the end-to-end decode harness
     "reskv_llama_rmsnorm": (_i, [_vp, _vp, _vp, _i, _i, _f, _vp]),
     "reskv_llama_silu_mul": (_i, [_vp, _vp, _i, _i, _vp]),

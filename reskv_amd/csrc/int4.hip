@@ -1,0 +1,797 @@
+// Paged cache of 4-bit keys and values: rows into pages, rows back, the attention of single
+// tokens that reads the pages, and page copies.  include/reskv_serving.h has the layout.
+//
+// The layout is that of the matrix cores' operands: a lane's 16-byte piece of a block holds
+// the codes that it multiplies, eight along the inner dimension per dword (eight channels
+// of a token for K, eight tokens of a channel for V), so that the attention takes them from
+// memory to v_mfma_f32_16x16x32_f16 without the LDS.  A code becomes an fp16 number by
+// masking alone: the bits 0 .. 15 of a nibble at bit 0 are the denormal code * 2^-24, at
+// bit 4 the number code * 2^-20 (the matrix cores keep denormals); the other operand carries
+// the factor 16 and the result the factor 2^24, both exact.
+#include "serving.h"
+#include "reskv_serving.h"
+
+using namespace reskv;
+
+namespace {
+
+typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
+typedef _Float16 half8_t __attribute__((ext_vector_type(8)));
+typedef float float4_t __attribute__((ext_vector_type(4)));
+
+constexpr int kBlock = 32;  // tokens (>> 5 below)
+constexpr int kBlockBytes = RESKV_INT4_BLOCK_BYTES;
+constexpr int kKScale = 2048, kVCodes = 2560, kVScale = 4608, kVLow = 4864;  // byte offsets in a block
+constexpr int kThreads = 256;
+
+struct Pool {
+    char* pages;
+    const int32_t* table;  // [sequences, width]
+    long num_pages;
+    int blocks;  // per page
+    int width, heads;
+
+    // Block `block` of sequence s and head h, null where the table holds no page for it.
+    __device__ __forceinline__ char* at(int s, int block, int h) const {
+        const int entry = block / blocks;
+        if (block < 0 || entry >= width) return nullptr;
+        const int page = table[(long)s * width + entry];
+        return in_page(page, block - entry * blocks, h);
+    }
+    __device__ __forceinline__ char* in_page(int page, int block, int h) const {
+        if (page < 0 || page >= num_pages) return nullptr;
+        return pages + (((long)page * heads + h) * blocks + block) * kBlockBytes;
+    }
+};
+
+// Position of the nibble of element e = 0 .. 7 in its dword, in bits.  Elements 2 i and
+// 2 i + 1 are 16 bits apart, so that one mask makes an operand register of both.
+__host__ __device__ constexpr int nibble(int e) { return 4 * (e / 2 + 4 * (e % 2)); }
+
+// ---------------------------------------------------------------------------
+// rows into pages and back
+// ---------------------------------------------------------------------------
+
+struct RowArgs {
+    Pool pool;
+    const int32_t* starts;
+    const int32_t* offsets;  // null: row s is the one row of sequence s
+    const uint16_t *k, *v;   // append: rows
+    uint16_t *k_out, *v_out; // gather: rows [N, heads, 128]
+    long k_token, k_head, v_token, v_head;  // strides of k, v in halves
+    int sequences, N, clear_rest;
+};
+
+// The tokens [lo, hi) of block `block` of sequence seq that this workgroup handles, and the row of the first.
+struct Part {
+    int seq, block, lo, hi;
+    long row;
+};
+
+__device__ __forceinline__ Part row_part(const RowArgs& A, int item) {
+    if (!A.offsets) {
+        const int start = A.starts[item], lead = start & (kBlock - 1);
+        return {item, start >> 5, lead, lead + 1, item};
+    }
+    const Item it = find_item(item, A.sequences, [&](int s) {
+        const int n = sequence_rows(A.offsets, s, A.N).count, lead = A.starts[s] & (kBlock - 1);
+        return n == 0 ? 0 : (lead + n + kBlock - 1) / kBlock;
+    });
+    if (it.seq < 0) return {-1, it.index, 0, 0, 0};
+    const Rows r = sequence_rows(A.offsets, it.seq, A.N);
+    const int start = A.starts[it.seq], lead = start & (kBlock - 1);  // before token 0: a block without a page
+    const int lo = it.index == 0 ? lead : 0, hi = min(kBlock, lead + r.count - it.index * kBlock);
+    if (it.index < 0 || hi <= lo) return {-1, 0, 0, 0, 0};
+    return {it.seq, (start >> 5) + it.index, lo, hi, (long)r.first + it.index * kBlock + lo - lead};
+}
+
+// Largest and smallest of 16 fp16 values and of the 16 of the lane next to it (which has the group's other half).
+struct Range {
+    float low, high;
+    bool finite;
+};
+__device__ __forceinline__ Range group_range(const float* x) {
+    float lo = x[0], hi = x[0], sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        lo = fminf(lo, x[i]);
+        hi = fmaxf(hi, x[i]);
+        sum += x[i] * 0.0f;  // NaN when a value is not finite
+    }
+    lo = fminf(lo, dpp<0xB1>(lo));
+    hi = fmaxf(hi, dpp<0xB1>(hi));
+    sum += dpp<0xB1>(sum);
+    return {lo, hi, sum == 0.0f};
+}
+
+// code of x in a group, exactly rint((x - low) / scale): the quotient in 32 bits is off by less
+// than 2^-20, and where it is nearer than that to a half, 64 bits (which hold both sides exactly) decide.
+__device__ __forceinline__ uint32_t code_of(float x, float low, float scale) {
+    if (!(scale > 0.0f)) return 0;
+    const float q = (x - low) / scale;
+    float r = rintf(q);
+    const float half_way = floorf(q) + 0.5f;
+    if (fabsf(q - half_way) < 0x1p-18f) {
+        const double side = ((double)x - (double)low) - (double)half_way * (double)scale;
+        r = side < 0.0 ? floorf(q) : side > 0.0 ? floorf(q) + 1.0f : 2.0f * rintf(0.5f * half_way);
+    }
+    return (uint32_t)fminf(fmaxf(r, 0.0f), 15.0f);
+}
+
+// One workgroup per (block of 32 tokens that gets rows, head); thread (token, part) has 16 channels.
+__global__ void __launch_bounds__(kThreads) append_kernel(RowArgs A) {
+    __shared__ __align__(16) uint32_t s_k[512];      // K codes as stored
+    __shared__ uint32_t s_kp[128];                   // K scalings as stored
+    __shared__ __align__(16) uint8_t s_v[kBlock][kDim + 16];  // V codes, a byte each
+    __shared__ uint16_t s_vp[256];                   // V scales and lowest values as stored
+    const int h = (int)blockIdx.x % A.pool.heads;
+    const Part P = row_part(A, (int)blockIdx.x / A.pool.heads);
+    if (P.seq < 0) return;
+    char* const block = A.pool.at(P.seq, P.block, h);
+    if (!block) return;
+    const int tid = threadIdx.x, token = tid >> 3, part = tid & 7, group = part >> 1;
+    const bool mine = token >= P.lo && token < P.hi;
+#pragma unroll
+    for (int side = 0; side < 2; ++side) {
+        float x[16];
+        const uint16_t* src = side == 0 ? A.k + (P.row + token - P.lo) * A.k_token + h * A.k_head
+                                        : A.v + (P.row + token - P.lo) * A.v_token + h * A.v_head;
+        uint4 w[2] = {};
+        if (mine) {
+            w[0] = reinterpret_cast<const uint4*>(src)[2 * part];
+            w[1] = reinterpret_cast<const uint4*>(src)[2 * part + 1];
+        }
+        const uint32_t words[8] = {w[0].x, w[0].y, w[0].z, w[0].w, w[1].x, w[1].y, w[1].z, w[1].w};
+#pragma unroll
+        for (int i = 0; i < 16; ++i) x[i] = h2f((uint16_t)(words[i >> 1] >> (16 * (i & 1))));
+        const Range r = group_range(x);
+        // one division in 64 bits: the quotient is then rounded once
+        const uint16_t scale16 = r.finite ? f2h((float)(((double)r.high - (double)r.low) / 15.0)) : 0x7E00;
+        const uint16_t low16 = r.finite ? f2h(r.low) : 0x7E00;
+        const float scale = h2f(scale16);
+        uint32_t code[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) code[i] = code_of(x[i], r.low, scale);
+        if (side == 0) {
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+                uint32_t packed = 0;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) packed |= code[8 * q + e] << nibble(e);
+                s_k[(((token >> 4) * 4 + 2 * (part & 1) + q) * 16 + (token & 15)) * 4 + group] = packed;
+            }
+            if ((part & 1) == 0) s_kp[((token >> 4) * 4 + group) * 16 + (token & 15)] = scale16 | ((uint32_t)low16 << 16);
+        } else {
+            uint32_t bytes[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                bytes[i] = code[4 * i] | (code[4 * i + 1] << 8) | (code[4 * i + 2] << 16) | (code[4 * i + 3] << 24);
+            *reinterpret_cast<uint4*>(&s_v[token][16 * part]) = make_uint4(bytes[0], bytes[1], bytes[2], bytes[3]);
+            if ((part & 1) == 0) {
+                s_vp[group * kBlock + token] = scale16;
+                s_vp[128 + group * kBlock + token] = low16;
+            }
+        }
+    }
+    __syncthreads();
+    if (tid < 128) {
+        const int t = (tid >> 6) * 16 + (tid & 15);  // the token of both: piece (tile, quarter, token), dword (tile, group, token)
+        if (t >= P.lo && t < P.hi) {
+            reinterpret_cast<uint4*>(block)[tid] = reinterpret_cast<const uint4*>(s_k)[tid];
+            reinterpret_cast<uint32_t*>(block + kKScale)[tid] = s_kp[tid];
+        }
+    }
+    {
+        const int t = tid & 31;  // half (scale or low, group, token)
+        if (t >= P.lo && t < P.hi) reinterpret_cast<uint16_t*>(block + kVScale)[tid] = s_vp[tid];
+    }
+    // V codes: dword (c / 64, t / 8, c % 16, c / 16 % 4) has the eight tokens of a channel; of a dword whose
+    // tokens are not all new the others' nibbles stay
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int d = tid + kThreads * i;
+        const int t0 = 8 * ((d >> 6) & 3), c = 64 * (d >> 8) + 16 * (d & 3) + ((d >> 2) & 15);
+        if (t0 + 8 <= P.lo || t0 >= P.hi) continue;
+        uint32_t packed = 0, keep = 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            if (t0 + e >= P.lo && t0 + e < P.hi) packed |= (uint32_t)s_v[t0 + e][c] << nibble(e);
+            else keep |= 15u << nibble(e);
+        }
+        uint32_t* dst = reinterpret_cast<uint32_t*>(block + kVCodes) + d;
+        if (keep) packed |= *dst & keep;
+        *dst = packed;
+    }
+}
+
+__device__ __forceinline__ uint32_t pack_halves(float a, float b) { return (uint32_t)f2h(a) | ((uint32_t)f2h(b) << 16); }
+
+// Rows of no sequence get zeros from the workgroups behind the last item (there is always one).
+__device__ void clear_rows(const RowArgs& A, int spare, int spares, int h) {
+    const int begin = min(max(A.offsets[0], 0), A.N);
+    const int end = A.sequences > 0 ? min(max(A.offsets[A.sequences], begin), A.N) : begin;
+    const int tid = threadIdx.x, rest = begin + A.N - end;
+    for (int i = spare * 16 + tid / 16; i < rest; i += spares * 16) {
+        const long row = ((long)(i < begin ? i : end + i - begin) * A.pool.heads + h) * kDim;
+        reinterpret_cast<uint4*>(A.k_out + row)[tid % 16] = make_uint4(0, 0, 0, 0);
+        reinterpret_cast<uint4*>(A.v_out + row)[tid % 16] = make_uint4(0, 0, 0, 0);
+    }
+}
+
+__global__ void __launch_bounds__(kThreads) gather_kernel(RowArgs A) {
+    __shared__ __align__(16) uint32_t s_v[512];
+    __shared__ uint32_t s_vp[128];
+    const int h = (int)blockIdx.x % A.pool.heads, items = (int)gridDim.x / A.pool.heads;
+    const int item = (int)blockIdx.x / A.pool.heads;
+    const Part P = row_part(A, item);
+    if (P.seq < 0) {
+        if (A.clear_rest && A.offsets && P.block >= 0 && P.hi == 0) {
+            const int first = item - P.block;  // the number of items
+            clear_rows(A, P.block, items - first, h);
+        }
+        return;
+    }
+    const char* const block = A.pool.at(P.seq, P.block, h);
+    const int tid = threadIdx.x, token = tid >> 3, part = tid & 7, group = part >> 1;
+    const bool mine = token >= P.lo && token < P.hi;
+    const long row = ((P.row + token - P.lo) * A.pool.heads + h) * kDim + 16 * part;
+    if (!block) {
+        if (A.clear_rest && mine)
+            for (int i = 0; i < 2; ++i) {
+                reinterpret_cast<uint4*>(A.k_out + row)[i] = make_uint4(0, 0, 0, 0);
+                reinterpret_cast<uint4*>(A.v_out + row)[i] = make_uint4(0, 0, 0, 0);
+            }
+        return;
+    }
+    if (tid < 128) {
+        reinterpret_cast<uint4*>(s_v)[tid] = reinterpret_cast<const uint4*>(block + kVCodes)[tid];
+        s_vp[tid] = reinterpret_cast<const uint32_t*>(block + kVScale)[tid];
+    }
+    uint32_t out[8];
+    if (mine) {
+        const uint32_t sl = reinterpret_cast<const uint32_t*>(block + kKScale)[((token >> 4) * 4 + group) * 16 + (token & 15)];
+        const float scale = h2f((uint16_t)sl), low = h2f((uint16_t)(sl >> 16));
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+            const uint32_t d = reinterpret_cast<const uint32_t*>(block)[(((token >> 4) * 4 + 2 * (part & 1) + q) * 16 + (token & 15)) * 4 + group];
+#pragma unroll
+            for (int e = 0; e < 8; e += 2)
+                out[4 * q + e / 2] = pack_halves(__builtin_fmaf((float)((d >> nibble(e)) & 15u), scale, low),
+                                                 __builtin_fmaf((float)((d >> nibble(e + 1)) & 15u), scale, low));
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+            reinterpret_cast<uint4*>(A.k_out + row)[i] = make_uint4(out[4 * i], out[4 * i + 1], out[4 * i + 2], out[4 * i + 3]);
+    }
+    __syncthreads();
+    if (!mine) return;
+    const uint16_t* vp = reinterpret_cast<const uint16_t*>(s_vp);
+    const float scale = h2f(vp[group * kBlock + token]), low = h2f(vp[128 + group * kBlock + token]);
+    const int e = token & 7, shift = 4 * (e / 2 + 4 * (e % 2));
+    const int base = (part >> 2) * 256 + (token >> 3) * 64 + (part & 3);
+#pragma unroll
+    for (int n = 0; n < 16; n += 2)
+        out[n / 2] = pack_halves(__builtin_fmaf((float)((s_v[base + 4 * n] >> shift) & 15u), scale, low),
+                                 __builtin_fmaf((float)((s_v[base + 4 * n + 4] >> shift) & 15u), scale, low));
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+        reinterpret_cast<uint4*>(A.v_out + row)[i] = make_uint4(out[4 * i], out[4 * i + 1], out[4 * i + 2], out[4 * i + 3]);
+}
+
+// ---------------------------------------------------------------------------
+// attention of single tokens
+// ---------------------------------------------------------------------------
+
+constexpr int kWaves = 4;
+constexpr float kLog2e = 1.4426950408889634f;
+// Weights are exp2(x - m) * 2^14: the largest stays below the largest fp16 number, and a weight
+// is lost to fp16 only when it is below 2^-39 of the largest one.
+constexpr float kWeightBits = 14.0f;
+
+struct AttnArgs {
+    Pool pool;
+    const uint16_t* q;  // [B, Hq, 128]
+    const int32_t* lengths;
+    uint16_t* out;      // [B, Hq, 128]
+    float* part;        // [B * Hq, splits, 130]: o[128], m, l
+    int Hq, G, sets, splits;
+    int chunk;          // blocks per split
+    int max_length;
+    float c;            // scaling * log2(e)
+};
+constexpr int kRecord = kDim + 2;
+
+__device__ __forceinline__ float swap_sum32(float a, float b) {
+    const auto r = __builtin_amdgcn_permlane32_swap((uint32_t)f2i(a), (uint32_t)f2i(b), false, false);
+    return i2f((int)r[0]) + i2f((int)r[1]);
+}
+__device__ __forceinline__ float swap_sum16(float a, float b) {
+    const auto r = __builtin_amdgcn_permlane16_swap((uint32_t)f2i(a), (uint32_t)f2i(b), false, false);
+    return i2f((int)r[0]) + i2f((int)r[1]);
+}
+
+// The operand register pair (elements 0 .. 7) of a dword of codes: elements 0, 1, 4, 5 times
+// 2^-24 and 2, 3, 6, 7 times 2^-20.
+__device__ __forceinline__ half8_t operand(uint32_t d) {
+    const uint32_t e = d >> 8;
+    const uint4 w = make_uint4(d & 0x000F000Fu, d & 0x00F000F0u, e & 0x000F000Fu, e & 0x00F000F0u);
+    return __builtin_bit_cast(half8_t, w);
+}
+
+// One block's codes and scalings as a lane takes them.
+struct Block {
+    uint4 k[2];       // tiles of 16 tokens: token lane % 16, channels 8 (lane / 16) + [0, 8) of the four groups
+    uint32_t ks[2];   // scale and low of token lane % 16, group lane / 16
+    uint4 v[2];       // channels 16 (4 i + j) + lane % 16 (dword j), tokens 8 (lane / 16) + [0, 8)
+    uint32_t vs[4], vl[4];  // scales and lowest values of group lane % 16 / 4, tokens 8 (lane / 16) + [0, 8)
+};
+
+__device__ __forceinline__ void load_block(Block& b, const char* p, int lane) {
+    const uint4* codes = reinterpret_cast<const uint4*>(p);
+    b.k[0] = codes[lane];
+    b.k[1] = codes[64 + lane];
+    b.ks[0] = reinterpret_cast<const uint32_t*>(p + kKScale)[lane];
+    b.ks[1] = reinterpret_cast<const uint32_t*>(p + kKScale)[64 + lane];
+    const uint4* vc = reinterpret_cast<const uint4*>(p + kVCodes);
+    b.v[0] = vc[lane];
+    b.v[1] = vc[64 + lane];
+    const int at = (lane & 15) / 4 * 4 + (lane >> 4);
+    const uint4 s = reinterpret_cast<const uint4*>(p + kVScale)[at], l = reinterpret_cast<const uint4*>(p + kVLow)[at];
+    b.vs[0] = s.x, b.vs[1] = s.y, b.vs[2] = s.z, b.vs[3] = s.w;
+    b.vl[0] = l.x, b.vl[1] = l.y, b.vl[2] = l.z, b.vl[3] = l.w;
+}
+
+// One workgroup per (sequence, KV head, set of 4 HB query heads, split); its four waves take a quarter
+// of the split's blocks each and join at the end.
+//
+// Scores: D[row 4 g + h][token] += Q_g K^T over the four groups, where Q_g has group g's channels of
+// head h in row 4 g + h and zeros elsewhere, so that lane (quarter g, token n) gets the four heads' sums over
+// group g alone and applies that group's scale and lowest value (times the sum of q over the group) in fp32;
+// three lane swaps add the groups and leave head h's score of token n in lane (h, n).
+// Values: D[row 4 g + h][channel] += (P s_g) V over 32 tokens, weights times scale of group g in row
+// 4 g + h; the rows of a channel's own group are the ones that count.  The lowest values are one
+// more product, with P alone.  The product P s is relative to a power of two `e2` not below any scale so far,
+// kept like the softmax's maximum.
+template <int HB>
+__global__ void __launch_bounds__(kThreads) attention_kernel(AttnArgs A) {
+    constexpr int kHeads = 4 * HB;
+    constexpr int kPitch = kBlock + 8;
+    __shared__ __align__(16) uint16_t s_p[kWaves][kHeads * kPitch];
+    __shared__ float s_o[kWaves][kHeads][kDim];
+    __shared__ float s_m[kWaves][kHeads], s_l[kWaves][kHeads];
+    const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, quarter = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    int w = blockIdx.x;
+    const int set = w % A.sets;
+    w /= A.sets;
+    const int hk = w % A.pool.heads;
+    w /= A.pool.heads;
+    const int split = w % A.splits, b = w / A.splits;
+    const int h0 = set * kHeads;                    // first query head of the set within the KV head
+    const int heads = min(kHeads, A.G - h0);
+    const long row0 = (long)b * A.Hq + hk * A.G + h0;
+    const int length = min(max(A.lengths[b], 0), A.max_length);
+    const int blocks = (length + kBlock - 1) / kBlock;
+    const int first = split * A.chunk, count = min(A.chunk, blocks - first);
+    if (count <= 0 && A.splits > 1) return;  // the merge looks at the sequence's own splits only
+    const int share = count > 0 ? (count + kWaves - 1) / kWaves : 0;
+    const int begin = first + wave * share, end = min(begin + share, first + count);
+
+    // Q: lane (n = 4 g + h, quarter): channels 32 g + 8 quarter + [0, 8) of head h, brought to a common power
+    // of two so that the sixteenth of an element keeps its bits
+    half8_t qa[HB][4];
+    float qs[HB][4], c24;
+    {
+        const int g = n >> 2;
+        float x[HB][8], top = 0.0f, sum[HB];
+#pragma unroll
+        for (int hb = 0; hb < HB; ++hb) {
+            const int h = 4 * hb + (n & 3);
+            uint4 r = {};
+            if (h < heads) r = reinterpret_cast<const uint4*>(A.q + (row0 + h) * kDim)[4 * g + quarter];
+            const uint32_t words[4] = {r.x, r.y, r.z, r.w};
+            sum[hb] = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                x[hb][e] = h2f((uint16_t)(words[e >> 1] >> (16 * (e & 1))));
+                top = fmaxf(top, fabsf(x[hb][e]));
+                sum[hb] += x[hb][e];
+            }
+            sum[hb] += __shfl_xor(sum[hb], 16);
+            sum[hb] += __shfl_xor(sum[hb], 32);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) qs[hb][i] = __shfl(sum[hb], 4 * quarter + i) * A.c;
+        }
+        top = wave_max(top);
+        // 2^e with top * 2^e in [2^11, 2^12); 1 where there is nothing to scale, or no number
+        const float up = top > 0.0f && top < INFINITY ? ldexpf(1.0f, 11 - ilogbf(top)) : 1.0f;
+        c24 = A.c * 0x1p24f / up;
+#pragma unroll
+        for (int hb = 0; hb < HB; ++hb) {
+            half8_t mine;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) mine[e] = (_Float16)(x[hb][e] * (e & 2 ? up * 0.0625f : up));
+#pragma unroll
+            for (int gg = 0; gg < 4; ++gg)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) qa[hb][gg][e] = gg == g ? mine[e] : (_Float16)0.0f;
+        }
+    }
+
+    float4_t acc[HB][8], accl[HB];
+    float m[HB], l[HB];  // head 4 hb + quarter; l: this lane's tokens
+#pragma unroll
+    for (int hb = 0; hb < HB; ++hb) {
+        m[hb] = -__FLT_MAX__;
+        l[hb] = 0.0f;
+        accl[hb] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int nb = 0; nb < 8; ++nb) acc[hb][nb] = {0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    float e2 = 0x1p-14f;  // not below any scale so far
+
+    for (int blk = begin; blk < end; ++blk) {
+        const char* p = A.pool.at(b, blk, hk);
+        if (!p) continue;
+        Block x;
+        load_block(x, p, lane);
+        const int valid = min(kBlock, length - blk * kBlock);
+        if (valid < kBlock) {  // what lies behind the last token may be anything
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int t = 8 * quarter + 2 * i;
+                const uint32_t keep = (t < valid ? 0xFFFFu : 0u) | (t + 1 < valid ? 0xFFFF0000u : 0u);
+                x.vs[i] &= keep;
+                x.vl[i] &= keep;
+            }
+        }
+        float score[HB][2];
+#pragma unroll
+        for (int tile = 0; tile < 2; ++tile) {
+            const uint32_t kd[4] = {x.k[tile].x, x.k[tile].y, x.k[tile].z, x.k[tile].w};
+            float4_t d[HB];
+#pragma unroll
+            for (int hb = 0; hb < HB; ++hb) d[hb] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const half8_t kf = operand(kd[g]);
+#pragma unroll
+                for (int hb = 0; hb < HB; ++hb) d[hb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(qa[hb][g], kf, d[hb], 0, 0, 0);
+            }
+            const float scale = h2f((uint16_t)x.ks[tile]) * c24, low = h2f((uint16_t)(x.ks[tile] >> 16));
+#pragma unroll
+            for (int hb = 0; hb < HB; ++hb) {
+                float t[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) t[i] = __builtin_fmaf(d[hb][i], scale, low * qs[hb][i]);
+                const float s = swap_sum16(swap_sum32(t[0], t[2]), swap_sum32(t[1], t[3]));
+                score[hb][tile] = 16 * tile + n < valid ? s : -INFINITY;
+            }
+        }
+        float top_scale = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            top_scale = fmaxf(top_scale, fmaxf(h2f((uint16_t)x.vs[i]), h2f((uint16_t)(x.vs[i] >> 16))));
+        bool grow = top_scale > e2;
+#pragma unroll
+        for (int hb = 0; hb < HB; ++hb) grow |= fmaxf(score[hb][0], score[hb][1]) > m[hb];
+        if (ballot(grow) != 0) {
+            const float ts = wave_max(top_scale);
+            float shrink = 1.0f;
+            if (ts > e2) {
+                const float up = ldexpf(1.0f, ilogbf(ts) + 1);
+                shrink = e2 / up;
+                e2 = up;
+            }
+#pragma unroll
+            for (int hb = 0; hb < HB; ++hb) {
+                const float mn = fmaxf(m[hb], row_max16(fmaxf(score[hb][0], score[hb][1])));
+                const float alpha = __builtin_amdgcn_exp2f(m[hb] - mn);
+                m[hb] = mn;
+                l[hb] *= alpha;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float a = readlane(alpha, 16 * i);
+                    accl[hb][i] *= a;
+#pragma unroll
+                    for (int nb = 0; nb < 8; ++nb) acc[hb][nb][i] *= a * shrink;
+                }
+            }
+        }
+        // weights to LDS as [head][token]
+#pragma unroll
+        for (int hb = 0; hb < HB; ++hb)
+#pragma unroll
+            for (int tile = 0; tile < 2; ++tile) {
+                const float p14 = __builtin_amdgcn_exp2f(score[hb][tile] - m[hb] + kWeightBits);
+                l[hb] += p14;
+                s_p[wave][(4 * hb + quarter) * kPitch + 16 * tile + n] = f2h(p14);
+            }
+        wave_sync();
+        const _Float16 one = (_Float16)(1.0f / e2), sixteenth = (_Float16)(0.0625f / e2);
+        const half8_t factor = {one, one, sixteenth, sixteenth, one, one, sixteenth, sixteenth};
+        const half8_t vscale = __builtin_bit_cast(half8_t, make_uint4(x.vs[0], x.vs[1], x.vs[2], x.vs[3])) * factor;
+        const half8_t vlow = __builtin_bit_cast(half8_t, make_uint4(x.vl[0], x.vl[1], x.vl[2], x.vl[3]));
+        half8_t ps[HB];
+#pragma unroll
+        for (int hb = 0; hb < HB; ++hb) {
+            const half8_t pw = *reinterpret_cast<const half8_t*>(&s_p[wave][(4 * hb + (n & 3)) * kPitch + 8 * quarter]);
+            accl[hb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(pw, vlow, accl[hb], 0, 0, 0);
+            ps[hb] = pw * vscale;
+        }
+#pragma unroll
+        for (int nb = 0; nb < 8; ++nb) {
+            const uint4& q4 = x.v[nb >> 2];
+            const half8_t vf = operand((nb & 3) == 0 ? q4.x : (nb & 3) == 1 ? q4.y : (nb & 3) == 2 ? q4.z : q4.w);
+#pragma unroll
+            for (int hb = 0; hb < HB; ++hb) acc[hb][nb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ps[hb], vf, acc[hb][nb], 0, 0, 0);
+        }
+        wave_sync();
+    }
+
+    // lane (quarter g, n): channels 32 g + n and 32 g + 16 + n of the four heads
+    const float back = e2 * 0x1p24f;
+#pragma unroll
+    for (int hb = 0; hb < HB; ++hb) {
+        const float total = row_sum16(l[hb]);
+        if (n == 0) {
+            s_m[wave][4 * hb + quarter] = m[hb];
+            s_l[wave][4 * hb + quarter] = total;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float lows = __shfl(accl[hb][i], 16 * quarter + 4 * quarter);  // row 4 g + i, column of group g
+#pragma unroll
+            for (int g = 0; g < 4; ++g)
+                if (g == quarter)
+#pragma unroll
+                    for (int half = 0; half < 2; ++half)
+                        s_o[wave][4 * hb + i][32 * g + 16 * half + n] = __builtin_fmaf(acc[hb][2 * g + half][i], back, lows);
+        }
+    }
+    __syncthreads();
+    for (int e = tid; e < heads * kDim; e += kThreads) {
+        const int h = e / kDim, ch = e % kDim;
+        float top = s_m[0][h];
+#pragma unroll
+        for (int i = 1; i < kWaves; ++i) top = fmaxf(top, s_m[i][h]);
+        float o = 0.0f, total = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kWaves; ++i) {
+            if (s_l[i][h] == 0.0f) continue;  // no tokens (a NaN goes on)
+            const float a = __builtin_amdgcn_exp2f(s_m[i][h] - top);
+            o += a * s_o[i][h][ch];
+            total += a * s_l[i][h];
+        }
+        if (A.splits == 1) {
+            A.out[(row0 + h) * kDim + ch] = f2h(total == 0.0f ? 0.0f : o / total);
+        } else {
+            float* rec = A.part + ((row0 + h) * A.splits + split) * kRecord;
+            rec[ch] = o;
+            if (ch == 0) {
+                rec[kDim] = top;
+                rec[kDim + 1] = total;
+            }
+        }
+    }
+}
+
+// Joins the splits of a query head: one workgroup of 128 threads, a channel each.
+__global__ void __launch_bounds__(kDim) merge_kernel(AttnArgs A) {
+    const long row = blockIdx.x;
+    const int b = (int)(row / A.Hq), ch = threadIdx.x;
+    const int length = min(max(A.lengths[b], 0), A.max_length);
+    const int blocks = (length + kBlock - 1) / kBlock;
+    const int splits = min(A.splits, (blocks + A.chunk - 1) / A.chunk);
+    const float* rec = A.part + row * A.splits * kRecord;
+    float top = -__FLT_MAX__;
+    for (int s = 0; s < splits; ++s) top = fmaxf(top, rec[s * kRecord + kDim]);
+    float o = 0.0f, total = 0.0f;
+    for (int s = 0; s < splits; ++s) {
+        const float l = rec[s * kRecord + kDim + 1];
+        if (l == 0.0f) continue;  // no tokens (a NaN goes on)
+        const float a = __builtin_amdgcn_exp2f(rec[s * kRecord + kDim] - top);
+        o += a * rec[s * kRecord + ch];
+        total += a * l;
+    }
+    A.out[row * kDim + ch] = f2h(total == 0.0f ? 0.0f : o / total);
+}
+
+// ---------------------------------------------------------------------------
+// page copies
+// ---------------------------------------------------------------------------
+
+constexpr int kPairs = 384;  // per launch: the numbers travel with the kernel's arguments
+struct CopyArgs {
+    uint4* pages;
+    long pieces;  // 16-byte pieces of a page
+    long layer;   // pieces of a pool
+    int32_t source[kPairs], target[kPairs];
+};
+constexpr int kCopyPieces = 1024;  // per workgroup
+
+__global__ void __launch_bounds__(kThreads) copy_kernel(CopyArgs A) {
+    const long at = (long)blockIdx.z * A.layer + (long)blockIdx.x * kCopyPieces + threadIdx.x;
+    const uint4* src = A.pages + A.source[blockIdx.y] * A.pieces + at;
+    uint4* dst = A.pages + A.target[blockIdx.y] * A.pieces + at;
+    const long left = A.pieces - (long)blockIdx.x * kCopyPieces - threadIdx.x;
+    uint4 r[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        if (i * kThreads < left) r[i] = src[i * kThreads];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        if (i * kThreads < left) dst[i * kThreads] = r[i];
+}
+
+// ---------------------------------------------------------------------------
+// host side
+// ---------------------------------------------------------------------------
+
+bool aligned16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
+
+bool pool_ok(const void* pages, int64_t num_pages, int page_tokens, int Hk, const int32_t* table, int width) {
+    if (!pages || !table) {
+        reskv_host::set_error("null pointer");
+        return false;
+    }
+    if (num_pages < 1 || num_pages >= (1LL << 31) || Hk < 1 || width < 1) {
+        reskv_host::set_error("bad pool sizes (pages %ld, KV heads %d, table width %d)", (long)num_pages, Hk, width);
+        return false;
+    }
+    if (page_tokens < kBlock || page_tokens % kBlock != 0 || (long)width * page_tokens >= (1L << 31)) {
+        reskv_host::set_error("a page holds a multiple of %d tokens, a sequence fewer than 2^31", kBlock);
+        return false;
+    }
+    if (!aligned16(pages)) {
+        reskv_host::set_error("pages must be 16-byte aligned");
+        return false;
+    }
+    return true;
+}
+
+Pool make_pool(const void* pages, int64_t num_pages, int page_tokens, int Hk, const int32_t* table, int width) {
+    return Pool{(char*)pages, table, (long)num_pages, page_tokens / kBlock, width, Hk};
+}
+
+// Blocks that N rows of S sequences can touch: a sequence of n rows touches at most n / 32 + 2.
+long row_items(const int32_t* offsets, int S, long N) { return offsets ? N / kBlock + 2L * S + 1 : (long)S; }
+
+// How many splits, and how many blocks each: about four workgroups for every CU, and no fewer
+// than four blocks (one for each wave).
+struct Split {
+    int splits, chunk;
+};
+constexpr int kTargetGroups = 1024;
+int head_sets(int G) { return G <= 4 ? 1 : (G + 7) / 8; }
+Split choose_split(int B, int Hk, int G, long max_length) {
+    const long blocks = max_length <= 0 ? 1 : (max_length + kBlock - 1) / kBlock;
+    const long groups = (long)B * Hk * head_sets(G);
+    long splits = (kTargetGroups + groups - 1) / groups;
+    if (splits > (blocks + kWaves - 1) / kWaves) splits = (blocks + kWaves - 1) / kWaves;
+    if (splits < 1) splits = 1;
+    const long chunk = (blocks + splits - 1) / splits;
+    return Split{(int)((blocks + chunk - 1) / chunk), (int)chunk};
+}
+
+}  // namespace
+
+extern "C" int reskv_int4_append(void* pages, int64_t num_pages, int page_tokens, int Hk, const int32_t* table,
+                                 int table_width, int S, const int32_t* starts, const int32_t* offsets, const void* k,
+                                 const void* v, int64_t N, const int64_t* strides, void* stream) {
+    RESKV_REQUIRE(starts && k && v && strides, "null pointer");
+    if (!pool_ok(pages, num_pages, page_tokens, Hk, table, table_width)) return 1;
+    RESKV_REQUIRE(S > 0 && N > 0 && N < (1LL << 30) && (offsets || N == S), "bad sizes (sequences %d, rows %ld)", S, (long)N);
+    RESKV_REQUIRE(aligned16(k) && aligned16(v), "rows must be 16-byte aligned");
+    for (int i = 0; i < 4; ++i) RESKV_REQUIRE(strides[i] >= 0 && strides[i] % 8 == 0, "rows must be 16-byte aligned");
+    const long items = row_items(offsets, S, N) * Hk;
+    RESKV_REQUIRE(items < (1L << 31), "too many rows");
+    RowArgs A{};
+    A.pool = make_pool(pages, num_pages, page_tokens, Hk, table, table_width);
+    A.starts = starts;
+    A.offsets = offsets;
+    A.k = (const uint16_t*)k;
+    A.v = (const uint16_t*)v;
+    A.k_token = strides[0];
+    A.k_head = strides[1];
+    A.v_token = strides[2];
+    A.v_head = strides[3];
+    A.sequences = S;
+    A.N = (int)N;
+    hipLaunchKernelGGL(append_kernel, dim3((unsigned)items), dim3(kThreads), 0, (hipStream_t)stream, A);
+    return reskv_host::check_launch("append_kernel");
+}
+
+extern "C" int reskv_int4_gather(const void* pages, int64_t num_pages, int page_tokens, int Hk, const int32_t* table,
+                                 int table_width, int S, const int32_t* starts, const int32_t* offsets, void* k_out,
+                                 void* v_out, int64_t N, int clear_rest, void* stream) {
+    RESKV_REQUIRE(starts && k_out && v_out, "null pointer");
+    if (!pool_ok(pages, num_pages, page_tokens, Hk, table, table_width)) return 1;
+    RESKV_REQUIRE(S > 0 && N > 0 && N < (1LL << 30) && (offsets || N == S), "bad sizes (sequences %d, rows %ld)", S, (long)N);
+    RESKV_REQUIRE(aligned16(k_out) && aligned16(v_out), "rows must be 16-byte aligned");
+    const long items = row_items(offsets, S, N) * Hk;
+    RESKV_REQUIRE(items < (1L << 31), "too many rows");
+    RowArgs A{};
+    A.pool = make_pool(pages, num_pages, page_tokens, Hk, table, table_width);
+    A.starts = starts;
+    A.offsets = offsets;
+    A.k_out = (uint16_t*)k_out;
+    A.v_out = (uint16_t*)v_out;
+    A.sequences = S;
+    A.N = (int)N;
+    A.clear_rest = clear_rest;
+    hipLaunchKernelGGL(gather_kernel, dim3((unsigned)items), dim3(kThreads), 0, (hipStream_t)stream, A);
+    return reskv_host::check_launch("gather_kernel");
+}
+
+extern "C" int64_t reskv_int4_workspace_bytes(int B, int Hq, int Hk, int64_t max_length) {
+    if (B < 1 || Hk < 1 || Hq < 1 || Hq % Hk != 0) return 0;
+    const Split s = choose_split(B, Hk, Hq / Hk, max_length);
+    return s.splits == 1 ? 0 : (int64_t)B * Hq * s.splits * kRecord * 4;
+}
+
+extern "C" int reskv_int4_attention(const void* q, const void* pages, int64_t num_pages, int page_tokens,
+                                    const int32_t* table, int table_width, const int32_t* lengths, int B, int Hq, int Hk,
+                                    float scaling, int64_t max_length, void* out, void* workspace, int64_t workspace_bytes,
+                                    void* stream) {
+    RESKV_REQUIRE(q && lengths && out, "null pointer");
+    if (!pool_ok(pages, num_pages, page_tokens, Hk, table, table_width)) return 1;
+    RESKV_REQUIRE(B > 0 && Hq > 0 && Hq % Hk == 0, "bad sizes (sequences %d, query heads %d, KV heads %d)", B, Hq, Hk);
+    RESKV_REQUIRE(max_length >= 0, "max_length must not be negative");
+    RESKV_REQUIRE(aligned16(q) && aligned16(out), "q and out must be 16-byte aligned");
+    const long most = (long)table_width * page_tokens;
+    if (max_length > most) max_length = most;
+    const int G = Hq / Hk;
+    const Split s = choose_split(B, Hk, G, max_length);
+    RESKV_REQUIRE(s.splits == 1 || (workspace && workspace_bytes >= reskv_int4_workspace_bytes(B, Hq, Hk, max_length)),
+                  "the workspace is too small");
+    AttnArgs A{};
+    A.pool = make_pool(pages, num_pages, page_tokens, Hk, table, table_width);
+    A.q = (const uint16_t*)q;
+    A.lengths = lengths;
+    A.out = (uint16_t*)out;
+    A.part = (float*)workspace;
+    A.Hq = Hq;
+    A.G = G;
+    A.sets = head_sets(G);
+    A.splits = s.splits;
+    A.chunk = s.chunk;
+    A.max_length = (int)max_length;
+    A.c = scaling * kLog2e;
+    const long groups = (long)B * Hk * A.sets * s.splits;
+    RESKV_REQUIRE(groups < (1L << 31) && (long)B * Hq < (1L << 31), "too many (sequence, head) rows");
+    hipLaunchKernelGGL(G <= 4 ? attention_kernel<1> : attention_kernel<2>, dim3((unsigned)groups), dim3(kThreads), 0,
+                       (hipStream_t)stream, A);
+    if (reskv_host::check_launch("int4 attention_kernel")) return 1;
+    if (s.splits == 1) return 0;
+    hipLaunchKernelGGL(merge_kernel, dim3((unsigned)(B * Hq)), dim3(kDim), 0, (hipStream_t)stream, A);
+    return reskv_host::check_launch("int4 merge_kernel");
+}
+
+extern "C" int reskv_copy_pages(void* pages, int layers, int64_t num_pages, int64_t page_bytes, const int32_t* source,
+                                const int32_t* target, int n, void* stream) {
+    RESKV_REQUIRE(pages && source && target, "null pointer");
+    RESKV_REQUIRE(layers > 0 && layers < (1 << 16) && num_pages > 0 && n >= 0 && page_bytes > 0 && page_bytes % 16 == 0,
+                  "bad pool sizes (layers %d, pages %ld of %ld bytes)", layers, (long)num_pages, (long)page_bytes);
+    RESKV_REQUIRE(aligned16(pages), "pages must be 16-byte aligned");
+    for (int i = 0; i < n; ++i)
+        RESKV_REQUIRE(source[i] >= 0 && source[i] < num_pages && target[i] >= 0 && target[i] < num_pages,
+                      "page pair %d (%d to %d) is outside the pool of %ld", i, source[i], target[i], (long)num_pages);
+    CopyArgs A;
+    A.pages = (uint4*)pages;
+    A.pieces = page_bytes / 16;
+    A.layer = A.pieces * num_pages;
+    const long groups = (A.pieces + kCopyPieces - 1) / kCopyPieces;
+    RESKV_REQUIRE(groups < (1L << 31), "pages are too large");
+    for (int first = 0; first < n; first += kPairs) {
+        const int count = n - first < kPairs ? n - first : kPairs;
+        for (int i = 0; i < count; ++i) {
+            A.source[i] = source[first + i];
+            A.target[i] = target[first + i];
+        }
+        hipLaunchKernelGGL(copy_kernel, dim3((unsigned)groups, (unsigned)count, (unsigned)layers), dim3(kThreads), 0,
+                           (hipStream_t)stream, A);
+        if (reskv_host::check_launch("copy_kernel")) return 1;
+    }
+    return 0;
+}

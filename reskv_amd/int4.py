@@ -1,0 +1,188 @@
+"""Paged cache of 4-bit keys and values, and the operators on its pages.
+
+A pool is a uint8 tensor [pages, KV heads, bytes] (``empty_pages``; 160 bytes per token and head, K and V
+together, against 512 in fp16); a sequence's tokens lie in the pages that its row of an
+int32 page table names.  Every row of 128 channels is quantised in groups of 32: ``low`` is
+the group's smallest value and ``scale`` a fifteenth of its range, both fp16, and a channel is stored as the
+nearest of the sixteen values ``code * scale + low``.
+
+* ``int4_append`` puts rows of K and V into pages, prompts and single tokens alike;
+* ``int4_gather`` gives them back in fp16, for a prompt that continues on cached tokens;
+* ``int4_attention`` attends one token of every sequence over its pages;
+* ``copy_pages`` copies pages in every layer's pool at once;
+* ``Int4Cache`` keeps the pages of a decoder stack: which sequence has which, forks that share
+  them, their release and compaction.
+
+K is stored as it is given: rotated keys, as the dense ring of ``ResKVLayerCache`` has them.
+Like ``attention`` these are inference operators: no gradient is recorded.  Page tables, positions and
+lengths stay on the GPU and are not read on the host: a page number outside the pool, or a position outside
+the table, stands for a token that is not there, which appends leave out and reads pass over.
+"""
+
+import ctypes
+
+import torch
+
+from . import _lib
+from ._extension import _require, _workspace
+from .packed import _int32, _kernel_rows, _launch, _rows, _same_gpu
+
+BLOCK_TOKENS = 32
+TOKEN_BYTES = 160  # of one KV head, K and V
+
+_STRIDES = ctypes.c_int64 * 4
+
+
+def _page_bytes(page_tokens):
+    page_tokens = int(page_tokens)
+    _require(page_tokens >= BLOCK_TOKENS and page_tokens % BLOCK_TOKENS == 0,
+             f"a page must hold a positive multiple of {BLOCK_TOKENS} tokens")
+    return page_tokens * TOKEN_BYTES
+
+
+def empty_pages(pages, kv_heads, page_tokens=64, layers=None, device="cuda"):
+    """A pool of unused pages: uint8 [pages, kv_heads, bytes], or [layers, pages, kv_heads, bytes]."""
+    shape = (int(pages), int(kv_heads), _page_bytes(page_tokens))
+    _require(shape[0] > 0 and shape[1] > 0, "a pool needs pages and KV heads")
+    return torch.zeros(shape if layers is None else (int(layers), *shape), dtype=torch.uint8, device=device)
+
+
+def _pool(pages):
+    """(pages, tokens per page, KV heads) of a pool."""
+    _require(pages.dtype == torch.uint8 and pages.dim() == 3 and pages.is_contiguous(),
+             "pages must be a contiguous uint8 tensor [pages, KV heads, bytes]")
+    count, heads, nbytes = pages.shape
+    _require(count > 0 and heads > 0 and nbytes > 0 and nbytes % (BLOCK_TOKENS * TOKEN_BYTES) == 0,
+             f"a page must hold a positive multiple of {BLOCK_TOKENS} tokens of {TOKEN_BYTES} bytes")
+    return count, nbytes // TOKEN_BYTES, heads
+
+
+def _table(table):
+    _require(table.dtype == torch.int32 and table.dim() == 2 and table.is_contiguous() and table.shape[1] > 0,
+             "table must be a contiguous int32 matrix [sequences, pages]")
+    return table.shape
+
+
+@torch.no_grad()
+def int4_append(pages, table, starts, k, v, offsets=None):
+    """Quantises rows of k and v, fp16 [N, Hk, 128] (any strides with unit channel stride), into pages.
+
+    Without ``offsets``, row s becomes token ``starts[s]`` of sequence s (a decode step); with them
+    (int32 [S + 1]), row ``offsets[s] + i`` becomes token ``starts[s] + i``.  ``starts`` is int32 [S], ``table`` int32 [S,
+    pages of a sequence].  Tokens of a block before and behind the new ones keep their values.  A group of
+    channels that holds a NaN or an infinity reads as NaN.  No two sequences of a call may write to one page.
+    """
+    count, tokens, heads = _pool(pages)
+    sequences, width = _table(table)
+    _int32("starts", starts, sequences)
+    _rows("k", k, heads)
+    _rows("v", v, heads)
+    n = k.shape[0]
+    _require(v.shape[0] == n, "k and v must have the same number of rows")
+    if offsets is None:
+        _require(n == sequences, "without offsets there must be one row for every sequence")
+    else:
+        _int32("offsets", offsets, sequences + 1)
+    dev = _same_gpu(pages, table, starts, k, v, offsets)
+    if n == 0 or sequences == 0:
+        return
+    k, v = _kernel_rows(k), _kernel_rows(v)
+    _launch("reskv_int4_append", dev, pages.data_ptr(), count, tokens, heads, table.data_ptr(), width, sequences,
+            starts.data_ptr(), None if offsets is None else offsets.data_ptr(), k.data_ptr(), v.data_ptr(), n,
+            _STRIDES(*k.stride()[:2], *v.stride()[:2]))
+
+
+@torch.no_grad()
+def int4_gather(pages, table, starts, offsets, rows, out=None):
+    """The stored values of tokens, as (k, v) fp16 [rows, Hk, 128]: row ``offsets[s] + i`` is token
+    ``starts[s] + i`` of sequence s (``rows`` is what ``offsets`` ends with; the host does not read it).
+
+    ``out`` = (k, v) to write to, contiguous; rows of no token are zero, or left as they are in ``out``.
+    """
+    count, tokens, heads = _pool(pages)
+    sequences, width = _table(table)
+    _int32("starts", starts, sequences)
+    _int32("offsets", offsets, sequences + 1)
+    rows = int(rows)
+    _require(rows >= 0, "rows must not be negative")
+    clear = out is None
+    if not clear:
+        for name, t in zip(("out k", "out v"), out):
+            _rows(name, t, heads)
+            _require(t.shape[0] == rows and t.is_contiguous(), f"{name} must be contiguous and have {rows} rows")
+    k, v = (None, None) if clear else out
+    dev = _same_gpu(pages, table, starts, offsets, k, v)
+    if clear:
+        k, v = (torch.empty((rows, heads, 128), dtype=torch.float16, device=dev) for _ in range(2))
+    if rows == 0:
+        return k, v
+    if sequences == 0:
+        return (k.zero_(), v.zero_()) if clear else (k, v)
+    _launch("reskv_int4_gather", dev, pages.data_ptr(), count, tokens, heads, table.data_ptr(), width, sequences,
+            starts.data_ptr(), offsets.data_ptr(), k.data_ptr(), v.data_ptr(), rows, int(clear))
+    return k, v
+
+
+@torch.no_grad()
+def int4_attention(q, pages, table, lengths, *, scaling=None, max_length=None, out=None):
+    """Attention of one token of every sequence: q fp16 [B, Hq, 128] (rotated) against the first
+    ``lengths[b]`` (int32 [B]) tokens of sequence b; fp16 [B, Hq, 128], ``out`` when given (contiguous).
+
+    Hq is any multiple of the pool's KV heads.  A sequence without tokens gives zeros.  ``max_length`` bounds
+    the lengths (default: what the table can hold; a longer length is cut to it) and steers how the work
+    is split over the GPU.  Scores, softmax and sums are fp32; the weights are rounded to fp16 for the
+    product with V.
+    """
+    count, tokens, kv_heads = _pool(pages)
+    sequences, width = _table(table)
+    _int32("lengths", lengths, sequences)
+    _rows("q", q)
+    heads = q.shape[1]
+    _require(q.shape[0] == sequences, "q must have one row for every sequence")
+    _require(heads > 0 and heads % kv_heads == 0, "the query heads must be a multiple of the KV heads")
+    scaling = 128 ** -0.5 if scaling is None else float(scaling)
+    _require(-float("inf") < scaling < float("inf"), "scaling must be finite")
+    most = width * tokens if max_length is None else int(max_length)
+    _require(most >= 0, "max_length must not be negative")
+    if out is not None:
+        _rows("out", out, heads)
+        _require(out.shape[0] == sequences and out.is_contiguous(), "out must be contiguous and shaped like q")
+    dev = _same_gpu(q, pages, table, lengths, out)
+    if out is None:
+        out = torch.empty((sequences, heads, 128), dtype=torch.float16, device=dev)
+    if sequences == 0:
+        return out
+    q = q if q.is_contiguous() and q.data_ptr() % 16 == 0 else q.clone(memory_format=torch.contiguous_format)
+    most = min(most, width * tokens)
+    nbytes = _lib.lib().reskv_int4_workspace_bytes(sequences, heads, kv_heads, most)
+    work = _workspace(nbytes, dev) if nbytes else None
+    _launch("reskv_int4_attention", dev, q.data_ptr(), pages.data_ptr(), count, tokens, table.data_ptr(), width,
+            lengths.data_ptr(), sequences, heads, kv_heads, scaling, most, out.data_ptr(),
+            None if work is None else work.data_ptr(), nbytes)
+    return out
+
+
+@torch.no_grad()
+def copy_pages(pages, source, target):
+    """Copies page ``source[i]`` to page ``target[i]`` (host sequences of page numbers) in a pool [pages, ...]
+    or in every layer's pool [layers, pages, KV heads, bytes], in one launch per 384 pages.
+
+    A target may be neither a source nor named twice: what it would hold then depends on the order.
+    """
+    _require(pages.dtype == torch.uint8 and pages.dim() in (3, 4) and pages.is_contiguous(),
+             "pages must be a contiguous uint8 tensor [pages, KV heads, bytes] or [layers, pages, KV heads, bytes]")
+    source, target = [int(p) for p in source], [int(p) for p in target]
+    _require(len(source) == len(target), "every source page needs a target page")
+    layers, count = (1, pages.shape[0]) if pages.dim() == 3 else pages.shape[:2]
+    nbytes = pages.shape[-2] * pages.shape[-1]
+    _require(nbytes > 0 and nbytes % 16 == 0, "a page must be a multiple of 16 bytes")
+    _require(all(0 <= p < count for p in source) and all(0 <= p < count for p in target),
+             f"page numbers must be in 0 .. {count - 1}")
+    _require(len(set(target)) == len(target) and not set(target) & set(source),
+             "a target page may be neither a source nor named twice")
+    dev = _same_gpu(pages)
+    n = len(source)
+    if n == 0 or layers == 0:
+        return
+    pairs = ctypes.c_int32 * n
+    _launch("reskv_copy_pages", dev, pages.data_ptr(), layers, count, nbytes, pairs(*source), pairs(*target), n)

@@ -11,7 +11,8 @@ first use of an operator.
 from .config import KernelPlan, ResKVKernelConfig
 
 __version__ = "0.1.0"
-__all__ = ["ResKVKernelConfig", "KernelPlan", "ResKVForCausalLM", "compress", "attention", "packed_attention"]
+__all__ = ["ResKVKernelConfig", "KernelPlan", "ResKVForCausalLM", "compress", "attention", "packed_attention",
+           "Int4Cache"]
 
 
 def __getattr__(name):
@@ -27,6 +28,10 @@ def __getattr__(name):
         from .packed import packed_attention
 
         return packed_attention
+    if name == "Int4Cache":
+        from .int4 import Int4Cache
+
+        return Int4Cache
     if name == "ResKVForCausalLM":
         from .models.llama import ResKVForCausalLM
 

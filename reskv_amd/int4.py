@@ -186,3 +186,186 @@ def copy_pages(pages, source, target):
         return
     pairs = ctypes.c_int32 * n
     _launch("reskv_copy_pages", dev, pages.data_ptr(), layers, count, nbytes, pairs(*source), pairs(*target), n)
+
+
+class Int4Cache:
+    """Paged 4-bit K/V cache of a decoder stack: ``sequences`` rows of up to ``max_length`` tokens over one pool
+    of pages per layer, with one page table for all layers.
+
+    A step reserves its tokens once, then every layer appends and attends::
+
+        cache.reserve(1)                       # or one count per sequence
+        for layer in range(layers):
+            cache.append(layer, k, v)          # rotated K, V [sequences, Hk, 128]
+            out = cache.attend(layer, q)       # rotated Q [sequences, Hq, 128]
+
+    Which page belongs to whom is kept on the host; ``table``, ``starts`` (of the reserved tokens) and
+    ``lengths`` (with them) are its copies on the GPU, at fixed addresses.  Sequences that were forked
+    share pages; ``reserve`` gives a sequence a copy of its last page before it writes to a shared one.
+    """
+
+    def __init__(self, layers, kv_heads, sequences, max_length, *, page_tokens=64, pages=None, device="cuda"):
+        _require(int(layers) > 0 and int(sequences) > 0 and int(max_length) > 0,
+                 "a cache needs layers, sequences and a length")
+        _page_bytes(page_tokens)
+        self.page_tokens, self.max_length = int(page_tokens), int(max_length)
+        width = -(-self.max_length // self.page_tokens)
+        self.pool = empty_pages(int(sequences) * width if pages is None else pages, kv_heads, page_tokens, layers, device)
+        self._table = torch.full((int(sequences), width), -1, dtype=torch.int32)
+        self.table = self._table.to(device, copy=True)
+        self.starts = torch.zeros(int(sequences), dtype=torch.int32, device=device)
+        self.lengths = torch.zeros_like(self.starts)
+        self._pages = [[] for _ in range(int(sequences))]
+        self._lengths = [0] * int(sequences)
+        self._counts = [0] * int(sequences)          # tokens reserved last
+        self._users = [0] * self.pool.shape[1]       # sequences that have a page
+        self._free = list(range(self.pool.shape[1] - 1, -1, -1))  # the lowest number last
+
+    # -- state ---------------------------------------------------------------
+    @property
+    def sequences(self) -> int:
+        return len(self._lengths)
+
+    @property
+    def free_pages(self) -> int:
+        return len(self._free)
+
+    def get_seq_length(self, sequence=0) -> int:
+        return self._lengths[sequence]
+
+    def _row(self, sequence):
+        _require(0 <= int(sequence) < self.sequences, f"sequence {sequence} is not in 0 .. {self.sequences - 1}")
+        return int(sequence)
+
+    def _publish(self, rows):
+        """The page table's changed rows, to the GPU."""
+        for s in rows:
+            self._table[s] = -1
+            self._table[s, : len(self._pages[s])] = torch.tensor(self._pages[s], dtype=torch.int32)
+        if rows:
+            self.table.copy_(self._table)
+
+    def _publish_lengths(self):
+        starts = [n - c for n, c in zip(self._lengths, self._counts)]
+        both = torch.tensor([starts, self._lengths], dtype=torch.int32).to(self.lengths.device)
+        self.starts.copy_(both[0])
+        self.lengths.copy_(both[1])
+
+    def _drop(self, pages):
+        freed = False
+        for p in pages:
+            self._users[p] -= 1
+            if self._users[p] == 0:
+                self._free.append(p)
+                freed = True
+        if freed:
+            self._free.sort(reverse=True)
+
+    # -- tokens ----------------------------------------------------------------
+    def reserve(self, counts):
+        """Makes room for ``counts`` more tokens (one number for every sequence, or one for each); the
+        appends that follow fill it.  Raises before any change when a sequence would pass
+        ``max_length`` or the pool has too few free pages."""
+        same = isinstance(counts, int)
+        counts = [counts] * self.sequences if same else [int(c) for c in counts]
+        _require(len(counts) == self.sequences and min(counts) >= 0, "reserve needs a count of tokens for every sequence")
+        ends = [n + c for n, c in zip(self._lengths, counts)]
+        _require(max(ends) <= self.max_length, f"a sequence would pass {self.max_length} tokens")
+        size, need, shared, users = self.page_tokens, 0, [], {}
+        for s, (n, c) in enumerate(zip(self._lengths, counts)):
+            need += -(-ends[s] // size) - len(self._pages[s])
+            if c and n % size:  # writes to its last page
+                last = self._pages[s][-1]
+                left = users.get(last, self._users[last])
+                if left > 1:  # of those who share it, the last one keeps it
+                    shared.append(s)
+                    users[last] = left - 1
+        need += len(shared)
+        _require(need <= len(self._free), f"{need} pages are needed and {len(self._free)} are free")
+        if shared:
+            source = [self._pages[s][-1] for s in shared]
+            target = [self._free.pop() for _ in shared]
+            copy_pages(self.pool, source, target)
+            for s, a, b in zip(shared, source, target):
+                self._users[a] -= 1
+                self._users[b] = 1
+                self._pages[s][-1] = b
+        changed = set(shared)
+        for s, end in enumerate(ends):
+            while len(self._pages[s]) * size < end:
+                p = self._free.pop()
+                self._users[p] = 1
+                self._pages[s].append(p)
+                changed.add(s)
+        self._publish(sorted(changed))
+        self._lengths, self._counts = ends, counts
+        if same:
+            self.starts.copy_(self.lengths)
+            self.lengths.add_(counts[0])
+        else:
+            self._publish_lengths()
+
+    def append(self, layer, k, v, offsets=None):
+        """The reserved tokens of one layer (``int4_append``): one row per sequence, or rows packed by ``offsets``."""
+        int4_append(self.pool[layer], self.table, self.starts, k, v, offsets)
+
+    def attend(self, layer, q, *, scaling=None, out=None):
+        """Attention of one token per sequence over all its tokens (``int4_attention``)."""
+        return int4_attention(q, self.pool[layer], self.table, self.lengths, scaling=scaling,
+                              max_length=max(self._lengths), out=out)
+
+    def gather(self, layer):
+        """(k, v, offsets): the stored values of all tokens, packed (``int4_gather``), as
+        ``packed_attention`` takes them for a prompt that continues."""
+        ends = torch.tensor([0, *self._lengths], dtype=torch.int64).cumsum(0)
+        offsets = ends.to(torch.int32).to(self.table.device)
+        k, v = int4_gather(self.pool[layer], self.table, torch.zeros_like(self.starts), offsets, int(ends[-1]))
+        return k, v, offsets
+
+    # -- sequences ---------------------------------------------------------------
+    def reorder(self, index):
+        """Row i takes the tokens of row ``index[i]`` (beams): pages are shared, not copied."""
+        index = [self._row(s) for s in (index.tolist() if torch.is_tensor(index) else index)]
+        _require(len(index) == self.sequences, "reorder needs a row for every sequence")
+        pages = [list(self._pages[s]) for s in index]
+        for row in pages:
+            for p in row:
+                self._users[p] += 1
+        old, self._pages = self._pages, pages
+        self._drop(p for row in old for p in row)
+        self._lengths = [self._lengths[s] for s in index]
+        self._counts = [self._counts[s] for s in index]
+        self._publish(list(range(self.sequences)))
+        self._publish_lengths()
+
+    def fork(self, source, target):
+        """Row ``target`` gives up its tokens and shares those of row ``source``."""
+        index = list(range(self.sequences))
+        index[self._row(target)] = self._row(source)
+        self.reorder(index)
+
+    def release(self, sequence):
+        """Row ``sequence`` gives up its tokens; pages that no other row shares are free again."""
+        s = self._row(sequence)
+        pages, self._pages[s] = self._pages[s], []
+        self._lengths[s] = self._counts[s] = 0
+        self._drop(pages)
+        self._publish([s])
+        self._publish_lengths()
+
+    def compact(self):
+        """Moves pages in use to the lowest numbers, so that the rest of the pool is free in one piece;
+        returns how many were moved."""
+        used = len(self._users) - len(self._free)
+        source = [p for p in range(used, len(self._users)) if self._users[p]]
+        target = [p for p in range(used) if not self._users[p]]
+        copy_pages(self.pool, source, target)
+        move = dict(zip(source, target))
+        for s, t in move.items():
+            self._users[t], self._users[s] = self._users[s], 0
+        self._free = [p for p in range(len(self._users) - 1, -1, -1) if not self._users[p]]
+        changed = [s for s, row in enumerate(self._pages) if any(p in move for p in row)]
+        for s in changed:
+            self._pages[s] = [move.get(p, p) for p in self._pages[s]]
+        self._publish(changed)
+        return len(source)

@@ -35,6 +35,8 @@ from . import _lib
 from ._extension import dense_decode, eager
 from .cache import ResKVLayerCache
 from .config import ResKVKernelConfig
+from .int4 import Int4Cache
+from .packed import packed_attention
 
 
 @dataclass(frozen=True)
@@ -265,17 +267,22 @@ class RandomLlama:
                 and all(w.dtype == torch.float16 and w.is_contiguous() and w.data_ptr() % 16 == 0
                         for p in self.layers for w in (p["n1"], p["n2"])))
 
-    def _layer_fused(self, li, p, x, cos, sin, sink, rows=16384):
+    def _layer_fused(self, li, p, x, cos, sin, sink, rows=16384, packed=None):
         """One layer of the prompt in place on x [B, T, hidden]: the norms, the split and
         rotation, attention and the activation are single launches, and the residual adds
-        ride in the projections (one rounding of x + y)."""
+        ride in the projections (one rounding of x + y).  With ``packed`` = (offsets,
+        longest), x [1, N, hidden] is sequences of different lengths."""
         s = self.shape
         b, t, _ = x.shape
         flat = x.view(b * t, s.hidden)
         h = fused_rmsnorm(flat, p["n1"], s.rms_eps, torch.empty_like(flat))
         qr, k, kr, v = fused_prefill_split(F.linear(h, p["wqkv"]), cos, sin, b, s.heads, s.kv_heads)
         sink(li, k, kr, v)
-        attn = fused_prefill_attention(qr, kr, v, self.scaling)
+        if packed is None:
+            attn = fused_prefill_attention(qr, kr, v, self.scaling)
+        else:
+            attn = packed_attention(*(y[0].transpose(0, 1) for y in (qr, kr, v)), packed[0], scaling=self.scaling,
+                                    max_keys=packed[1])
         del qr, k, kr, v
         flat.addmm_(attn.view(b * t, s.hidden), p["wo"].t())
         del attn
@@ -333,14 +340,44 @@ class RandomLlama:
         return out if logits else torch.argmax(out, dim=-1)
 
 
+    @torch.no_grad()
+    def prefill_packed(self, ids, lengths, sink, logits=False):
+        """``prefill`` of prompts of different lengths: ids [N] one prompt behind the other,
+        ``lengths`` their token counts (host numbers, at least 1, N in all).  ``sink(layer, raw_k,
+        rot_k, v)`` receives [1, Hk, N, 128]; returns the next token of each prompt [S]
+        (or, with ``logits``, its last position's logits [S, vocab])."""
+        s = self.shape
+        lengths = [int(n) for n in lengths]
+        _need(ids.dim() == 1 and len(lengths) > 0 and min(lengths) >= 1 and sum(lengths) == ids.shape[0],
+              "ids must be a vector of the prompts' tokens, lengths their counts (at least 1)")
+        if not self._fused(max(lengths)):
+            held, rows = [[] for _ in self.layers], []
+            for part in torch.split(ids, lengths):
+                rows.append(self.prefill(part[None], lambda li, *kv: held[li].append(kv), logits=logits))
+            for li, parts in enumerate(held):
+                sink(li, *(torch.cat(y, dim=2) for y in zip(*parts)))
+            return torch.cat(rows)
+        ends = torch.tensor([0, *lengths]).cumsum(0)
+        offsets = ends.to(torch.int32).to(self.device)
+        pos = torch.cat([torch.arange(n) for n in lengths]).to(self.device)
+        cos, sin = (y[pos] for y in self.rope_tables(max(lengths)))
+        x = self.embed[ids][None]  # [1, N, hidden]
+        for li, p in enumerate(self.layers):
+            self._layer_fused(li, p, x, cos, sin, sink, packed=(offsets, max(lengths)))
+        last = _rmsnorm(x[0, (ends[1:] - 1).to(self.device)], self.norm, s.rms_eps)
+        out = F.linear(last, self.lm_head)
+        return out if logits else torch.argmax(out, dim=-1)
+
+
 class GreedyDecoder:
     """Batch greedy decoding, one token per sequence per step, over ResKV
-    (``mode="reskv"``) or dense fp16 (``mode="dense"``) KV caches."""
+    (``mode="reskv"``), dense fp16 (``mode="dense"``) or paged 4-bit (``mode="int4"``)
+    KV caches."""
 
     def __init__(self, model: RandomLlama, batch: int, prompt_len: int, max_new: int, mode: str,
                  kernel_config: ResKVKernelConfig | None = None):
-        if mode not in ("reskv", "dense"):
-            raise ValueError("mode must be 'reskv' or 'dense'")
+        if mode not in ("reskv", "dense", "int4"):
+            raise ValueError("mode must be 'reskv', 'dense' or 'int4'")
         s = model.shape
         dev = model.device
         self.model, self.mode, self.batch = model, mode, batch
@@ -363,6 +400,8 @@ class GreedyDecoder:
         if mode == "reskv":
             cfg = kernel_config or ResKVKernelConfig(sparsity=0.75)
             self.caches = [ResKVLayerCache(cfg) for _ in range(s.layers)]
+        elif mode == "int4":
+            self.pages = Int4Cache(s.layers, s.kv_heads, batch, self.max_pos, device=dev)
         else:
             shape = (batch, s.kv_heads, self.max_pos, s.head_dim)
             self.kc = [torch.zeros(shape, **f16) for _ in range(s.layers)]
@@ -375,6 +414,12 @@ class GreedyDecoder:
         t = raw_k.shape[2]
         if self.mode == "reskv":
             self.caches[layer].update(rot_k, v, {"raw_keys": raw_k})
+        elif self.mode == "int4":
+            if layer == 0:
+                self.pages.reserve(t)
+            ends = torch.arange(0, (self.batch + 1) * t, t, dtype=torch.int32, device=v.device)
+            rows = [y.transpose(1, 2).reshape(-1, *y.shape[1::2]) for y in (rot_k, v)]
+            self.pages.append(layer, *rows, ends)
         else:
             self.kc[layer][:, :, :t].copy_(raw_k)
             self.vc[layer][:, :, :t].copy_(v)
@@ -394,7 +439,10 @@ class GreedyDecoder:
     def _append_targets(self, li):
         """Where the pre graph appends the new token's K/V in layer li's cache: ring
         slot ``live`` (ResKV: rotated K, pre-RoPE K, V) or position ``pos`` (dense:
-        pre-RoPE K, V), read from device memory when the graph runs."""
+        pre-RoPE K, V), read from device memory when the graph runs.  The 4-bit cache
+        quantises the token beside the attention (None)."""
+        if self.mode == "int4":
+            return None
         if self.mode == "reskv":
             layer = self.caches[li]
             return layer.keys, layer.raw_keys, layer.values, self.slot_buf
@@ -464,6 +512,9 @@ class GreedyDecoder:
             layer.advance()
             layer.attend(self.q[:, :, None], self.qr[:, :, None], scaling=self.model.scaling,
                          inv_freq=self.model.inv_freq, out=self.attn)
+        elif self.mode == "int4":
+            self.pages.append(li, self.kr, self.v)
+            self.pages.attend(li, self.qr, scaling=self.model.scaling, out=self.attn)
         else:
             t = self.pos + 1
             dense_decode(self.q[:, :, None], self.kc[li][:, :, :t], self.vc[li][:, :, :t], self.model.inv_freq,
@@ -481,6 +532,8 @@ class GreedyDecoder:
         if self.graphs is None:
             self.capture()
         self._set_slots()
+        if self.mode == "int4":
+            self.pages.reserve(1)
         pre, post, head = self.graphs
         for li in range(len(pre)):
             pre[li].replay()

@@ -85,93 +85,135 @@ __device__ __forceinline__ Part row_part(const RowArgs& A, int item) {
     return {it.seq, (start >> 5) + it.index, lo, hi, (long)r.first + it.index * kBlock + lo - lead};
 }
 
-// Largest and smallest of 16 fp16 values and of the 16 of the lane next to it (which has the group's other half).
-struct Range {
-    float low, high;
-    bool finite;
+// Range of a group of 32 channels, of which this lane has 16 and the lane next to it the others.
+// `maximum` and `minimum` hand a NaN on.
+struct Group {
+    float low, scale;
+    uint16_t low16, scale16;
 };
-__device__ __forceinline__ Range group_range(const float* x) {
-    float lo = x[0], hi = x[0], sum = 0.0f;
+__device__ __forceinline__ Group group_of(const half2_t* x) {
+    half2_t lo = x[0], hi = x[0];
+#pragma unroll
+    for (int i = 1; i < 8; ++i) {
+        lo = __builtin_elementwise_minimum(lo, x[i]);
+        hi = __builtin_elementwise_maximum(hi, x[i]);
+    }
+    lo = __builtin_elementwise_minimum(lo, __builtin_bit_cast(half2_t, dpp_u<0xB1>(__builtin_bit_cast(uint32_t, lo))));
+    hi = __builtin_elementwise_maximum(hi, __builtin_bit_cast(half2_t, dpp_u<0xB1>(__builtin_bit_cast(uint32_t, hi))));
+    const float low = (float)__builtin_elementwise_minimum(lo[0], lo[1]);
+    const float high = (float)__builtin_elementwise_maximum(hi[0], hi[1]);
+    if (!(high < INFINITY && low > -INFINITY)) return {0.0f, 0.0f, 0x7E00, 0x7E00};
+    const float range = high - low;
+    float scale = range / 15.0f;
+    // a range of more than 24 bits: 64 bits hold it
+    if (high - range != low || low + range != high) scale = (float)(((double)high - (double)low) / 15.0);
+    const uint16_t scale16 = f2h(scale);
+    return {low, h2f(scale16), f2h(low), scale16};
+}
+
+// The codes of 16 values: exactly rint((x - low) / scale), at most 15.  The product with the
+// reciprocal is within 2^-17 of the quotient (four roundings of 2^-23 at most, of a number below 2^5;
+// larger ones become 15); where it is nearer than 2^-16 to a half, 64 bits decide, which hold both sides
+// exactly.  That is one value in 2^15.
+__device__ __forceinline__ void codes_of(const half2_t* x, const Group& g, uint32_t* code) {
+    const float inv = g.scale > 0.0f ? __builtin_amdgcn_rcpf(g.scale) : 0.0f;
+    bool near_half = false;
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-        lo = fminf(lo, x[i]);
-        hi = fmaxf(hi, x[i]);
-        sum += x[i] * 0.0f;  // NaN when a value is not finite
+        const float q = ((float)x[i >> 1][i & 1] - g.low) * inv;
+        near_half |= fabsf(__builtin_amdgcn_fractf(q) - 0.5f) < 0x1p-16f;
+        code[i] = (uint32_t)fminf(rintf(q), 15.0f);
     }
-    lo = fminf(lo, dpp<0xB1>(lo));
-    hi = fmaxf(hi, dpp<0xB1>(hi));
-    sum += dpp<0xB1>(sum);
-    return {lo, hi, sum == 0.0f};
+    if (!near_half) return;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        const float v = (float)x[i >> 1][i & 1], q = (v - g.low) * inv;
+        if (q < 16.0f && fabsf(__builtin_amdgcn_fractf(q) - 0.5f) < 0x1p-16f) {
+            const float below = floorf(q), half_way = below + 0.5f;
+            const double side = ((double)v - (double)g.low) - (double)half_way * (double)g.scale;
+            const float r = side < 0.0 ? below : side > 0.0 ? below + 1.0f : 2.0f * rintf(0.5f * half_way);
+            code[i] = (uint32_t)fminf(r, 15.0f);
+        }
+    }
 }
 
-// code of x in a group, exactly rint((x - low) / scale): the quotient in 32 bits is off by less
-// than 2^-20, and where it is nearer than that to a half, 64 bits (which hold both sides exactly) decide.
-__device__ __forceinline__ uint32_t code_of(float x, float low, float scale) {
-    if (!(scale > 0.0f)) return 0;
-    const float q = (x - low) / scale;
-    float r = rintf(q);
-    const float half_way = floorf(q) + 0.5f;
-    if (fabsf(q - half_way) < 0x1p-18f) {
-        const double side = ((double)x - (double)low) - (double)half_way * (double)scale;
-        r = side < 0.0 ? floorf(q) : side > 0.0 ? floorf(q) + 1.0f : 2.0f * rintf(0.5f * half_way);
-    }
-    return (uint32_t)fminf(fmaxf(r, 0.0f), 15.0f);
-}
-
-// One workgroup per (block of 32 tokens that gets rows, head); thread (token, part) has 16 channels.
+// One workgroup per (block of 32 tokens that gets rows, head); thread (token, part) has 16 channels
+// of K and of V, so that a wave has the eight tokens that share the dwords of V.
+//
+// Bound: the vector ALU, and memory behind it (512 bytes in and 160 out per row).
 __global__ void __launch_bounds__(kThreads) append_kernel(RowArgs A) {
-    __shared__ __align__(16) uint32_t s_k[512];      // K codes as stored
-    __shared__ uint32_t s_kp[128];                   // K scalings as stored
-    __shared__ __align__(16) uint8_t s_v[kBlock][kDim + 16];  // V codes, a byte each
-    __shared__ uint16_t s_vp[256];                   // V scales and lowest values as stored
+    __shared__ __align__(16) uint32_t s_k[512], s_v[512];  // codes as stored
+    __shared__ uint32_t s_kp[128];                         // K scalings as stored
+    __shared__ uint16_t s_vp[256];                         // V scales and lowest values as stored
     const int h = (int)blockIdx.x % A.pool.heads;
     const Part P = row_part(A, (int)blockIdx.x / A.pool.heads);
     if (P.seq < 0) return;
-    char* const block = A.pool.at(P.seq, P.block, h);
-    if (!block) return;
     const int tid = threadIdx.x, token = tid >> 3, part = tid & 7, group = part >> 1;
     const bool mine = token >= P.lo && token < P.hi;
+    uint4 kw[2] = {}, vw[2] = {};
+    if (mine) {
+        const long row = P.row + token - P.lo;
+        const uint4* ks = reinterpret_cast<const uint4*>(A.k + row * A.k_token + h * A.k_head) + 2 * part;
+        const uint4* vs = reinterpret_cast<const uint4*>(A.v + row * A.v_token + h * A.v_head) + 2 * part;
+        kw[0] = ks[0], kw[1] = ks[1];
+        vw[0] = vs[0], vw[1] = vs[1];
+    }
+    char* const block = A.pool.at(P.seq, P.block, h);
+    if (!block) return;
+    uint32_t code[16];
+    half2_t x[8];
+    auto unpack = [&](const uint4* w) {
 #pragma unroll
-    for (int side = 0; side < 2; ++side) {
-        float x[16];
-        const uint16_t* src = side == 0 ? A.k + (P.row + token - P.lo) * A.k_token + h * A.k_head
-                                        : A.v + (P.row + token - P.lo) * A.v_token + h * A.v_head;
-        uint4 w[2] = {};
-        if (mine) {
-            w[0] = reinterpret_cast<const uint4*>(src)[2 * part];
-            w[1] = reinterpret_cast<const uint4*>(src)[2 * part + 1];
+        for (int i = 0; i < 2; ++i) {
+            x[4 * i] = __builtin_bit_cast(half2_t, w[i].x);
+            x[4 * i + 1] = __builtin_bit_cast(half2_t, w[i].y);
+            x[4 * i + 2] = __builtin_bit_cast(half2_t, w[i].z);
+            x[4 * i + 3] = __builtin_bit_cast(half2_t, w[i].w);
         }
-        const uint32_t words[8] = {w[0].x, w[0].y, w[0].z, w[0].w, w[1].x, w[1].y, w[1].z, w[1].w};
+    };
+    {
+        unpack(kw);
+        const Group g = group_of(x);
+        codes_of(x, g, code);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) x[i] = h2f((uint16_t)(words[i >> 1] >> (16 * (i & 1))));
-        const Range r = group_range(x);
-        // one division in 64 bits: the quotient is then rounded once
-        const uint16_t scale16 = r.finite ? f2h((float)(((double)r.high - (double)r.low) / 15.0)) : 0x7E00;
-        const uint16_t low16 = r.finite ? f2h(r.low) : 0x7E00;
-        const float scale = h2f(scale16);
-        uint32_t code[16];
+        for (int q = 0; q < 2; ++q) {
+            uint32_t packed = 0;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) code[i] = code_of(x[i], r.low, scale);
-        if (side == 0) {
-#pragma unroll
-            for (int q = 0; q < 2; ++q) {
-                uint32_t packed = 0;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) packed |= code[8 * q + e] << nibble(e);
-                s_k[(((token >> 4) * 4 + 2 * (part & 1) + q) * 16 + (token & 15)) * 4 + group] = packed;
-            }
-            if ((part & 1) == 0) s_kp[((token >> 4) * 4 + group) * 16 + (token & 15)] = scale16 | ((uint32_t)low16 << 16);
-        } else {
-            uint32_t bytes[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                bytes[i] = code[4 * i] | (code[4 * i + 1] << 8) | (code[4 * i + 2] << 16) | (code[4 * i + 3] << 24);
-            *reinterpret_cast<uint4*>(&s_v[token][16 * part]) = make_uint4(bytes[0], bytes[1], bytes[2], bytes[3]);
-            if ((part & 1) == 0) {
-                s_vp[group * kBlock + token] = scale16;
-                s_vp[128 + group * kBlock + token] = low16;
-            }
+            for (int e = 0; e < 8; ++e) packed |= code[8 * q + e] << nibble(e);
+            s_k[(((token >> 4) * 4 + 2 * (part & 1) + q) * 16 + (token & 15)) * 4 + group] = packed;
         }
+        if ((part & 1) == 0) s_kp[((token >> 4) * 4 + group) * 16 + (token & 15)] = g.scale16 | ((uint32_t)g.low16 << 16);
+    }
+    {
+        unpack(vw);
+        const Group g = group_of(x);
+        codes_of(x, g, code);
+        if ((part & 1) == 0) {
+            s_vp[group * kBlock + token] = g.scale16;
+            s_vp[128 + group * kBlock + token] = g.low16;
+        }
+        // the eight tokens' nibbles of a channel come together over the lanes (token, part) of the wave: each
+        // of three exchanges halves the channels that a lane still has, and joins two tokens' nibbles
+        const int e = token & 7, shift = 4 * (e / 2 + 4 * (e % 2));
+#pragma unroll
+        for (int i = 0; i < 16; ++i) code[i] <<= shift;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const auto r = __builtin_amdgcn_permlane32_swap(code[i], code[i + 8], false, false);
+            code[i] = r[0] | r[1];  // channels i of lanes below 32, i + 8 of the others
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const auto r = __builtin_amdgcn_permlane16_swap(code[i], code[i + 4], false, false);
+            code[i] = r[0] | r[1];
+        }
+        const bool upper = (token & 1) != 0;  // lane ^ 8 is the token next to it
+        const uint32_t keep0 = upper ? code[2] : code[0], keep1 = upper ? code[3] : code[1];
+        const uint32_t give0 = upper ? code[0] : code[2], give1 = upper ? code[1] : code[3];
+        const int n = 8 * ((token >> 2) & 1) + 4 * ((token >> 1) & 1) + 2 * (token & 1);  // channel in the part
+        const int at = (part >> 2) * 256 + ((token >> 3) * 16 + n) * 4 + (part & 3);
+        s_v[at] = keep0 | dpp_u<0x128>(give0);  // row_ror:8
+        s_v[at + 4] = keep1 | dpp_u<0x128>(give1);
     }
     __syncthreads();
     if (tid < 128) {
@@ -187,20 +229,23 @@ __global__ void __launch_bounds__(kThreads) append_kernel(RowArgs A) {
     }
     // V codes: dword (c / 64, t / 8, c % 16, c / 16 % 4) has the eight tokens of a channel; of a dword whose
     // tokens are not all new the others' nibbles stay
+    if (tid < 128) {
+        const int t0 = 8 * ((tid >> 4) & 3);
+        if (t0 + 8 <= P.lo || t0 >= P.hi) return;
+        uint4* const dst = reinterpret_cast<uint4*>(block + kVCodes) + tid;
+        uint4 w = reinterpret_cast<const uint4*>(s_v)[tid];
+        if (t0 < P.lo || t0 + 8 > P.hi) {
+            uint32_t fresh = 0;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const int d = tid + kThreads * i;
-        const int t0 = 8 * ((d >> 6) & 3), c = 64 * (d >> 8) + 16 * (d & 3) + ((d >> 2) & 15);
-        if (t0 + 8 <= P.lo || t0 >= P.hi) continue;
-        uint32_t packed = 0, keep = 0;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            if (t0 + e >= P.lo && t0 + e < P.hi) packed |= (uint32_t)s_v[t0 + e][c] << nibble(e);
-            else keep |= 15u << nibble(e);
+            for (int i = 0; i < 8; ++i)
+                if (t0 + i >= P.lo && t0 + i < P.hi) fresh |= 15u << nibble(i);
+            const uint4 old = *dst;
+            w.x = (w.x & fresh) | (old.x & ~fresh);
+            w.y = (w.y & fresh) | (old.y & ~fresh);
+            w.z = (w.z & fresh) | (old.z & ~fresh);
+            w.w = (w.w & fresh) | (old.w & ~fresh);
         }
-        uint32_t* dst = reinterpret_cast<uint32_t*>(block + kVCodes) + d;
-        if (keep) packed |= *dst & keep;
-        *dst = packed;
+        *dst = w;
     }
 }
 
@@ -293,13 +338,14 @@ struct AttnArgs {
     const uint16_t* q;  // [B, Hq, 128]
     const int32_t* lengths;
     uint16_t* out;      // [B, Hq, 128]
-    float* part;        // [B * Hq, splits, 130]: o[128], m, l
+    float* part;        // [B * Hq, splits, 128]: weighted values
+    float2* stat;       // [B * Hq, splits]: maximum, sum of the weights
     int Hq, G, sets, splits;
     int chunk;          // blocks per split
     int max_length;
     float c;            // scaling * log2(e)
 };
-constexpr int kRecord = kDim + 2;
+constexpr int kRecord = kDim + 2;  // floats of a split's record
 
 __device__ __forceinline__ float swap_sum32(float a, float b) {
     const auto r = __builtin_amdgcn_permlane32_swap((uint32_t)f2i(a), (uint32_t)f2i(b), false, false);
@@ -348,12 +394,13 @@ __device__ __forceinline__ void load_block(Block& b, const char* p, int lane) {
 // head h in row 4 g + h and zeros elsewhere, so that lane (quarter g, token n) gets the four heads' sums over
 // group g alone and applies that group's scale and lowest value (times the sum of q over the group) in fp32;
 // three lane swaps add the groups and leave head h's score of token n in lane (h, n).
-// Values: D[row 4 g + h][channel] += (P s_g) V over 32 tokens, weights times scale of group g in row
-// 4 g + h; the rows of a channel's own group are the ones that count.  The lowest values are one
+// Values: D[row 4 g + h][16 channels] += (P s_g) V over 32 tokens for each group's two sets of channels, the
+// weights times the scale of group g in rows 4 g + h and zeros elsewhere, so that the four groups
+// share one set of accumulators (32 registers otherwise, a quarter of them used).  The lowest values are one
 // more product, with P alone.  The product P s is relative to a power of two `e2` not below any scale so far,
 // kept like the softmax's maximum.
 template <int HB>
-__global__ void __launch_bounds__(kThreads) attention_kernel(AttnArgs A) {
+__global__ void __launch_bounds__(kThreads, HB == 1 ? 3 : 2) attention_kernel(AttnArgs A) {
     constexpr int kHeads = 4 * HB;
     constexpr int kPitch = kBlock + 8;
     __shared__ __align__(16) uint16_t s_p[kWaves][kHeads * kPitch];
@@ -418,7 +465,7 @@ __global__ void __launch_bounds__(kThreads) attention_kernel(AttnArgs A) {
         }
     }
 
-    float4_t acc[HB][8], accl[HB];
+    float4_t acc[HB][2], accl[HB];  // acc: channels 32 quarter + 16 i + n of the four heads
     float m[HB], l[HB];  // head 4 hb + quarter; l: this lane's tokens
 #pragma unroll
     for (int hb = 0; hb < HB; ++hb) {
@@ -426,16 +473,30 @@ __global__ void __launch_bounds__(kThreads) attention_kernel(AttnArgs A) {
         l[hb] = 0.0f;
         accl[hb] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int nb = 0; nb < 8; ++nb) acc[hb][nb] = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (int i = 0; i < 2; ++i) acc[hb][i] = {0.0f, 0.0f, 0.0f, 0.0f};
     }
     float e2 = 0x1p-14f;  // not below any scale so far
 
-    for (int blk = begin; blk < end; ++blk) {
-        const char* p = A.pool.at(b, blk, hk);
-        if (!p) continue;
-        Block x;
-        load_block(x, p, lane);
-        const int valid = min(kBlock, length - blk * kBlock);
+    // The wave's blocks, one after the other, each fetched while the one before is worked on.  Page
+    // numbers come 64 at a time, one per lane.
+    int entry0 = begin / A.pool.blocks, entry = 0, inside = begin - entry0 * A.pool.blocks, numbers = 0;
+    auto fetch_numbers = [&]() { numbers = A.pool.table[(long)b * A.pool.width + min(entry0 + lane, A.pool.width - 1)]; };
+    // next block's data, and whether its page is there
+    auto fetch = [&](Block& x) {
+        const char* p = A.pool.in_page(__builtin_amdgcn_readlane(numbers, entry), inside, hk);
+        load_block(x, p ? p : A.pool.pages, lane);
+        if (++inside == A.pool.blocks) {
+            inside = 0;
+            if (++entry == kWave) {
+                entry0 += kWave;
+                entry = 0;
+                fetch_numbers();
+            }
+        }
+        return p != nullptr;
+    };
+    auto work = [&](Block& x, int blk, bool there) {
+        const int valid = there ? min(kBlock, length - blk * kBlock) : 0;
         if (valid < kBlock) {  // what lies behind the last token may be anything
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -468,10 +529,10 @@ __global__ void __launch_bounds__(kThreads) attention_kernel(AttnArgs A) {
                 score[hb][tile] = 16 * tile + n < valid ? s : -INFINITY;
             }
         }
-        float top_scale = 0.0f;
+        half2_t tops = {(_Float16)0.0f, (_Float16)0.0f};
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            top_scale = fmaxf(top_scale, fmaxf(h2f((uint16_t)x.vs[i]), h2f((uint16_t)(x.vs[i] >> 16))));
+        for (int i = 0; i < 4; ++i) tops = __builtin_elementwise_max(tops, __builtin_bit_cast(half2_t, x.vs[i]));
+        const float top_scale = fmaxf((float)tops[0], (float)tops[1]);
         bool grow = top_scale > e2;
 #pragma unroll
         for (int hb = 0; hb < HB; ++hb) grow |= fmaxf(score[hb][0], score[hb][1]) > m[hb];
@@ -494,7 +555,7 @@ __global__ void __launch_bounds__(kThreads) attention_kernel(AttnArgs A) {
                     const float a = readlane(alpha, 16 * i);
                     accl[hb][i] *= a;
 #pragma unroll
-                    for (int nb = 0; nb < 8; ++nb) acc[hb][nb][i] *= a * shrink;
+                    for (int j = 0; j < 2; ++j) acc[hb][j][i] *= a * shrink;
                 }
             }
         }
@@ -512,21 +573,39 @@ __global__ void __launch_bounds__(kThreads) attention_kernel(AttnArgs A) {
         const half8_t factor = {one, one, sixteenth, sixteenth, one, one, sixteenth, sixteenth};
         const half8_t vscale = __builtin_bit_cast(half8_t, make_uint4(x.vs[0], x.vs[1], x.vs[2], x.vs[3])) * factor;
         const half8_t vlow = __builtin_bit_cast(half8_t, make_uint4(x.vl[0], x.vl[1], x.vl[2], x.vl[3]));
-        half8_t ps[HB];
+        uint4 ps[HB];
 #pragma unroll
         for (int hb = 0; hb < HB; ++hb) {
             const half8_t pw = *reinterpret_cast<const half8_t*>(&s_p[wave][(4 * hb + (n & 3)) * kPitch + 8 * quarter]);
             accl[hb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(pw, vlow, accl[hb], 0, 0, 0);
-            ps[hb] = pw * vscale;
+            ps[hb] = __builtin_bit_cast(uint4, pw * vscale);
         }
 #pragma unroll
-        for (int nb = 0; nb < 8; ++nb) {
-            const uint4& q4 = x.v[nb >> 2];
-            const half8_t vf = operand((nb & 3) == 0 ? q4.x : (nb & 3) == 1 ? q4.y : (nb & 3) == 2 ? q4.z : q4.w);
+        for (int g = 0; g < 4; ++g) {
+            const uint4& codes = x.v[g >> 1];
+            const half8_t v0 = operand(g & 1 ? codes.z : codes.x), v1 = operand(g & 1 ? codes.w : codes.y);
+            const uint32_t rows = (n >> 2) == g ? ~0u : 0u;
 #pragma unroll
-            for (int hb = 0; hb < HB; ++hb) acc[hb][nb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ps[hb], vf, acc[hb][nb], 0, 0, 0);
+            for (int hb = 0; hb < HB; ++hb) {
+                const half8_t pg = __builtin_bit_cast(half8_t, make_uint4(ps[hb].x & rows, ps[hb].y & rows, ps[hb].z & rows,
+                                                                          ps[hb].w & rows));
+                acc[hb][0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(pg, v0, acc[hb][0], 0, 0, 0);
+                acc[hb][1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(pg, v1, acc[hb][1], 0, 0, 0);
+            }
         }
         wave_sync();
+    };
+    if (begin < end) {
+        Block x0, x1;
+        fetch_numbers();
+        bool there0 = fetch(x0), there1 = false;
+        for (int blk = begin; blk < end; blk += 2) {
+            if (blk + 1 < end) there1 = fetch(x1);
+            work(x0, blk, there0);
+            if (blk + 1 >= end) break;
+            if (blk + 2 < end) there0 = fetch(x0);
+            work(x1, blk + 1, there1);
+        }
     }
 
     // lane (quarter g, n): channels 32 g + n and 32 g + 16 + n of the four heads
@@ -542,11 +621,8 @@ __global__ void __launch_bounds__(kThreads) attention_kernel(AttnArgs A) {
         for (int i = 0; i < 4; ++i) {
             const float lows = __shfl(accl[hb][i], 16 * quarter + 4 * quarter);  // row 4 g + i, column of group g
 #pragma unroll
-            for (int g = 0; g < 4; ++g)
-                if (g == quarter)
-#pragma unroll
-                    for (int half = 0; half < 2; ++half)
-                        s_o[wave][4 * hb + i][32 * g + 16 * half + n] = __builtin_fmaf(acc[hb][2 * g + half][i], back, lows);
+            for (int j = 0; j < 2; ++j)
+                s_o[wave][4 * hb + i][32 * quarter + 16 * j + n] = __builtin_fmaf(acc[hb][j][i], back, lows);
         }
     }
     __syncthreads();
@@ -566,35 +642,64 @@ __global__ void __launch_bounds__(kThreads) attention_kernel(AttnArgs A) {
         if (A.splits == 1) {
             A.out[(row0 + h) * kDim + ch] = f2h(total == 0.0f ? 0.0f : o / total);
         } else {
-            float* rec = A.part + ((row0 + h) * A.splits + split) * kRecord;
-            rec[ch] = o;
-            if (ch == 0) {
-                rec[kDim] = top;
-                rec[kDim + 1] = total;
-            }
+            const long rec = (row0 + h) * A.splits + split;
+            A.part[rec * kDim + ch] = o;
+            if (ch == 0) A.stat[rec] = make_float2(top, total);
         }
     }
 }
 
-// Joins the splits of a query head: one workgroup of 128 threads, a channel each.
-__global__ void __launch_bounds__(kDim) merge_kernel(AttnArgs A) {
+// Joins the splits of a query head: one workgroup per (sequence, query head).  Lanes take the splits'
+// maxima and sums, 64 at a time; the waves then take every fourth split's 128 channels, two per lane,
+// with eight loads under way (one after the other a split costs a trip to memory: 51 splits took 28 us).
+__global__ void __launch_bounds__(kThreads) merge_kernel(AttnArgs A) {
+    __shared__ float2 s_o[kWaves][kWave];
     const long row = blockIdx.x;
-    const int b = (int)(row / A.Hq), ch = threadIdx.x;
+    const int b = (int)(row / A.Hq), lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int length = min(max(A.lengths[b], 0), A.max_length);
     const int blocks = (length + kBlock - 1) / kBlock;
     const int splits = min(A.splits, (blocks + A.chunk - 1) / A.chunk);
-    const float* rec = A.part + row * A.splits * kRecord;
+    const float2* const stat = A.stat + row * A.splits;
+    const float2* const part = reinterpret_cast<const float2*>(A.part) + row * A.splits * kWave + lane;
     float top = -__FLT_MAX__;
-    for (int s = 0; s < splits; ++s) top = fmaxf(top, rec[s * kRecord + kDim]);
-    float o = 0.0f, total = 0.0f;
-    for (int s = 0; s < splits; ++s) {
-        const float l = rec[s * kRecord + kDim + 1];
-        if (l == 0.0f) continue;  // no tokens (a NaN goes on)
-        const float a = __builtin_amdgcn_exp2f(rec[s * kRecord + kDim] - top);
-        o += a * rec[s * kRecord + ch];
-        total += a * l;
+    for (int s = lane; s < splits; s += kWave) top = fmaxf(top, stat[s].x);
+    top = wave_max(top);
+    float2 o = make_float2(0.0f, 0.0f);
+    float total = 0.0f;
+    for (int s0 = 0; s0 < splits; s0 += kWave) {
+        const float2 ml = s0 + lane < splits ? stat[s0 + lane] : make_float2(0.0f, 0.0f);
+        const float weight = ml.y == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(ml.x - top);  // no tokens (a NaN goes on)
+        total += wave_sum(weight * ml.y);
+        const int n = min(kWave, splits - s0);
+        for (int i0 = wave; i0 < n; i0 += 8 * kWaves) {
+            float2 r[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int at = min(i0 + kWaves * i, n - 1);
+                r[i] = part[(long)(s0 + at) * kWave];
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int at = i0 + kWaves * i;
+                const float a = readlane(weight, at & 63);
+                if (at < n) {
+                    o.x += a * r[i].x;
+                    o.y += a * r[i].y;
+                }
+            }
+        }
     }
-    A.out[row * kDim + ch] = f2h(total == 0.0f ? 0.0f : o / total);
+    s_o[wave][lane] = o;
+    __syncthreads();
+    if (wave != 0) return;
+#pragma unroll
+    for (int i = 1; i < kWaves; ++i) {
+        o.x += s_o[i][lane].x;
+        o.y += s_o[i][lane].y;
+    }
+    const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+    reinterpret_cast<uint32_t*>(A.out + row * kDim)[lane] = pack_halves(o.x * inv, o.y * inv);
 }
 
 // ---------------------------------------------------------------------------
@@ -615,13 +720,14 @@ __global__ void __launch_bounds__(kThreads) copy_kernel(CopyArgs A) {
     const uint4* src = A.pages + A.source[blockIdx.y] * A.pieces + at;
     uint4* dst = A.pages + A.target[blockIdx.y] * A.pieces + at;
     const long left = A.pieces - (long)blockIdx.x * kCopyPieces - threadIdx.x;
-    uint4 r[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-        if (i * kThreads < left) r[i] = src[i * kThreads];
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-        if (i * kThreads < left) dst[i * kThreads] = r[i];
+    if (left <= 0) return;
+    // (an array of uint4 would be put into the LDS here)
+    const uint4 a = src[0], b = src[kThreads < left ? kThreads : 0];
+    const uint4 c = src[2 * kThreads < left ? 2 * kThreads : 0], d = src[3 * kThreads < left ? 3 * kThreads : 0];
+    dst[0] = a;
+    if (kThreads < left) dst[kThreads] = b;
+    if (2 * kThreads < left) dst[2 * kThreads] = c;
+    if (3 * kThreads < left) dst[3 * kThreads] = d;
 }
 
 // ---------------------------------------------------------------------------
@@ -751,6 +857,7 @@ extern "C" int reskv_int4_attention(const void* q, const void* pages, int64_t nu
     A.lengths = lengths;
     A.out = (uint16_t*)out;
     A.part = (float*)workspace;
+    A.stat = (float2*)(A.part + (long)B * Hq * s.splits * kDim);
     A.Hq = Hq;
     A.G = G;
     A.sets = head_sets(G);
@@ -764,7 +871,7 @@ extern "C" int reskv_int4_attention(const void* q, const void* pages, int64_t nu
                        (hipStream_t)stream, A);
     if (reskv_host::check_launch("int4 attention_kernel")) return 1;
     if (s.splits == 1) return 0;
-    hipLaunchKernelGGL(merge_kernel, dim3((unsigned)(B * Hq)), dim3(kDim), 0, (hipStream_t)stream, A);
+    hipLaunchKernelGGL(merge_kernel, dim3((unsigned)(B * Hq)), dim3(kThreads), 0, (hipStream_t)stream, A);
     return reskv_host::check_launch("int4 merge_kernel");
 }
 

@@ -20,17 +20,16 @@ the table, stands for a token that is not there, which appends leave out and rea
 """
 
 import ctypes
+from functools import lru_cache
 
 import torch
 
 from . import _lib
 from ._extension import _require, _workspace
-from .packed import _int32, _kernel_rows, _launch, _rows, _same_gpu
+from .packed import _INF, _int32, _kernel_rows, _launch, _new, _rows, _same_gpu, _strides
 
 BLOCK_TOKENS = 32
 TOKEN_BYTES = 160  # of one KV head, K and V
-
-_STRIDES = ctypes.c_int64 * 4
 
 
 def _page_bytes(page_tokens):
@@ -49,21 +48,20 @@ def empty_pages(pages, kv_heads, page_tokens=64, layers=None, device="cuda"):
 
 def _pool(pages):
     """(pages, tokens per page, KV heads) of a pool."""
-    _require(pages.dtype == torch.uint8 and pages.dim() == 3 and pages.is_contiguous(),
+    _require(pages.dtype is torch.uint8 and pages.dim() == 3 and pages.is_contiguous(),
              "pages must be a contiguous uint8 tensor [pages, KV heads, bytes]")
     count, heads, nbytes = pages.shape
-    _require(count > 0 and heads > 0 and nbytes > 0 and nbytes % (BLOCK_TOKENS * TOKEN_BYTES) == 0,
-             f"a page must hold a positive multiple of {BLOCK_TOKENS} tokens of {TOKEN_BYTES} bytes")
+    if not (count > 0 and heads > 0 and nbytes > 0 and nbytes % (BLOCK_TOKENS * TOKEN_BYTES) == 0):
+        raise RuntimeError(f"a page must hold a positive multiple of {BLOCK_TOKENS} tokens of {TOKEN_BYTES} bytes")
     return count, nbytes // TOKEN_BYTES, heads
 
 
 def _table(table):
-    _require(table.dtype == torch.int32 and table.dim() == 2 and table.is_contiguous() and table.shape[1] > 0,
+    _require(table.dtype is torch.int32 and table.dim() == 2 and table.is_contiguous() and table.shape[1] > 0,
              "table must be a contiguous int32 matrix [sequences, pages]")
     return table.shape
 
 
-@torch.no_grad()
 def int4_append(pages, table, starts, k, v, offsets=None):
     """Quantises rows of k and v, fp16 [N, Hk, 128] (any strides with unit channel stride), into pages.
 
@@ -83,16 +81,15 @@ def int4_append(pages, table, starts, k, v, offsets=None):
         _require(n == sequences, "without offsets there must be one row for every sequence")
     else:
         _int32("offsets", offsets, sequences + 1)
-    dev = _same_gpu(pages, table, starts, k, v, offsets)
+    index = _same_gpu(pages, table, starts, k, v, offsets)
     if n == 0 or sequences == 0:
         return
     k, v = _kernel_rows(k), _kernel_rows(v)
-    _launch("reskv_int4_append", dev, pages.data_ptr(), count, tokens, heads, table.data_ptr(), width, sequences,
+    _launch("reskv_int4_append", index, pages.data_ptr(), count, tokens, heads, table.data_ptr(), width, sequences,
             starts.data_ptr(), None if offsets is None else offsets.data_ptr(), k.data_ptr(), v.data_ptr(), n,
-            _STRIDES(*k.stride()[:2], *v.stride()[:2]))
+            _strides(k, v))
 
 
-@torch.no_grad()
 def int4_gather(pages, table, starts, offsets, rows, out=None):
     """The stored values of tokens, as (k, v) fp16 [rows, Hk, 128]: row ``offsets[s] + i`` is token
     ``starts[s] + i`` of sequence s (``rows`` is what ``offsets`` ends with; the host does not read it).
@@ -111,19 +108,23 @@ def int4_gather(pages, table, starts, offsets, rows, out=None):
             _rows(name, t, heads)
             _require(t.shape[0] == rows and t.is_contiguous(), f"{name} must be contiguous and have {rows} rows")
     k, v = (None, None) if clear else out
-    dev = _same_gpu(pages, table, starts, offsets, k, v)
+    index = _same_gpu(pages, table, starts, offsets, k, v)
     if clear:
-        k, v = (torch.empty((rows, heads, 128), dtype=torch.float16, device=dev) for _ in range(2))
+        k, v = (torch.empty((rows, heads, 128), dtype=torch.float16, device=pages.device) for _ in range(2))
     if rows == 0:
         return k, v
     if sequences == 0:
         return (k.zero_(), v.zero_()) if clear else (k, v)
-    _launch("reskv_int4_gather", dev, pages.data_ptr(), count, tokens, heads, table.data_ptr(), width, sequences,
-            starts.data_ptr(), offsets.data_ptr(), k.data_ptr(), v.data_ptr(), rows, int(clear))
+    _launch("reskv_int4_gather", index, pages.data_ptr(), count, tokens, heads, table.data_ptr(), width, sequences,
+            starts.data_ptr(), offsets.data_ptr(), k.data_ptr(), v.data_ptr(), rows, clear)
     return k, v
 
 
-@torch.no_grad()
+@lru_cache(4096)  # a function of the sizes alone
+def _attention_workspace(sequences, heads, kv_heads, most):
+    return _lib.lib().reskv_int4_workspace_bytes(sequences, heads, kv_heads, most)
+
+
 def int4_attention(q, pages, table, lengths, *, scaling=None, max_length=None, out=None):
     """Attention of one token of every sequence: q fp16 [B, Hq, 128] (rotated) against the first
     ``lengths[b]`` (int32 [B]) tokens of sequence b; fp16 [B, Hq, 128], ``out`` when given (contiguous).
@@ -141,51 +142,52 @@ def int4_attention(q, pages, table, lengths, *, scaling=None, max_length=None, o
     _require(q.shape[0] == sequences, "q must have one row for every sequence")
     _require(heads > 0 and heads % kv_heads == 0, "the query heads must be a multiple of the KV heads")
     scaling = 128 ** -0.5 if scaling is None else float(scaling)
-    _require(-float("inf") < scaling < float("inf"), "scaling must be finite")
+    _require(-_INF < scaling < _INF, "scaling must be finite")
     most = width * tokens if max_length is None else int(max_length)
     _require(most >= 0, "max_length must not be negative")
     if out is not None:
         _rows("out", out, heads)
         _require(out.shape[0] == sequences and out.is_contiguous(), "out must be contiguous and shaped like q")
-    dev = _same_gpu(q, pages, table, lengths, out)
+    index = _same_gpu(q, pages, table, lengths, out)
     if out is None:
-        out = torch.empty((sequences, heads, 128), dtype=torch.float16, device=dev)
+        out = _new(q, (sequences, heads, 128))
     if sequences == 0:
         return out
-    q = q if q.is_contiguous() and q.data_ptr() % 16 == 0 else q.clone(memory_format=torch.contiguous_format)
+    if not q.is_contiguous() or q.data_ptr() & 15:
+        q = q.detach().clone(memory_format=torch.contiguous_format)
     most = min(most, width * tokens)
-    nbytes = _lib.lib().reskv_int4_workspace_bytes(sequences, heads, kv_heads, most)
-    work = _workspace(nbytes, dev) if nbytes else None
-    _launch("reskv_int4_attention", dev, q.data_ptr(), pages.data_ptr(), count, tokens, table.data_ptr(), width,
+    nbytes = _attention_workspace(sequences, heads, kv_heads, most)
+    work = _workspace(nbytes, q.device) if nbytes else None
+    _launch("reskv_int4_attention", index, q.data_ptr(), pages.data_ptr(), count, tokens, table.data_ptr(), width,
             lengths.data_ptr(), sequences, heads, kv_heads, scaling, most, out.data_ptr(),
             None if work is None else work.data_ptr(), nbytes)
     return out
 
 
-@torch.no_grad()
 def copy_pages(pages, source, target):
     """Copies page ``source[i]`` to page ``target[i]`` (host sequences of page numbers) in a pool [pages, ...]
     or in every layer's pool [layers, pages, KV heads, bytes], in one launch per 384 pages.
 
     A target may be neither a source nor named twice: what it would hold then depends on the order.
     """
-    _require(pages.dtype == torch.uint8 and pages.dim() in (3, 4) and pages.is_contiguous(),
+    _require(pages.dtype is torch.uint8 and pages.dim() in (3, 4) and pages.is_contiguous(),
              "pages must be a contiguous uint8 tensor [pages, KV heads, bytes] or [layers, pages, KV heads, bytes]")
-    source, target = [int(p) for p in source], [int(p) for p in target]
+    source, target = list(map(int, source)), list(map(int, target))
     _require(len(source) == len(target), "every source page needs a target page")
     layers, count = (1, pages.shape[0]) if pages.dim() == 3 else pages.shape[:2]
     nbytes = pages.shape[-2] * pages.shape[-1]
     _require(nbytes > 0 and nbytes % 16 == 0, "a page must be a multiple of 16 bytes")
-    _require(all(0 <= p < count for p in source) and all(0 <= p < count for p in target),
-             f"page numbers must be in 0 .. {count - 1}")
-    _require(len(set(target)) == len(target) and not set(target) & set(source),
+    if source and not (0 <= min(source) and max(source) < count and 0 <= min(target) and max(target) < count):
+        raise RuntimeError(f"page numbers must be in 0 .. {count - 1}")
+    written = set(target)
+    _require(len(written) == len(target) and written.isdisjoint(source),
              "a target page may be neither a source nor named twice")
-    dev = _same_gpu(pages)
+    index = _same_gpu(pages)
     n = len(source)
     if n == 0 or layers == 0:
         return
     pairs = ctypes.c_int32 * n
-    _launch("reskv_copy_pages", dev, pages.data_ptr(), layers, count, nbytes, pairs(*source), pairs(*target), n)
+    _launch("reskv_copy_pages", index, pages.data_ptr(), layers, count, nbytes, pairs(*source), pairs(*target), n)
 
 
 class Int4Cache:

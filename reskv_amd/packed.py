@@ -6,54 +6,83 @@ prompts that continue on keys already there.  Like ``attention`` it is an infere
 operator: no gradient is recorded.
 """
 
-import ctypes
+import struct
+from functools import lru_cache
 
 import torch
 
 from . import _lib
-from ._extension import _require, _stream, _workspace
+from ._extension import _require, _workspace
 
-_STRIDES = ctypes.c_int64 * 6
+_INF = float("inf")
 
 
+# The checks run for every call of a decode step, so that a message is put together only
+# where it is needed.
 def _rows(name, t, heads=None):
-    _require(t.dtype == torch.float16 and t.dim() == 3 and t.shape[2] == 128, f"{name} must be fp16 [rows, heads, 128]")
-    _require(heads is None or t.shape[1] == heads, f"{name} has {t.shape[1]} heads, expected {heads}")
+    if t.dtype is not torch.float16 or t.dim() != 3 or t.shape[2] != 128:
+        raise RuntimeError(f"{name} must be fp16 [rows, heads, 128]")
+    if heads is not None and t.shape[1] != heads:
+        raise RuntimeError(f"{name} has {t.shape[1]} heads, expected {heads}")
 
 
 def _int32(name, t, count):
-    _require(t.dtype == torch.int32 and t.dim() == 1 and t.is_contiguous(), f"{name} must be a contiguous int32 vector")
-    _require(count is None or t.shape[0] == count, f"{name} has {t.shape[0]} entries, expected {count}")
+    if t.dtype is not torch.int32 or t.dim() != 1 or not t.is_contiguous():
+        raise RuntimeError(f"{name} must be a contiguous int32 vector")
+    if count is not None and t.shape[0] != count:
+        raise RuntimeError(f"{name} has {t.shape[0]} entries, expected {count}")
 
 
-def _same_gpu(*tensors):
-    """Checked last, after every shape, dtype and layout check."""
-    _require(all(t is None or t.is_cuda for t in tensors), "every tensor must be a CUDA tensor")
-    dev = tensors[0].device
-    _require(all(t is None or t.device == dev for t in tensors), "all tensors must be on the same GPU")
-    return dev
+def _same_gpu(first, *others):
+    """The index of the GPU that all tensors are on.  Checked last, after every shape, dtype and layout check."""
+    index = first.get_device() if first.is_cuda else -1
+    for t in others:
+        if t is not None and (not t.is_cuda or t.get_device() != index):
+            index = -1
+    if index < 0:
+        _require(all(t is None or t.is_cuda for t in (first, *others)), "every tensor must be a CUDA tensor")
+        raise RuntimeError("all tensors must be on the same GPU")
+    return index
 
 
-def _launch(name, dev, *args):
-    """Calls the library's ``name`` on the current stream of dev, made the current device meanwhile: a
-    launch goes to the current device, whatever the device of its pointers."""
-    fn = getattr(_lib.lib(), name)
-    if torch.cuda.current_device() == dev.index:
-        _lib.check(fn(*args, _stream(dev)), name)
-    else:
-        with torch.cuda.device(dev):
-            _lib.check(fn(*args, _stream(dev)), name)
+def _launch(name, index, *args):
+    """Calls the library's ``name`` on the current stream of GPU ``index``, made the current device
+    meanwhile: a launch goes to the current device, whatever the device of its pointers."""
+    if torch._C._cuda_getDevice() != index:
+        with torch.cuda.device(index):
+            return _launch(name, index, *args)
+    status = getattr(_lib.lib(), name)(*args, torch._C._cuda_getCurrentRawStream(index))
+    if status:
+        _lib.check(status, name)
 
 
-def _kernel_rows(t, most=None):
+def _kernel_rows(t, most=1 << 62):
     """t itself when its rows of 128 channels can be read in place (16-byte aligned; token stride
     below ``most``), else a contiguous copy."""
     token, head, channel = t.stride()
-    fits = channel == 1 and token % 8 == 0 and head % 8 == 0 and t.data_ptr() % 16 == 0
-    return t if fits and (most is None or token < most) else t.clone(memory_format=torch.contiguous_format)
+    if channel == 1 and not (token | head) & 7 and token < most and not t.data_ptr() & 15:
+        return t
+    return t.detach().clone(memory_format=torch.contiguous_format)
 
 
-@torch.no_grad()
+def _new(like, shape):
+    """An fp16 tensor (a plain one, also for a subclass's ``like``) on the GPU of ``like``."""
+    return like.new_empty(shape) if type(like) is torch.Tensor else torch.empty(shape, dtype=torch.float16, device=like.device)
+
+
+_pack = [struct.Struct(f"{2 * n}q").pack for n in range(4)]
+
+
+def _strides(*tensors):
+    """Token and head strides of row tensors, as the library reads them (int64 values in memory)."""
+    return _pack[len(tensors)](*(n for t in tensors for n in t.stride()[:2]))
+
+
+@lru_cache(4096)  # a function of the sizes alone
+def _packed_workspace(sequences, queries, heads, kv_heads, most):
+    return _lib.lib().reskv_packed_workspace_bytes(sequences, queries, heads, kv_heads, most)
+
+
 def packed_attention(q, k, v, q_offsets, k_offsets=None, *, scaling=None, max_keys=None, out=None):
     """Causal attention of S sequences packed one behind the other.
 
@@ -76,8 +105,8 @@ def packed_attention(q, k, v, q_offsets, k_offsets=None, *, scaling=None, max_ke
     _rows("k", k)
     _rows("v", v, k.shape[1])
     _require(k.shape[0] == v.shape[0], "k and v must have the same number of rows")
-    nq, heads = q.shape[0], q.shape[1]
-    nk, kv_heads = k.shape[0], k.shape[1]
+    nq, heads, _ = q.shape
+    nk, kv_heads, _ = k.shape
     _require(kv_heads > 0 and heads > 0 and heads % kv_heads == 0, "the query heads must be a multiple of the KV heads")
     _int32("q_offsets", q_offsets, None)
     count = q_offsets.shape[0] - 1
@@ -87,28 +116,27 @@ def packed_attention(q, k, v, q_offsets, k_offsets=None, *, scaling=None, max_ke
     else:
         _int32("k_offsets", k_offsets, count + 1)
     scaling = 128 ** -0.5 if scaling is None else float(scaling)
-    _require(scaling > 0.0 and scaling < float("inf"), "scaling must be positive")
+    _require(0.0 < scaling < _INF, "scaling must be positive")
     most = nk if max_keys is None else int(max_keys)
     _require(most >= 0, "max_keys must not be negative")
     clear = out is None
     if not clear:
         _rows("out", out, heads)
         _require(out.shape[0] == nq and out.is_contiguous(), "out must be contiguous and have a row for every query")
-    dev = _same_gpu(q, k, v, q_offsets, k_offsets, out)
+    index = _same_gpu(q, k, v, q_offsets, k_offsets, out)
     if clear:
-        out = torch.empty((nq, heads, 128), dtype=torch.float16, device=dev)
+        out = _new(q, (nq, heads, 128))
     if nq == 0:
         return out
     if nk == 0:  # nobody sees anything
         if clear:
             return out.zero_()
-        k = v = torch.empty((1, kv_heads, 128), dtype=torch.float16, device=dev)
+        k = v = _new(q, (1, kv_heads, 128))
         k_offsets, nk = torch.zeros_like(q_offsets), 1
     q, k, v = _kernel_rows(q), _kernel_rows(k, 1 << 23), _kernel_rows(v, 1 << 23)
-    nbytes = _lib.lib().reskv_packed_workspace_bytes(count, nq, heads, kv_heads, most)
-    work = _workspace(nbytes, dev) if nbytes else None
-    strides = _STRIDES(*q.stride()[:2], *k.stride()[:2], *v.stride()[:2])
-    _launch("reskv_packed_attention", dev, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
-            q_offsets.data_ptr(), k_offsets.data_ptr(), count, nq, nk, heads, kv_heads, strides, scaling, most,
-            int(clear), None if work is None else work.data_ptr(), nbytes)
+    nbytes = _packed_workspace(count, nq, heads, kv_heads, most)
+    work = _workspace(nbytes, q.device) if nbytes else None
+    _launch("reskv_packed_attention", index, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
+            q_offsets.data_ptr(), k_offsets.data_ptr(), count, nq, nk, heads, kv_heads, _strides(q, k, v), scaling, most,
+            clear, None if work is None else work.data_ptr(), nbytes)
     return out

@@ -328,24 +328,50 @@ __global__ void __launch_bounds__(kThreads) gather_kernel(RowArgs A) {
 // ---------------------------------------------------------------------------
 
 constexpr int kWaves = 4;
+// Waves at work on each SIMD.  Three of them fit with 4 query heads, and are no faster: 32 sequences of
+// 16384 tokens 130 us against 124, of 2000 to 8192 tokens 38 against 37.5.
+constexpr int kWavesPerSimd = 2;
 constexpr float kLog2e = 1.4426950408889634f;
 // Weights are exp2(x - m) * 2^14: the largest stays below the largest fp16 number, and a weight
 // is lost to fp16 only when it is below 2^-39 of the largest one.
 constexpr float kWeightBits = 14.0f;
 
+// Work: a column is (sequence, KV head, set of query heads), `blocks` long; the columns lie one behind the
+// other and every wave takes an equal run of blocks, across columns where it has to, so that lengths may
+// differ as they like.  A wave leaves one record (maxima, sums, weighted values of its set's query heads) per
+// column that it works on, at wave + column: both grow along the run, so no two share a place.
 struct AttnArgs {
     Pool pool;
     const uint16_t* q;  // [B, Hq, 128]
     const int32_t* lengths;
     uint16_t* out;      // [B, Hq, 128]
-    float* part;        // [B * Hq, splits, 128]: weighted values
-    float2* stat;       // [B * Hq, splits]: maximum, sum of the weights
-    int Hq, G, sets, splits;
-    int chunk;          // blocks per split
+    float* part;        // [records, heads of a set, 128]: weighted values
+    float2* stat;       // [records, heads of a set]: maximum, sum of the weights
+    int B, Hq, G, sets, columns;  // columns: of a sequence
+    int waves;
     int max_length;
     float c;            // scaling * log2(e)
+
+    __device__ __forceinline__ int blocks(int b) const { return (tokens(b) + kBlock - 1) / kBlock; }
+    __device__ __forceinline__ int tokens(int b) const { return min(max(lengths[b], 0), max_length); }
 };
-constexpr int kRecord = kDim + 2;  // floats of a split's record
+
+// Blocks of a column of each sequence, summed over the sequences before b and over all.
+struct Sums {
+    int before, all;
+};
+__device__ __forceinline__ Sums sum_blocks(const AttnArgs& A, int b) {
+    const int lane = lane_id();
+    int before = 0, all = 0;
+    for (int s = lane; s < A.B; s += kWave) {
+        const int n = A.blocks(s);
+        all += n;
+        before += s < b ? n : 0;
+    }
+    return {wave_sum_int(before), wave_sum_int(all)};
+}
+// Blocks of a wave's run.
+__device__ __forceinline__ int run_length(const AttnArgs& A, int all) { return max((all * A.columns + A.waves - 1) / A.waves, 1); }
 
 __device__ __forceinline__ float swap_sum32(float a, float b) {
     const auto r = __builtin_amdgcn_permlane32_swap((uint32_t)f2i(a), (uint32_t)f2i(b), false, false);
@@ -387,8 +413,7 @@ __device__ __forceinline__ void load_block(Block& b, const char* p, int lane) {
     b.vl[0] = l.x, b.vl[1] = l.y, b.vl[2] = l.z, b.vl[3] = l.w;
 }
 
-// One workgroup per (sequence, KV head, set of 4 HB query heads, split); its four waves take a quarter
-// of the split's blocks each and join at the end.
+// One wave per workgroup; 4 HB query heads.
 //
 // Scores: D[row 4 g + h][token] += Q_g K^T over the four groups, where Q_g has group g's channels of
 // head h in row 4 g + h and zeros elsewhere, so that lane (quarter g, token n) gets the four heads' sums over
@@ -400,29 +425,13 @@ __device__ __forceinline__ void load_block(Block& b, const char* p, int lane) {
 // more product, with P alone.  The product P s is relative to a power of two `e2` not below any scale so far,
 // kept like the softmax's maximum.
 template <int HB>
-__global__ void __launch_bounds__(kThreads, HB == 1 ? 3 : 2) attention_kernel(AttnArgs A) {
+__device__ __forceinline__ void work_on_column(const AttnArgs& A, uint16_t* s_p, int b, int column, int begin, int end) {
     constexpr int kHeads = 4 * HB;
     constexpr int kPitch = kBlock + 8;
-    __shared__ __align__(16) uint16_t s_p[kWaves][kHeads * kPitch];
-    __shared__ float s_o[kWaves][kHeads][kDim];
-    __shared__ float s_m[kWaves][kHeads], s_l[kWaves][kHeads];
-    const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, quarter = lane >> 4;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    int w = blockIdx.x;
-    const int set = w % A.sets;
-    w /= A.sets;
-    const int hk = w % A.pool.heads;
-    w /= A.pool.heads;
-    const int split = w % A.splits, b = w / A.splits;
-    const int h0 = set * kHeads;                    // first query head of the set within the KV head
-    const int heads = min(kHeads, A.G - h0);
+    const int lane = threadIdx.x, n = lane & 15, quarter = lane >> 4;
+    const int hk = column / A.sets, h0 = (column - hk * A.sets) * kHeads;  // KV head, first query head of the set within it
+    const int heads = min(kHeads, A.G - h0), length = A.tokens(b);
     const long row0 = (long)b * A.Hq + hk * A.G + h0;
-    const int length = min(max(A.lengths[b], 0), A.max_length);
-    const int blocks = (length + kBlock - 1) / kBlock;
-    const int first = split * A.chunk, count = min(A.chunk, blocks - first);
-    if (count <= 0 && A.splits > 1) return;  // the merge looks at the sequence's own splits only
-    const int share = count > 0 ? (count + kWaves - 1) / kWaves : 0;
-    const int begin = first + wave * share, end = min(begin + share, first + count);
 
     // Q: lane (n = 4 g + h, quarter): channels 32 g + 8 quarter + [0, 8) of head h, brought to a common power
     // of two so that the sixteenth of an element keeps its bits
@@ -566,7 +575,7 @@ __global__ void __launch_bounds__(kThreads, HB == 1 ? 3 : 2) attention_kernel(At
             for (int tile = 0; tile < 2; ++tile) {
                 const float p14 = __builtin_amdgcn_exp2f(score[hb][tile] - m[hb] + kWeightBits);
                 l[hb] += p14;
-                s_p[wave][(4 * hb + quarter) * kPitch + 16 * tile + n] = f2h(p14);
+                s_p[(4 * hb + quarter) * kPitch + 16 * tile + n] = f2h(p14);
             }
         wave_sync();
         const _Float16 one = (_Float16)(1.0f / e2), sixteenth = (_Float16)(0.0625f / e2);
@@ -576,7 +585,7 @@ __global__ void __launch_bounds__(kThreads, HB == 1 ? 3 : 2) attention_kernel(At
         uint4 ps[HB];
 #pragma unroll
         for (int hb = 0; hb < HB; ++hb) {
-            const half8_t pw = *reinterpret_cast<const half8_t*>(&s_p[wave][(4 * hb + (n & 3)) * kPitch + 8 * quarter]);
+            const half8_t pw = *reinterpret_cast<const half8_t*>(&s_p[(4 * hb + (n & 3)) * kPitch + 8 * quarter]);
             accl[hb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(pw, vlow, accl[hb], 0, 0, 0);
             ps[hb] = __builtin_bit_cast(uint4, pw * vscale);
         }
@@ -595,90 +604,97 @@ __global__ void __launch_bounds__(kThreads, HB == 1 ? 3 : 2) attention_kernel(At
         }
         wave_sync();
     };
-    if (begin < end) {
-        Block x0, x1;
-        fetch_numbers();
-        bool there0 = fetch(x0), there1 = false;
-        for (int blk = begin; blk < end; blk += 2) {
-            if (blk + 1 < end) there1 = fetch(x1);
-            work(x0, blk, there0);
-            if (blk + 1 >= end) break;
-            if (blk + 2 < end) there0 = fetch(x0);
-            work(x1, blk + 1, there1);
-        }
+    Block x0, x1;
+    fetch_numbers();
+    bool there0 = fetch(x0), there1 = false;
+    for (int blk = begin; blk < end; blk += 2) {
+        if (blk + 1 < end) there1 = fetch(x1);
+        work(x0, blk, there0);
+        if (blk + 1 >= end) break;
+        if (blk + 2 < end) there0 = fetch(x0);
+        work(x1, blk + 1, there1);
     }
 
     // lane (quarter g, n): channels 32 g + n and 32 g + 16 + n of the four heads
     const float back = e2 * 0x1p24f;
+    const long record = (long)blockIdx.x + (long)b * A.columns + column;
+    float* const part = A.part + record * kHeads * kDim;
 #pragma unroll
     for (int hb = 0; hb < HB; ++hb) {
         const float total = row_sum16(l[hb]);
-        if (n == 0) {
-            s_m[wave][4 * hb + quarter] = m[hb];
-            s_l[wave][4 * hb + quarter] = total;
-        }
+        if (n == 0) A.stat[record * kHeads + 4 * hb + quarter] = make_float2(m[hb], total);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const float lows = __shfl(accl[hb][i], 16 * quarter + 4 * quarter);  // row 4 g + i, column of group g
 #pragma unroll
             for (int j = 0; j < 2; ++j)
-                s_o[wave][4 * hb + i][32 * quarter + 16 * j + n] = __builtin_fmaf(acc[hb][j][i], back, lows);
+                part[(4 * hb + i) * kDim + 32 * quarter + 16 * j + n] = __builtin_fmaf(acc[hb][j][i], back, lows);
         }
     }
-    __syncthreads();
-    for (int e = tid; e < heads * kDim; e += kThreads) {
-        const int h = e / kDim, ch = e % kDim;
-        float top = s_m[0][h];
-#pragma unroll
-        for (int i = 1; i < kWaves; ++i) top = fmaxf(top, s_m[i][h]);
-        float o = 0.0f, total = 0.0f;
-#pragma unroll
-        for (int i = 0; i < kWaves; ++i) {
-            if (s_l[i][h] == 0.0f) continue;  // no tokens (a NaN goes on)
-            const float a = __builtin_amdgcn_exp2f(s_m[i][h] - top);
-            o += a * s_o[i][h][ch];
-            total += a * s_l[i][h];
-        }
-        if (A.splits == 1) {
-            A.out[(row0 + h) * kDim + ch] = f2h(total == 0.0f ? 0.0f : o / total);
-        } else {
-            const long rec = (row0 + h) * A.splits + split;
-            A.part[rec * kDim + ch] = o;
-            if (ch == 0) A.stat[rec] = make_float2(top, total);
+    wave_sync();
+}
+
+template <int HB>
+__global__ void __launch_bounds__(kWave, kWavesPerSimd) attention_kernel(AttnArgs A) {
+    constexpr int kHeads = 4 * HB;
+    constexpr int kPitch = kBlock + 8;
+    __shared__ __align__(16) uint16_t s_p[kHeads * kPitch];
+    const int all = sum_blocks(A, 0).all, run = run_length(A, all);
+    const int start = (int)blockIdx.x * run;
+    int left = min(run, all * A.columns - start);
+    if (left <= 0) return;
+    const Item it = find_item(start / A.columns, A.B, [&](int s) { return A.blocks(s); });
+    int b = it.seq;
+    if (b < 0) return;
+    int blocks = A.blocks(b), column = (it.index * A.columns + start % A.columns) / blocks;
+    int begin = it.index * A.columns + start % A.columns - column * blocks;
+    for (;;) {
+        const int count = min(left, blocks - begin);
+        work_on_column<HB>(A, s_p, b, column, begin, begin + count);
+        left -= count;
+        if (left <= 0) return;
+        begin = 0;
+        if (++column == A.columns) {
+            column = 0;
+            do {
+                if (++b == A.B) return;
+                blocks = A.blocks(b);
+            } while (blocks == 0);
         }
     }
 }
 
-// Joins the splits of a query head: one workgroup per (sequence, query head).  Lanes take the splits'
-// maxima and sums, 64 at a time; the waves then take every fourth split's 128 channels, two per lane,
-// with eight loads under way (one after the other a split costs a trip to memory: 51 splits took 28 us).
+// Joins the records of a query head: one workgroup per (sequence, query head).  Lanes take the records'
+// maxima and sums, 64 at a time; the waves then take every fourth record's 128 channels, two per lane,
+// with eight loads under way (one after the other a record costs a trip to memory: 51 of them took 28 us).
 __global__ void __launch_bounds__(kThreads) merge_kernel(AttnArgs A) {
     __shared__ float2 s_o[kWaves][kWave];
     const long row = blockIdx.x;
-    const int b = (int)(row / A.Hq), lane = threadIdx.x & 63;
+    const int b = (int)(row / A.Hq), hq = (int)(row - (long)b * A.Hq), lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int length = min(max(A.lengths[b], 0), A.max_length);
-    const int blocks = (length + kBlock - 1) / kBlock;
-    const int splits = min(A.splits, (blocks + A.chunk - 1) / A.chunk);
-    const float2* const stat = A.stat + row * A.splits;
-    const float2* const part = reinterpret_cast<const float2*>(A.part) + row * A.splits * kWave + lane;
+    const int heads = A.G <= 4 ? 4 : 8;  // of a set
+    const int hk = hq / A.G, set = (hq - hk * A.G) / heads, column = hk * A.sets + set;
+    const Sums sums = sum_blocks(A, b);
+    const int blocks = A.blocks(b), run = run_length(A, sums.all);
+    const int start = sums.before * A.columns + column * blocks, first = start / run;
+    const int records = blocks == 0 ? 0 : (start + blocks - 1) / run - first + 1;
+    const long at = ((long)first + (long)b * A.columns + column) * heads + (hq - hk * A.G - set * heads);
+    const float2* const stat = A.stat + at;  // a record's every `heads`
+    const float2* const part = reinterpret_cast<const float2*>(A.part) + at * kWave + lane;
     float top = -__FLT_MAX__;
-    for (int s = lane; s < splits; s += kWave) top = fmaxf(top, stat[s].x);
+    for (int s = lane; s < records; s += kWave) top = fmaxf(top, stat[(long)s * heads].x);
     top = wave_max(top);
     float2 o = make_float2(0.0f, 0.0f);
     float total = 0.0f;
-    for (int s0 = 0; s0 < splits; s0 += kWave) {
-        const float2 ml = s0 + lane < splits ? stat[s0 + lane] : make_float2(0.0f, 0.0f);
+    for (int s0 = 0; s0 < records; s0 += kWave) {
+        const float2 ml = s0 + lane < records ? stat[(long)(s0 + lane) * heads] : make_float2(0.0f, 0.0f);
         const float weight = ml.y == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(ml.x - top);  // no tokens (a NaN goes on)
         total += wave_sum(weight * ml.y);
-        const int n = min(kWave, splits - s0);
+        const int n = min(kWave, records - s0);
         for (int i0 = wave; i0 < n; i0 += 8 * kWaves) {
             float2 r[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int at = min(i0 + kWaves * i, n - 1);
-                r[i] = part[(long)(s0 + at) * kWave];
-            }
+            for (int i = 0; i < 8; ++i) r[i] = part[(long)(s0 + min(i0 + kWaves * i, n - 1)) * heads * kWave];
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const int at = i0 + kWaves * i;
@@ -763,21 +779,18 @@ Pool make_pool(const void* pages, int64_t num_pages, int page_tokens, int Hk, co
 // Blocks that N rows of S sequences can touch: a sequence of n rows touches at most n / 32 + 2.
 long row_items(const int32_t* offsets, int S, long N) { return offsets ? N / kBlock + 2L * S + 1 : (long)S; }
 
-// How many splits, and how many blocks each: about four workgroups for every CU, and no fewer
-// than four blocks (one for each wave).
-struct Split {
-    int splits, chunk;
-};
-constexpr int kTargetGroups = 1024;
+// Sets of query heads of a KV head: of 4, or of 8 when there are more.
 int head_sets(int G) { return G <= 4 ? 1 : (G + 7) / 8; }
-Split choose_split(int B, int Hk, int G, long max_length) {
-    const long blocks = max_length <= 0 ? 1 : (max_length + kBlock - 1) / kBlock;
-    const long groups = (long)B * Hk * head_sets(G);
-    long splits = (kTargetGroups + groups - 1) / groups;
-    if (splits > (blocks + kWaves - 1) / kWaves) splits = (blocks + kWaves - 1) / kWaves;
-    if (splits < 1) splits = 1;
-    const long chunk = (blocks + splits - 1) / splits;
-    return Split{(int)((blocks + chunk - 1) / chunk), (int)chunk};
+int set_heads(int G) { return G <= 4 ? 4 : 8; }
+
+// Waves: as many as the chip holds at once (256 CUs of 4 SIMDs), or one per block when there are fewer.
+long attention_waves(int B, int Hk, int G, long max_length) {
+    const long blocks = (max_length + kBlock - 1) / kBlock * B * Hk * head_sets(G);
+    const long most = 1024L * kWavesPerSimd;
+    return blocks < 1 ? 1 : blocks < most ? blocks : most;
+}
+long attention_records(int B, int Hk, int G, long max_length) {
+    return attention_waves(B, Hk, G, max_length) + (long)B * Hk * head_sets(G);
 }
 
 }  // namespace
@@ -831,9 +844,9 @@ extern "C" int reskv_int4_gather(const void* pages, int64_t num_pages, int page_
 }
 
 extern "C" int64_t reskv_int4_workspace_bytes(int B, int Hq, int Hk, int64_t max_length) {
-    if (B < 1 || Hk < 1 || Hq < 1 || Hq % Hk != 0) return 0;
-    const Split s = choose_split(B, Hk, Hq / Hk, max_length);
-    return s.splits == 1 ? 0 : (int64_t)B * Hq * s.splits * kRecord * 4;
+    if (B < 1 || Hk < 1 || Hq < 1 || Hq % Hk != 0 || max_length < 0 || max_length >= (1LL << 31)) return 0;
+    const int G = Hq / Hk;
+    return (int64_t)attention_records(B, Hk, G, max_length) * set_heads(G) * (kDim + 2) * 4;
 }
 
 extern "C" int reskv_int4_attention(const void* q, const void* pages, int64_t num_pages, int page_tokens,
@@ -844,33 +857,34 @@ extern "C" int reskv_int4_attention(const void* q, const void* pages, int64_t nu
     if (!pool_ok(pages, num_pages, page_tokens, Hk, table, table_width)) return 1;
     RESKV_REQUIRE(B > 0 && Hq > 0 && Hq % Hk == 0, "bad sizes (sequences %d, query heads %d, KV heads %d)", B, Hq, Hk);
     RESKV_REQUIRE(max_length >= 0, "max_length must not be negative");
-    RESKV_REQUIRE(aligned16(q) && aligned16(out), "q and out must be 16-byte aligned");
+    RESKV_REQUIRE(aligned16(q) && aligned16(out) && aligned16(workspace), "tensors must be 16-byte aligned");
     const long most = (long)table_width * page_tokens;
     if (max_length > most) max_length = most;
     const int G = Hq / Hk;
-    const Split s = choose_split(B, Hk, G, max_length);
-    RESKV_REQUIRE(s.splits == 1 || (workspace && workspace_bytes >= reskv_int4_workspace_bytes(B, Hq, Hk, max_length)),
-                  "the workspace is too small");
+    RESKV_REQUIRE(workspace && workspace_bytes >= reskv_int4_workspace_bytes(B, Hq, Hk, max_length), "the workspace is too small");
+    const long columns = (long)Hk * head_sets(G), blocks = (max_length + kBlock - 1) / kBlock;
+    // blocks, records and rows are counted in 32 bits; the last wave's run may end behind the last block
+    RESKV_REQUIRE((long)B * columns * (blocks + 1) < (1L << 30) && (long)B * Hq < (1L << 31),
+                  "too many tokens: sequences x KV heads x blocks of %d must stay below 2^30", kBlock);
+    const long records = attention_records(B, Hk, G, max_length);
     AttnArgs A{};
     A.pool = make_pool(pages, num_pages, page_tokens, Hk, table, table_width);
     A.q = (const uint16_t*)q;
     A.lengths = lengths;
     A.out = (uint16_t*)out;
     A.part = (float*)workspace;
-    A.stat = (float2*)(A.part + (long)B * Hq * s.splits * kDim);
+    A.stat = (float2*)(A.part + records * set_heads(G) * kDim);
+    A.B = B;
     A.Hq = Hq;
     A.G = G;
     A.sets = head_sets(G);
-    A.splits = s.splits;
-    A.chunk = s.chunk;
+    A.columns = (int)columns;
+    A.waves = (int)attention_waves(B, Hk, G, max_length);
     A.max_length = (int)max_length;
     A.c = scaling * kLog2e;
-    const long groups = (long)B * Hk * A.sets * s.splits;
-    RESKV_REQUIRE(groups < (1L << 31) && (long)B * Hq < (1L << 31), "too many (sequence, head) rows");
-    hipLaunchKernelGGL(G <= 4 ? attention_kernel<1> : attention_kernel<2>, dim3((unsigned)groups), dim3(kThreads), 0,
+    hipLaunchKernelGGL(G <= 4 ? attention_kernel<1> : attention_kernel<2>, dim3((unsigned)A.waves), dim3(kWave), 0,
                        (hipStream_t)stream, A);
     if (reskv_host::check_launch("int4 attention_kernel")) return 1;
-    if (s.splits == 1) return 0;
     hipLaunchKernelGGL(merge_kernel, dim3((unsigned)(B * Hq)), dim3(kThreads), 0, (hipStream_t)stream, A);
     return reskv_host::check_launch("int4 merge_kernel");
 }

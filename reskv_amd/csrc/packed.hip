@@ -9,11 +9,12 @@
 //     32-key block, so the softmax needs one lane swap, and the fp16 weights are the
 //     B operand of
 //   O^T = V^T P^T as they are: its 16-key steps take the keys in the order in which
-//     a lane holds them, and V^T comes from the staged rows through LDS transpose
-//     reads of the same keys.
-// Scores, softmax and sums are fp32.  The weights are rounded to fp16 for the second product;
-// they are 2^14 exp2(x - m), so that a weight is lost only when it is below 2^-39 of the
-// largest.
+//     a lane holds them.
+// The 16-byte pieces of a row of K are staged permuted so that the rows' reads fall on different banks; V is staged transposed, in the order of keys of the weights, so that its operand is one
+// 16-byte read (transposing reads run at half the rate).
+// Scores, softmax and sums are fp32.  The weights are rounded to fp16 for the second product, and summed
+// as rounded; they are 2^6 exp2(x - m) with m at most 2^8 below the row's largest score so far, so
+// that a weight is lost only when it is below 2^-30 of the largest.
 #include "serving.h"
 #include "reskv_serving.h"
 
@@ -21,21 +22,18 @@ using namespace reskv;
 
 namespace {
 
-typedef _Float16 half4_t __attribute__((ext_vector_type(4)));
+typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
 typedef _Float16 half8_t __attribute__((ext_vector_type(8)));
 typedef float float16_t __attribute__((ext_vector_type(16)));
-typedef short short4_t __attribute__((ext_vector_type(4)));
-typedef __attribute__((address_space(3))) short4_t lds_short4_t;
 
-constexpr int kWaves = 4;
+constexpr int kWaves = 8;
 constexpr int kThreads = kWaves * kWave;
 constexpr int kWaveRows = 32;
 constexpr int kRows = kWaves * kWaveRows;
-constexpr int kKeys = 64;         // keys per tile
-constexpr int kPitch = kDim + 8;  // halves per staged row (16-byte aligned, rows start on different banks)
-constexpr int kTileHalves = kKeys * kPitch;
-constexpr int kPieces = kKeys * kDim / 8 / kThreads;  // 16-byte pieces of a K (or V) tile per thread
-constexpr float kWeightBits = 14.0f;
+constexpr int kKeys = 64;           // keys per tile
+constexpr int kVPitch = kKeys + 8;  // halves per staged row of V transposed: rows start on different banks
+constexpr float kWeightBits = 6.0f;
+constexpr float kSlack = 8.0f;      // how far a score may pass m before m moves up
 constexpr int kRecord = kDim + 2;
 
 struct PackedArgs {
@@ -56,21 +54,71 @@ __device__ __forceinline__ uint32_t finite_or_zero(uint32_t pair) {
     return pair & (((pair & 0x7C00u) == 0x7C00u ? 0u : 0xFFFFu) | ((pair & 0x7C000000u) == 0x7C000000u ? 0u : 0xFFFF0000u));
 }
 
+// Item `index` of sequence `seq` (see find_item), and the sequence's rows.
+struct Place {
+    Item item;
+    Rows q, k;
+};
+
+__device__ __forceinline__ int row_tiles(const PackedArgs& A, int queries) {
+    return (int)(((long)queries * A.G + kRows - 1) / kRows);
+}
+
+__device__ __forceinline__ Place place_in_order(const PackedArgs& A, int t) {
+    const Item it = find_item(t, A.sequences, [&](int s) { return row_tiles(A, sequence_rows(A.q_offsets, s, A.Nq).count); });
+    if (it.seq < 0) return {it, {0, 0}, {0, 0}};
+    return {it, sequence_rows(A.q_offsets, it.seq, A.Nq), sequence_rows(A.k_offsets, it.seq, A.Nk)};
+}
+
+// Item t in the order of their cost, the dearest first, so that the last ones to start are short: a tile's
+// cost is its number among the sequence's, on top of what the keys in front of the queries cost.  One lane
+// has each sequence; the cost of item t is found by halving, with one sum over the wave per step.
+__device__ __forceinline__ Place place_by_cost(const PackedArgs& A, int t) {
+    const int lane = lane_id();
+    Rows q = {0, 0}, k = {0, 0};
+    if (lane < A.sequences) {
+        q = sequence_rows(A.q_offsets, lane, A.Nq);
+        k = sequence_rows(A.k_offsets, lane, A.Nk);
+    }
+    const int tiles = row_tiles(A, q.count), base = (int)((long)max(k.count - q.count, 0) * A.G / kRows);
+    auto dearer = [&](int cost) __attribute__((always_inline)) {  // items of this lane's sequence that cost more: base + 1 .. base + tiles
+        return min(max(base + tiles - cost, 0), tiles);
+    };
+    const int all = wave_sum_int(tiles);
+    if (t >= all) return {{-1, t - all}, {0, 0}, {0, 0}};
+    int low = 0, high = wave_max_int(base + tiles);  // items dearer than low: more than t; than high: at most t
+    while (high - low > 1) {
+        const int mid = low + (high - low) / 2;
+        if (wave_sum_int(dearer(mid)) > t) low = mid;
+        else high = mid;
+    }
+    // cost `high`: at most one item per sequence
+    const bool has = base < high && high <= base + tiles;
+    const uint64_t with = ballot(has);
+    int nth = t - wave_sum_int(dearer(high));
+    const uint64_t who = ballot(has && (int)lanes_below(with) == nth);
+    if (who == 0) return {{-1, 0}, {0, 0}, {0, 0}};
+    const int seq = __builtin_ctzll(who);
+    auto of = [&](int v) __attribute__((always_inline)) { return __builtin_amdgcn_readlane(v, seq); };
+    return {{seq, high - 1 - of(base)}, {of(q.first), of(q.count)}, {of(k.first), of(k.count)}};
+}
+
 __global__ void __launch_bounds__(kThreads, 2) packed_kernel(PackedArgs A) {
-    __shared__ __align__(16) uint16_t s_kv[2][2][kTileHalves];  // [buffer][K, V]
+    __shared__ __align__(16) uint16_t s_k[2][kKeys * kDim];
+    __shared__ __align__(16) uint16_t s_v[2][kDim * kVPitch];
     __shared__ int s_odd[2];  // the last tile on the diagonal whose V held a value that is not finite, per buffer
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int col = lane & 31, half = lane >> 5;
-    // the KV heads take turns, so that a head's workgroups share an XCD's L2 when there are
-    // 8 heads; the last sequence and a sequence's last rows, which see most keys, come first
+    // the KV heads take turns, so that a head's workgroups share an XCD's L2 when there are 8 heads
     int w = blockIdx.x;
     const int hk = w % A.Hk;
     w /= A.Hk;
-    const int split = w % A.splits, item = A.items - 1 - w / A.splits;
-    const Item it = find_item(item, A.sequences, [&](int s) {
-        return (int)(((long)sequence_rows(A.q_offsets, s, A.Nq).count * A.G + kRows - 1) / kRows);
-    });
+    const int split = w % A.splits, item = w / A.splits;
+    Place at_item;
+    if (A.sequences <= kWave) at_item = place_by_cost(A, item);
+    else at_item = place_in_order(A, item);
+    const Item it = at_item.item;
     if (it.seq < 0) {
         // behind the last item (there is always one such): rows of no sequence
         if (A.clear_rest && split == 0) {
@@ -86,21 +134,20 @@ __global__ void __launch_bounds__(kThreads, 2) packed_kernel(PackedArgs A) {
         }
         return;
     }
-    const Rows qr = sequence_rows(A.q_offsets, it.seq, A.Nq), kr = sequence_rows(A.k_offsets, it.seq, A.Nk);
-    const int nq = qr.count, nk = kr.count, ahead = nk - nq;  // query i sees keys up to i + ahead
-    const long rows = (long)nq * A.G;
-    const long r0 = (long)it.index * kRows + wave * kWaveRows;  // the wave's first row
-    if (it.index < 0 || (long)it.index * kRows >= rows) return;
-    const long r = min(r0 + col, rows - 1);
-    const int query = (int)(r / A.G), head = hk * A.G + (int)(r - (long)query * A.G);
+    const Rows qr = at_item.q, kr = at_item.k;
+    const int nk = kr.count, ahead = nk - qr.count;          // query i sees keys up to i + ahead
+    const int rows = qr.count * A.G, g0 = it.index * kRows;  // the sequence's rows, the workgroup's first
+    const int r0 = g0 + wave * kWaveRows;                    // the wave's first row
+    if (it.index < 0 || g0 >= rows) return;
+    const int r = min(r0 + col, rows - 1);
+    const int query = r / A.G, head = hk * A.G + r - query * A.G;
     const int sees = min(query + ahead + 1, nk);  // keys that this lane's row sees; none when not positive
-    // keys that some row of the wave sees, and that all of them see
-    const int wave_last = min((int)(min(r0 + kWaveRows, rows) - 1) / A.G + ahead + 1, nk);
-    const int wave_all = r0 < rows ? (int)(r0 / A.G) + ahead + 1 : 0;
-    const int wave_any = r0 < rows ? wave_last : 0;
-    const int group_last = min((int)((min((long)(it.index + 1) * kRows, rows) - 1) / A.G) + ahead + 1, nk);
-    const int group_all = (int)((long)it.index * kRows / A.G) + ahead + 1;
-    const int tiles = group_last > 0 ? (group_last + kKeys - 1) / kKeys : 0;
+    // keys that all rows of the wave see, and that some row sees; the same of the workgroup
+    const int wave_all = min(r0, rows - 1) / A.G + ahead + 1;
+    const int wave_any = r0 < rows ? min((min(r0 + kWaveRows, rows) - 1) / A.G + ahead + 1, nk) : 0;
+    const int group_all = g0 / A.G + ahead + 1;
+    const int group_any = min((min(g0 + kRows, rows) - 1) / A.G + ahead + 1, nk);
+    const int tiles = group_any > 0 ? (group_any + kKeys - 1) / kKeys : 0;
     const int per_split = (tiles + A.splits - 1) / A.splits;
     const int tile0 = split * per_split, tile1 = min(tile0 + per_split, tiles);
 
@@ -113,46 +160,54 @@ __global__ void __launch_bounds__(kThreads, 2) packed_kernel(PackedArgs A) {
     }
 
     // Tiles are fetched through range-checked buffer loads without branches: a row behind the
-    // sequence's last key has an offset behind the resource's end and comes as zeros.
-    const uint16_t* kb = A.k + kr.first * A.k_token + hk * A.k_head;
-    const uint16_t* vb = A.v + kr.first * A.v_token + hk * A.v_head;
-    constexpr int kEnd = 0x40000000;
-    uint4 kreg[kPieces], vreg[kPieces];
-    auto fetch = [&](int tile) {
-        const __amdgpu_buffer_rsrc_t kres =
-            __builtin_amdgcn_make_buffer_rsrc((void*)(kb + (long)tile * kKeys * A.k_token), 0, kEnd, 0x00020000);
-        const __amdgpu_buffer_rsrc_t vres =
-            __builtin_amdgcn_make_buffer_rsrc((void*)(vb + (long)tile * kKeys * A.v_token), 0, kEnd, 0x00020000);
-        const int left = nk - tile * kKeys;
+    // sequence's last key lies behind the resource's end and comes as zeros.
+    const int k_step = (int)A.k_token * 2, v_step = (int)A.v_token * 2;  // bytes
+    const char* const v_base = (const char*)(A.v + kr.first * A.v_token + hk * A.v_head);
+    // Each half of the workgroup brings one of the two, in 16-byte pieces.  K: thread (row = part / 16 + 16 i, place =
+    // part % 16) brings piece place ^ row % 16; V: thread (keys 4 (part % 16) + i, piece = part / 16).
+    const int part = tid & 255;
+    const bool first = wave < 4;  // of the two halves
+    const int step = first ? v_step : k_step, apart = first ? v_step : 16 * k_step;
+    const int at = first ? 4 * (part & 15) * v_step + 16 * (part >> 4) : (part >> 4) * k_step + 16 * ((part & 15) ^ (part >> 4));
+    const char* next = (first ? v_base : (const char*)(A.k + kr.first * A.k_token + hk * A.k_head)) + (long)tile0 * kKeys * step;
+    int left = nk - tile0 * kKeys;  // rows from there on
+    uint4 reg[4];
+    auto fetch = [&]() __attribute__((always_inline)) {
+        const __amdgpu_buffer_rsrc_t res = __builtin_amdgcn_make_buffer_rsrc(
+            (void*)next, 0, left > 0 ? (min(left, kKeys) - 1) * step + 2 * kDim : 0, 0x00020000);
 #pragma unroll
-        for (int i = 0; i < kPieces; ++i) {
-            const int p = tid + kThreads * i, row = p >> 4, at = 16 * (p & 15);
-            const int ko = row < left ? row * (int)A.k_token * 2 + at : kEnd;
-            const int vo = row < left ? row * (int)A.v_token * 2 + at : kEnd;
-            kreg[i] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(kres, ko, 0, 0));
-            vreg[i] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(vres, vo, 0, 0));
-        }
+        for (int i = 0; i < 4; ++i) reg[i] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(res, at, i * apart, 0));
+        next += (long)kKeys * step;
+        left -= kKeys;
+    };
+    auto stage_k = [&](int buf) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) reinterpret_cast<uint4*>(s_k[buf])[part + 256 * i] = reg[i];
     };
     // A key that a row does not see has weight 0, and its value must not matter to the row, also
     // when it is infinite or NaN: in the tiles on the diagonal such values are staged as zeros
     // and added to the rows that see them apart.
-    auto stage = [&](int buf, int tile) {
+    auto stage_v = [&](int tile, int buf) __attribute__((always_inline)) {
         if ((tile + 1) * kKeys > group_all) {
             bool odd = false;
 #pragma unroll
-            for (int i = 0; i < kPieces; ++i) {
-                odd = odd || not_finite(vreg[i].x) || not_finite(vreg[i].y) || not_finite(vreg[i].z) || not_finite(vreg[i].w);
-                vreg[i] = make_uint4(finite_or_zero(vreg[i].x), finite_or_zero(vreg[i].y), finite_or_zero(vreg[i].z),
-                                     finite_or_zero(vreg[i].w));
+            for (int i = 0; i < 4; ++i) {
+                odd = odd || not_finite(reg[i].x) || not_finite(reg[i].y) || not_finite(reg[i].z) || not_finite(reg[i].w);
+                reg[i] = make_uint4(finite_or_zero(reg[i].x), finite_or_zero(reg[i].y), finite_or_zero(reg[i].z),
+                                    finite_or_zero(reg[i].w));
             }
             if (odd) s_odd[buf] = tile;
         }
+        // four keys' 8 channels become 8 channels' four keys; key 4 q + i of a group of 16 goes to place 8 (q % 2) + 4 (q / 2) + i
+        const int b = part & 15, q = b & 3;
+        uint16_t* const dst = s_v[buf] + 8 * (part >> 4) * kVPitch + 16 * (b >> 2) + 8 * (q & 1) + 4 * (q >> 1);
+        const uint32_t in[4][4] = {{reg[0].x, reg[0].y, reg[0].z, reg[0].w}, {reg[1].x, reg[1].y, reg[1].z, reg[1].w},
+                                   {reg[2].x, reg[2].y, reg[2].z, reg[2].w}, {reg[3].x, reg[3].y, reg[3].z, reg[3].w}};
 #pragma unroll
-        for (int i = 0; i < kPieces; ++i) {
-            const int p = tid + kThreads * i;
-            const int at = (p >> 4) * kPitch + 8 * (p & 15);
-            *reinterpret_cast<uint4*>(&s_kv[buf][0][at]) = kreg[i];
-            *reinterpret_cast<uint4*>(&s_kv[buf][1][at]) = vreg[i];
+        for (int e = 0; e < 8; ++e) {
+            const uint32_t sel = e & 1 ? 0x07060302u : 0x05040100u;  // the upper or lower halves of two dwords
+            *reinterpret_cast<uint2*>(dst + e * kVPitch) =
+                make_uint2(__builtin_amdgcn_perm(in[1][e >> 1], in[0][e >> 1], sel), __builtin_amdgcn_perm(in[3][e >> 1], in[2][e >> 1], sel));
         }
     };
 
@@ -161,103 +216,125 @@ __global__ void __launch_bounds__(kThreads, 2) packed_kernel(PackedArgs A) {
     for (int db = 0; db < 4; ++db)
 #pragma unroll
         for (int i = 0; i < 16; ++i) acc[db][i] = 0.0f;
-    // log2-domain maximum, and this lane's half of the weights' sum.  The maximum starts at
+    // log2-domain reference of the weights, and this lane's half of their sum.  The reference starts at
     // the lowest finite value: scores of minus infinity then weigh exp2(-inf) = 0, where
-    // against a maximum of minus infinity they would give NaN
+    // against a reference of minus infinity they would give NaN
     float m = -__FLT_MAX__, l = 0.0f;
-    // transpose reads: lane i of a 16-lane row points at key i / 4, channel 4 (i % 4) of
-    // its 4 x 16 block and receives the block's four keys of channel i
-    const int i16 = lane & 15;
-    const int vt = (4 * half + (i16 >> 2)) * kPitch + 16 * ((lane >> 4) & 1) + 4 * (i16 & 3);
+    const half2_t ones = {(_Float16)1.0f, (_Float16)1.0f};
+    // K operand: piece 2 kk + half of row col (and 32 + col, permuted alike) lies at place (2 kk + half) ^ col % 16
+    const int k_read = col * 2 * kDim + 16 * (half ^ (col & 15));  // bytes, of kk = 0
 
-    if (tid < 2) s_odd[tid] = -1;
-    __syncthreads();
-    if (tile0 < tile1) {
-        fetch(tile0);
-        stage(tile0 & 1, tile0);
-    }
-    __syncthreads();
-    for (int tile = tile0; tile < tile1; ++tile) {
-        const int buf = tile & 1, base = tile * kKeys;
-        fetch(tile + 1);
-        if (base < wave_any) {  // wave-uniform: a tile that no row of the wave sees is left out
-            const uint16_t* sk = s_kv[buf][0];
-            const uint16_t* sv = s_kv[buf][1];
-            float16_t s[2];
+    float16_t s[2];
+    auto scores = [&](int buf) __attribute__((always_inline)) {
 #pragma unroll
-            for (int kb2 = 0; kb2 < 2; ++kb2) {
+        for (int kb = 0; kb < 2; ++kb) {
 #pragma unroll
-                for (int i = 0; i < 16; ++i) s[kb2][i] = 0.0f;
+            for (int i = 0; i < 16; ++i) s[kb][i] = 0.0f;
 #pragma unroll
-                for (int kk = 0; kk < 8; ++kk) {
-                    const half8_t kf = *reinterpret_cast<const half8_t*>(sk + (32 * kb2 + col) * kPitch + 16 * kk + 8 * half);
-                    s[kb2] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qf[kk], s[kb2], 0, 0, 0);
-                }
+            for (int kk = 0; kk < 8; ++kk) {
+                const half8_t kf = *reinterpret_cast<const half8_t*>((const char*)s_k[buf] + 64 * kb * kDim + (k_read ^ 32 * kk));
+                s[kb] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qf[kk], s[kb], 0, 0, 0);
             }
-            if (base + kKeys > wave_all) {  // the diagonal
+        }
+        // reads ahead of the products by four
+        __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
 #pragma unroll
-                for (int kb2 = 0; kb2 < 2; ++kb2)
+        for (int i = 0; i < 12; ++i) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        }
+        __builtin_amdgcn_sched_group_barrier(0x008, 4, 0);
+    };
+    auto values = [&](int tile, int buf) __attribute__((always_inline)) {
+        if ((tile + 1) * kKeys > wave_all) {  // the diagonal
+            const int seen = sees - tile * kKeys - 4 * half;
 #pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                        if (base + 32 * kb2 + 8 * (i >> 2) + 4 * half + (i & 3) >= sees) s[kb2][i] = -INFINITY;
+            for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if (32 * kb + 8 * (i >> 2) + (i & 3) >= seen) s[kb][i] = -INFINITY;
+        }
+        float mx = s[0][0];
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[kb][i]);
+        const auto sw = __builtin_amdgcn_permlane32_swap((uint32_t)f2i(mx), (uint32_t)f2i(mx), false, false);
+        mx = fmaxf(i2f((int)sw[0]), i2f((int)sw[1])) * A.c;  // c > 0
+        if (ballot(mx > m + kSlack) != 0) {
+            const float mn = fmaxf(m, mx);
+            const float alpha = __builtin_amdgcn_exp2f(m - mn);
+            m = mn;
+            l *= alpha;
+#pragma unroll
+            for (int db = 0; db < 4; ++db)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) acc[db][i] *= alpha;
+        }
+        const float shift = kWeightBits - m;
+        const uint16_t* const sv = s_v[buf] + col * kVPitch + 8 * half;
+#pragma unroll
+        for (int st = 0; st < 4; ++st) {
+            half8_t pf;  // the weights of a 16-key step, keys in the lane's order
+#pragma unroll
+            for (int i = 0; i < 8; i += 2) {
+                const half2_t p = {(_Float16)__builtin_amdgcn_exp2f(__builtin_fmaf(s[st >> 1][8 * (st & 1) + i], A.c, shift)),
+                                   (_Float16)__builtin_amdgcn_exp2f(__builtin_fmaf(s[st >> 1][8 * (st & 1) + i + 1], A.c, shift))};
+                l = __builtin_amdgcn_fdot2(p, ones, l, false);
+                pf[i] = p[0];
+                pf[i + 1] = p[1];
             }
-            float mx = s[0][0];
 #pragma unroll
-            for (int kb2 = 0; kb2 < 2; ++kb2)
+            for (int db = 0; db < 4; ++db) {
+                const half8_t vf = *reinterpret_cast<const half8_t*>(sv + 32 * db * kVPitch + 16 * st);
+                acc[db] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pf, acc[db], 0, 0, 0);
+            }
+        }
+        // a step's weights between the products of the step before
+        __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
 #pragma unroll
-                for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[kb2][i]);
-            const auto sw = __builtin_amdgcn_permlane32_swap((uint32_t)f2i(mx), (uint32_t)f2i(mx), false, false);
-            mx = fmaxf(i2f((int)sw[0]), i2f((int)sw[1])) * A.c;  // c > 0
-            if (ballot(mx > m) != 0) {
-                const float mn = fmaxf(m, mx);
-                const float alpha = __builtin_amdgcn_exp2f(m - mn);
-                m = mn;
-                l *= alpha;
+        for (int i = 0; i < 12; ++i) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        }
+        __builtin_amdgcn_sched_group_barrier(0x008, 4, 0);
+        if ((tile + 1) * kKeys > group_all && s_odd[buf] == tile) {  // rare: what was staged as zero, to the rows that see it
+            const int last = min((tile + 1) * kKeys, nk);
+            for (int j = tile * kKeys; j < last; ++j) {
+                const uint16_t* row = (const uint16_t*)(v_base + (long)j * v_step);
 #pragma unroll
                 for (int db = 0; db < 4; ++db)
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) acc[db][i] *= alpha;
-            }
-            half8_t pf[4];  // the weights of 16-key steps, keys in the lane's order
-            float sum = 0.0f;
-            const float shift = kWeightBits - m;
-#pragma unroll
-            for (int kb2 = 0; kb2 < 2; ++kb2)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb2][i], A.c, shift));
-                    sum += p;
-                    pf[2 * kb2 + (i >> 3)][i & 7] = (_Float16)p;
-                }
-            l += sum;
-#pragma unroll
-            for (int st = 0; st < 4; ++st)
-#pragma unroll
-                for (int db = 0; db < 4; ++db) {
-                    const uint16_t* src = sv + vt + 16 * st * kPitch + 32 * db;
-                    const half4_t lo = __builtin_bit_cast(half4_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4_t*)src));
-                    const half4_t hi = __builtin_bit_cast(
-                        half4_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4_t*)(src + 8 * kPitch)));
-                    const half8_t vf = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-                    acc[db] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pf[st], acc[db], 0, 0, 0);
-                }
-            if (s_odd[buf] == tile) {  // rare: what was staged as zero, to the rows that see it
-                const int last = min(base + kKeys, nk);
-                for (int j = base; j < last; ++j) {
-                    const uint16_t* row = vb + (long)j * A.v_token;
-#pragma unroll
-                    for (int db = 0; db < 4; ++db)
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) {
-                            const float x = h2f(row[32 * db + 8 * (i >> 2) + 4 * half + (i & 3)]);
-                            if (j < sees && !(fabsf(x) < INFINITY)) acc[db][i] += x;
-                        }
-                }
+                    for (int i = 0; i < 16; ++i) {
+                        const float x = h2f(row[32 * db + 8 * (i >> 2) + 4 * half + (i & 3)]);
+                        if (j < sees && !(fabsf(x) < INFINITY)) acc[db][i] += x;
+                    }
             }
         }
-        if (tile + 1 < tile1) stage(buf ^ 1, tile + 1);  // last read in the tile before, which a barrier ended
+    };
+
+    // The halves take turns: while one multiplies with K, the other does its softmax and multiplies with V, half a
+    // tile behind.  Each brings its share of the next tile in the first of these.
+    if (tid < 2) s_odd[tid] = -1;
+    fetch();
+    if (!first) {
+        stage_k(0);
+        fetch();
+    }
+    __syncthreads();
+    if (!first) __syncthreads();
+    for (int tile = tile0; tile < tile1; ++tile) {
+        const int buf = (tile - tile0) & 1;
+        const bool sees_any = tile * kKeys < wave_any;  // wave-uniform: a tile that no row of the wave sees is left out
+        if (first) stage_v(tile, buf);
+        else stage_k(buf ^ 1);
+        fetch();
+        if (sees_any) scores(buf);
+        __syncthreads();
+        if (sees_any) values(tile, buf);
         __syncthreads();
     }
+    if (first) __syncthreads();
 
     const auto ls = __builtin_amdgcn_permlane32_swap((uint32_t)f2i(l), (uint32_t)f2i(l), false, false);
     const float total = i2f((int)ls[0]) + i2f((int)ls[1]);
@@ -314,14 +391,14 @@ __global__ void __launch_bounds__(kThreads) packed_merge_kernel(PackedArgs A) {
 
 bool aligned16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
 
-// Tiles of 128 rows that S sequences of Nq rows in all can bring, and one that is always free.
+// Tiles of 256 rows that S sequences of Nq rows in all can bring, and one that is always free.
 long packed_items(int S, long Nq, int G) { return Nq * G / kRows + S + 1; }
 
-// Splits of the keys: none while the rows alone give every CU its two workgroups, else up to as
-// many as do, of at least 512 keys each.
+// Splits of the keys: none while the rows alone (half a tile more per sequence, as a rule) give
+// every second CU its workgroup, else as many as give every CU one, of at least 512 keys each.
 int packed_splits(int S, long Nq, int Hk, int G, long max_keys) {
-    const long groups = packed_items(S, Nq, G) * Hk;
-    long splits = 512 / groups;
+    const long groups = (2 * Nq * G / kRows + S + 1) / 2 * Hk;
+    long splits = groups < 1 ? 256 : 256 / groups;
     if (splits > max_keys / 512) splits = max_keys / 512;
     return splits < 1 ? 1 : (int)splits;
 }
@@ -342,10 +419,11 @@ extern "C" int reskv_packed_attention(const void* q, const void* k, const void* 
     RESKV_REQUIRE(S > 0 && Nq > 0 && Nk > 0 && Hk > 0 && Hq > 0 && Hq % Hk == 0,
                   "bad sizes (sequences %d, Nq %ld, Nk %ld, Hq %d, Hk %d)", S, (long)Nq, (long)Nk, Hq, Hk);
     const int G = Hq / Hk;
-    RESKV_REQUIRE(Nq < (1LL << 30) && Nk < (1LL << 30), "too many rows");
+    RESKV_REQUIRE(Nq * G < (1LL << 30) && Nk < (1LL << 30), "too many rows");
     RESKV_REQUIRE(aligned16(q) && aligned16(k) && aligned16(v) && aligned16(out), "tensors must be 16-byte aligned");
     for (int i = 0; i < 6; ++i) RESKV_REQUIRE(strides[i] >= 0 && strides[i] % 8 == 0, "rows must be 16-byte aligned");
     RESKV_REQUIRE(strides[2] < (1 << 23) && strides[4] < (1 << 23), "token strides of k and v must be below 2^23");
+    RESKV_REQUIRE(strides[2] >= kDim && strides[4] >= kDim, "rows of k and v must not overlap");
     RESKV_REQUIRE(scaling > 0.0f, "scaling must be positive");
     const int splits = packed_splits(S, Nq, Hk, G, max_keys);
     RESKV_REQUIRE(splits == 1 || (workspace && workspace_bytes >= reskv_packed_workspace_bytes(S, Nq, Hq, Hk, max_keys)),

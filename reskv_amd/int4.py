@@ -157,10 +157,10 @@ def int4_attention(q, pages, table, lengths, *, scaling=None, max_length=None, o
         q = q.detach().clone(memory_format=torch.contiguous_format)
     most = min(most, width * tokens)
     nbytes = _attention_workspace(sequences, heads, kv_heads, most)
-    work = _workspace(nbytes, q.device) if nbytes else None
+    work = _workspace(nbytes, q.device)
     _launch("reskv_int4_attention", index, q.data_ptr(), pages.data_ptr(), count, tokens, table.data_ptr(), width,
             lengths.data_ptr(), sequences, heads, kv_heads, scaling, most, out.data_ptr(),
-            None if work is None else work.data_ptr(), nbytes)
+            work.data_ptr(), nbytes)
     return out
 
 

@@ -56,11 +56,11 @@ def _launch(name, index, *args):
         _lib.check(status, name)
 
 
-def _kernel_rows(t, most=1 << 62):
+def _kernel_rows(t, least=0, most=1 << 62):
     """t itself when its rows of 128 channels can be read in place (16-byte aligned; token stride
-    below ``most``), else a contiguous copy."""
+    from ``least`` to below ``most``), else a contiguous copy."""
     token, head, channel = t.stride()
-    if channel == 1 and not (token | head) & 7 and token < most and not t.data_ptr() & 15:
+    if channel == 1 and not (token | head) & 7 and least <= token < most and not t.data_ptr() & 15:
         return t
     return t.detach().clone(memory_format=torch.contiguous_format)
 
@@ -133,7 +133,7 @@ def packed_attention(q, k, v, q_offsets, k_offsets=None, *, scaling=None, max_ke
             return out.zero_()
         k = v = _new(q, (1, kv_heads, 128))
         k_offsets, nk = torch.zeros_like(q_offsets), 1
-    q, k, v = _kernel_rows(q), _kernel_rows(k, 1 << 23), _kernel_rows(v, 1 << 23)
+    q, k, v = _kernel_rows(q), _kernel_rows(k, 128, 1 << 23), _kernel_rows(v, 128, 1 << 23)
     nbytes = _packed_workspace(count, nq, heads, kv_heads, most)
     work = _workspace(nbytes, q.device) if nbytes else None
     _launch("reskv_packed_attention", index, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),

@@ -32,6 +32,7 @@ constexpr int kWaveRows = 32;
 constexpr int kRows = kWaves * kWaveRows;
 constexpr int kKeys = 64;           // keys per tile
 constexpr int kVPitch = kKeys + 8;  // halves per staged row of V transposed: rows start on different banks
+constexpr int kOutPitch = kDim + 8;
 constexpr float kWeightBits = 6.0f;
 constexpr float kSlack = 8.0f;      // how far a score may pass m before m moves up
 constexpr int kRecord = kDim + 2;
@@ -106,6 +107,7 @@ __device__ __forceinline__ Place place_by_cost(const PackedArgs& A, int t) {
 __global__ void __launch_bounds__(kThreads, 2) packed_kernel(PackedArgs A) {
     __shared__ __align__(16) uint16_t s_k[2][kKeys * kDim];
     __shared__ __align__(16) uint16_t s_v[2][kDim * kVPitch];
+    __shared__ __align__(16) uint16_t s_out[kWaves][kWaveRows * kOutPitch];
     __shared__ int s_odd[2];  // the last tile on the diagonal whose V held a value that is not finite, per buffer
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -322,7 +324,9 @@ __global__ void __launch_bounds__(kThreads, 2) packed_kernel(PackedArgs A) {
         fetch();
     }
     __syncthreads();
-    if (!first) __syncthreads();
+    // (both halves meet 2 n + 1 barriers for n tiles: the second one starts a barrier later and needs none
+    // behind its last tile)
+    if (!first && tile0 < tile1) __syncthreads();
     for (int tile = tile0; tile < tile1; ++tile) {
         const int buf = (tile - tile0) & 1;
         const bool sees_any = tile * kKeys < wave_any;  // wave-uniform: a tile that no row of the wave sees is left out
@@ -332,15 +336,13 @@ __global__ void __launch_bounds__(kThreads, 2) packed_kernel(PackedArgs A) {
         if (sees_any) scores(buf);
         __syncthreads();
         if (sees_any) values(tile, buf);
-        __syncthreads();
+        if (first || tile + 1 < tile1) __syncthreads();
     }
-    if (first) __syncthreads();
-
     const auto ls = __builtin_amdgcn_permlane32_swap((uint32_t)f2i(l), (uint32_t)f2i(l), false, false);
     const float total = i2f((int)ls[0]) + i2f((int)ls[1]);
-    if (r0 + col >= rows) return;
-    const long row = ((long)qr.first + query) * A.Hq + head;
     if (A.splits > 1) {
+        if (r0 + col >= rows) return;
+        const long row = ((long)qr.first + query) * A.Hq + head;
         float* rec = A.part + ((long)split * A.Nq * A.Hq + row) * kRecord;
 #pragma unroll
         for (int db = 0; db < 4; ++db)
@@ -350,8 +352,9 @@ __global__ void __launch_bounds__(kThreads, 2) packed_kernel(PackedArgs A) {
         if (half == 0) *reinterpret_cast<float2*>(rec + kDim) = make_float2(m, total);
         return;
     }
+    // through the LDS to whole rows: sixteen lanes write one
     const float inv = total == 0.0f ? 0.0f : 1.0f / total;
-    uint16_t* dst = A.out + row * kDim;
+    uint16_t* const mine = s_out[wave];
 #pragma unroll
     for (int db = 0; db < 4; ++db)
 #pragma unroll
@@ -360,8 +363,17 @@ __global__ void __launch_bounds__(kThreads, 2) packed_kernel(PackedArgs A) {
 #pragma unroll
             for (int e = 0; e < 2; ++e)
                 word[e] = (uint32_t)f2h(acc[db][4 * j + 2 * e] * inv) | ((uint32_t)f2h(acc[db][4 * j + 2 * e + 1] * inv) << 16);
-            *reinterpret_cast<uint2*>(dst + 32 * db + 8 * j + 4 * half) = make_uint2(word[0], word[1]);
+            *reinterpret_cast<uint2*>(mine + col * kOutPitch + 32 * db + 8 * j + 4 * half) = make_uint2(word[0], word[1]);
         }
+    wave_sync();
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const int n = 4 * i + (lane >> 4), at_row = r0 + n;
+        if (at_row >= rows) break;
+        const int of = at_row / A.G;
+        reinterpret_cast<uint4*>(A.out + (((long)qr.first + of) * A.Hq + hk * A.G + at_row - of * A.G) * kDim)[lane & 15] =
+            *reinterpret_cast<const uint4*>(mine + n * kOutPitch + 8 * (lane & 15));
+    }
 }
 
 // Joins the splits: one wave per (query, head) row, two channels per lane.  Rows of no

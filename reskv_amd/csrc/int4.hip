@@ -332,9 +332,10 @@ constexpr int kWaves = 4;
 // 16384 tokens 130 us against 124, of 2000 to 8192 tokens 38 against 37.5.
 constexpr int kWavesPerSimd = 2;
 constexpr float kLog2e = 1.4426950408889634f;
-// Weights are exp2(x - m) * 2^14: the largest stays below the largest fp16 number, and a weight
-// is lost to fp16 only when it is below 2^-39 of the largest one.
-constexpr float kWeightBits = 14.0f;
+// Weights are exp2(x - m) * 2^10 with m at most 2^4 below the largest score so far: the largest stays below the
+// largest fp16 number, and a weight is lost to fp16 only when it is below 2^-35 of the largest one.
+constexpr float kWeightBits = 10.0f;
+constexpr float kSlack = 4.0f;  // how far a score may pass m before m moves up
 
 // Work: a column is (sequence, KV head, set of query heads), `blocks` long; the columns lie one behind the
 // other and every wave takes an equal run of blocks, across columns where it has to, so that lengths may
@@ -485,6 +486,7 @@ __device__ __forceinline__ void work_on_column(const AttnArgs& A, uint16_t* s_p,
         for (int i = 0; i < 2; ++i) acc[hb][i] = {0.0f, 0.0f, 0.0f, 0.0f};
     }
     float e2 = 0x1p-14f;  // not below any scale so far
+    half2_t f1 = {(_Float16)0x1p14f, (_Float16)0x1p14f}, f16 = {(_Float16)0x1p10f, (_Float16)0x1p10f};  // its reciprocal, and a sixteenth
 
     // The wave's blocks, one after the other, each fetched while the one before is worked on.  Page
     // numbers come 64 at a time, one per lane.
@@ -544,14 +546,16 @@ __device__ __forceinline__ void work_on_column(const AttnArgs& A, uint16_t* s_p,
         const float top_scale = fmaxf((float)tops[0], (float)tops[1]);
         bool grow = top_scale > e2;
 #pragma unroll
-        for (int hb = 0; hb < HB; ++hb) grow |= fmaxf(score[hb][0], score[hb][1]) > m[hb];
+        for (int hb = 0; hb < HB; ++hb) grow |= fmaxf(score[hb][0], score[hb][1]) > m[hb] + kSlack;
         if (ballot(grow) != 0) {
             const float ts = wave_max(top_scale);
             float shrink = 1.0f;
             if (ts > e2) {
-                const float up = ldexpf(1.0f, ilogbf(ts) + 1);
-                shrink = e2 / up;
+                const float up = ldexpf(1.0f, ilogbf(ts) + 1), down = ldexpf(1.0f, -1 - ilogbf(ts));
+                shrink = e2 * down;
                 e2 = up;
+                f1[0] = f1[1] = (_Float16)down;
+                f16[0] = f16[1] = (_Float16)(0.0625f * down);
             }
 #pragma unroll
             for (int hb = 0; hb < HB; ++hb) {
@@ -573,13 +577,12 @@ __device__ __forceinline__ void work_on_column(const AttnArgs& A, uint16_t* s_p,
         for (int hb = 0; hb < HB; ++hb)
 #pragma unroll
             for (int tile = 0; tile < 2; ++tile) {
-                const float p14 = __builtin_amdgcn_exp2f(score[hb][tile] - m[hb] + kWeightBits);
-                l[hb] += p14;
-                s_p[(4 * hb + quarter) * kPitch + 16 * tile + n] = f2h(p14);
+                const float p = __builtin_amdgcn_exp2f(score[hb][tile] - m[hb] + kWeightBits);
+                l[hb] += p;
+                s_p[(4 * hb + quarter) * kPitch + 16 * tile + n] = f2h(p);
             }
         wave_sync();
-        const _Float16 one = (_Float16)(1.0f / e2), sixteenth = (_Float16)(0.0625f / e2);
-        const half8_t factor = {one, one, sixteenth, sixteenth, one, one, sixteenth, sixteenth};
+        const half8_t factor = {f1[0], f1[1], f16[0], f16[1], f1[0], f1[1], f16[0], f16[1]};
         const half8_t vscale = __builtin_bit_cast(half8_t, make_uint4(x.vs[0], x.vs[1], x.vs[2], x.vs[3])) * factor;
         const half8_t vlow = __builtin_bit_cast(half8_t, make_uint4(x.vl[0], x.vl[1], x.vl[2], x.vl[3]));
         uint4 ps[HB];

@@ -67,7 +67,9 @@ def _kernel_rows(t, least=0, most=1 << 62):
 
 def _new(like, shape):
     """An fp16 tensor (a plain one, also for a subclass's ``like``) on the GPU of ``like``."""
-    return like.new_empty(shape) if type(like) is torch.Tensor else torch.empty(shape, dtype=torch.float16, device=like.device)
+    if type(like) is torch.Tensor:
+        return torch.empty_like(like) if like.shape == shape and like.is_contiguous() else like.new_empty(shape)
+    return torch.empty(shape, dtype=torch.float16, device=like.device)
 
 
 _pack = [struct.Struct(f"{2 * n}q").pack for n in range(4)]

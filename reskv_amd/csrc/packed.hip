@@ -169,8 +169,12 @@ __global__ void __launch_bounds__(kThreads, 2) packed_kernel(PackedArgs A) {
     // part % 16) brings piece place ^ row % 16; V: thread (keys 4 (part % 16) + i, piece = part / 16).
     const int part = tid & 255;
     const bool first = wave < 4;  // of the two halves
-    const int step = first ? v_step : k_step, apart = first ? v_step : 16 * k_step;
-    const int at = first ? 4 * (part & 15) * v_step + 16 * (part >> 4) : (part >> 4) * k_step + 16 * ((part & 15) ^ (part >> 4));
+    const int step = first ? v_step : k_step;
+    int at[4];  // the whole offset in the lane's: a scalar one would be left out of the range check
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        at[i] = first ? (4 * (part & 15) + i) * v_step + 16 * (part >> 4)
+                      : (16 * i + (part >> 4)) * k_step + 16 * ((part & 15) ^ (part >> 4));
     const char* next = (first ? v_base : (const char*)(A.k + kr.first * A.k_token + hk * A.k_head)) + (long)tile0 * kKeys * step;
     int left = nk - tile0 * kKeys;  // rows from there on
     uint4 reg[4];
@@ -178,7 +182,7 @@ __global__ void __launch_bounds__(kThreads, 2) packed_kernel(PackedArgs A) {
         const __amdgpu_buffer_rsrc_t res = __builtin_amdgcn_make_buffer_rsrc(
             (void*)next, 0, left > 0 ? (min(left, kKeys) - 1) * step + 2 * kDim : 0, 0x00020000);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) reg[i] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(res, at, i * apart, 0));
+        for (int i = 0; i < 4; ++i) reg[i] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(res, at[i], 0, 0));
         next += (long)kKeys * step;
         left -= kKeys;
     };

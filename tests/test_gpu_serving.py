@@ -137,6 +137,19 @@ def test_packed_attention_what_is_not_seen_does_not_matter(device, bad):
         assert np.isnan(got[150:160]).all()
 
 
+@pytest.mark.parametrize("n", [1, 15, 16, 17, 62, 63, 65, 100])
+def test_packed_attention_reads_no_row_of_another_sequence(device, n):
+    """A sequence between others of NaN keys and values, for every place where its last tile may end."""
+    q, k, v = packed_inputs(40 + n, [n], [n], 2, 4)
+    want, bound = ref.packed(*(x.astype(np.float64) for x in (q, k, v)), [0, n], [0, n], 128 ** -0.5)
+    bad = np.full((70, 2, 128), np.nan, np.float16)
+    k, v = (np.concatenate((bad, x, bad)) for x in (k, v))
+    q = np.concatenate((q, np.ones((1, 8, 128), np.float16)))
+    got = packed_attention(gpu(q), gpu(k), gpu(v), i32([0, 0, n, n + 1]), i32([0, 70, 70 + n, 140 + n]))
+    check(got[:n], want, bound)
+    assert torch.isnan(got[n:].float()).all()
+
+
 def test_packed_attention_rows_of_no_sequence(device):
     nq = [20, 33]
     q, k, v = packed_inputs(6, [70], [70], 2, 4)

@@ -153,14 +153,6 @@ __global__ void __launch_bounds__(kThreads, 2) packed_kernel(PackedArgs A) {
     const int per_split = (tiles + A.splits - 1) / A.splits;
     const int tile0 = split * per_split, tile1 = min(tile0 + per_split, tiles);
 
-    // Q operand: lane (col, half) holds its row, channels 16 kk + 8 half + [0, 8)
-    half8_t qf[8];
-    {
-        const uint4* src = reinterpret_cast<const uint4*>(A.q + (qr.first + query) * A.q_token + head * A.q_head);
-#pragma unroll
-        for (int kk = 0; kk < 8; ++kk) qf[kk] = __builtin_bit_cast(half8_t, src[2 * kk + half]);
-    }
-
     // Tiles are fetched through range-checked buffer loads without branches: a row behind the
     // sequence's last key lies behind the resource's end and comes as zeros.
     const int k_step = (int)A.k_token * 2, v_step = (int)A.v_token * 2;  // bytes
@@ -186,6 +178,16 @@ __global__ void __launch_bounds__(kThreads, 2) packed_kernel(PackedArgs A) {
         next += (long)kKeys * step;
         left -= kKeys;
     };
+    fetch();  // before Q, so that the first tile does not wait for it
+
+    // Q operand: lane (col, half) holds its row, channels 16 kk + 8 half + [0, 8)
+    half8_t qf[8];
+    {
+        const uint4* src = reinterpret_cast<const uint4*>(A.q + (qr.first + query) * A.q_token + head * A.q_head);
+#pragma unroll
+        for (int kk = 0; kk < 8; ++kk) qf[kk] = __builtin_bit_cast(half8_t, src[2 * kk + half]);
+    }
+
     auto stage_k = [&](int buf) __attribute__((always_inline)) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) reinterpret_cast<uint4*>(s_k[buf])[part + 256 * i] = reg[i];
@@ -322,7 +324,6 @@ __global__ void __launch_bounds__(kThreads, 2) packed_kernel(PackedArgs A) {
     // The halves take turns: while one multiplies with K, the other does its softmax and multiplies with V, half a
     // tile behind.  Each brings its share of the next tile in the first of these.
     if (tid < 2) s_odd[tid] = -1;
-    fetch();
     if (!first) {
         stage_k(0);
         fetch();

@@ -110,7 +110,8 @@ def int4_gather(pages, table, starts, offsets, rows, out=None):
     k, v = (None, None) if clear else out
     index = _same_gpu(pages, table, starts, offsets, k, v)
     if clear:
-        k, v = (torch.empty((rows, heads, 128), dtype=torch.float16, device=pages.device) for _ in range(2))
+        shape = (rows, heads, 128)
+        k, v = pages.new_empty(shape, dtype=torch.float16), pages.new_empty(shape, dtype=torch.float16)
     if rows == 0:
         return k, v
     if sequences == 0:

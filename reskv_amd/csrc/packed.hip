@@ -48,9 +48,6 @@ struct PackedArgs {
     float c;                     // scaling * log2(e)
 };
 
-__device__ __forceinline__ bool not_finite(uint32_t pair) {
-    return ((pair & 0x7C00u) == 0x7C00u) || ((pair & 0x7C000000u) == 0x7C000000u);
-}
 __device__ __forceinline__ uint32_t finite_or_zero(uint32_t pair) {
     return pair & (((pair & 0x7C00u) == 0x7C00u ? 0u : 0xFFFFu) | ((pair & 0x7C000000u) == 0x7C000000u ? 0u : 0xFFFF0000u));
 }
@@ -197,14 +194,20 @@ __global__ void __launch_bounds__(kThreads, 2) packed_kernel(PackedArgs A) {
     // and added to the rows that see them apart.
     auto stage_v = [&](int tile, int buf) __attribute__((always_inline)) {
         if ((tile + 1) * kKeys > group_all) {
-            bool odd = false;
+            half2_t zero = {(_Float16)0.0f, (_Float16)0.0f}, sum = zero;  // NaN when a value is not finite
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                odd = odd || not_finite(reg[i].x) || not_finite(reg[i].y) || not_finite(reg[i].z) || not_finite(reg[i].w);
-                reg[i] = make_uint4(finite_or_zero(reg[i].x), finite_or_zero(reg[i].y), finite_or_zero(reg[i].z),
-                                    finite_or_zero(reg[i].w));
+                const uint32_t w[4] = {reg[i].x, reg[i].y, reg[i].z, reg[i].w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sum += __builtin_bit_cast(half2_t, w[e]) * zero;
             }
-            if (odd) s_odd[buf] = tile;
+            if (!(sum[0] == 0.0f && sum[1] == 0.0f)) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    reg[i] = make_uint4(finite_or_zero(reg[i].x), finite_or_zero(reg[i].y), finite_or_zero(reg[i].z),
+                                        finite_or_zero(reg[i].w));
+                s_odd[buf] = tile;
+            }
         }
         // four keys' 8 channels become 8 channels' four keys; key 4 q + i of a group of 16 goes to place 8 (q % 2) + 4 (q / 2) + i
         const int b = part & 15, q = b & 3;

@@ -41,10 +41,11 @@ struct PackedArgs {
     const uint16_t *q, *k, *v;
     uint16_t* out;               // [Nq, Hq, 128]
     const int32_t *q_offsets, *k_offsets;
-    float* part;                 // [splits, Nq * Hq, 130]: o[128], m, l
+    float* part;                 // split keys: [workgroups, 256 rows, 130]: o[128], m, l
     long q_token, q_head, k_token, k_head, v_token, v_head;  // strides in halves
     int sequences, Nq, Nk, Hq, Hk, G;
-    int items, splits, clear_rest;
+    int items, clear_rest;
+    int groups;                  // split keys: workgroups of a KV head
     float c;                     // scaling * log2(e)
 };
 
@@ -71,13 +72,7 @@ __device__ __forceinline__ Place place_in_order(const PackedArgs& A, int t) {
 // Item t in the order of their cost, the dearest first, so that the last ones to start are short: a tile's
 // cost is its number among the sequence's, on top of what the keys in front of the queries cost.  One lane
 // has each sequence; the cost of item t is found by halving, with one sum over the wave per step.
-__device__ __forceinline__ Place place_by_cost(const PackedArgs& A, int t) {
-    const int lane = lane_id();
-    Rows q = {0, 0}, k = {0, 0};
-    if (lane < A.sequences) {
-        q = sequence_rows(A.q_offsets, lane, A.Nq);
-        k = sequence_rows(A.k_offsets, lane, A.Nk);
-    }
+__device__ __forceinline__ Place place_by_cost(const PackedArgs& A, int t, const Rows& q, const Rows& k) {
     const int tiles = row_tiles(A, q.count), base = (int)((long)max(k.count - q.count, 0) * A.G / kRows);
     auto dearer = [&](int cost) __attribute__((always_inline)) {  // items of this lane's sequence that cost more: base + 1 .. base + tiles
         return min(max(base + tiles - cost, 0), tiles);
@@ -101,6 +96,26 @@ __device__ __forceinline__ Place place_by_cost(const PackedArgs& A, int t) {
     return {{seq, high - 1 - of(base)}, {of(q.first), of(q.count)}, {of(k.first), of(k.count)}};
 }
 
+// Split keys.  A sequence's tiles of rows are each shared by `parts` workgroups, which take as many keys each
+// as lets all workgroups together stay within `groups`: the longest sequences are split most, and no split is
+// much longer than another.  Lane s has sequence s; `first` counts the workgroups of those before it.
+struct Parts {
+    int tiles, parts, first;
+};
+constexpr int kMinPart = 8;  // tiles of keys
+__device__ __forceinline__ Parts split_parts(const PackedArgs& A, const Rows& q, const Rows& k) {
+    const int tiles = row_tiles(A, q.count), key_tiles = tiles > 0 ? (k.count + kKeys - 1) / kKeys : 0;
+    int low = kMinPart - 1, high = max(wave_max_int(key_tiles), kMinPart);  // high is long enough, low is not
+    while (high - low > 1) {
+        const int mid = low + (high - low) / 2;
+        if (wave_sum_int(tiles * max((key_tiles + mid - 1) / mid, 1)) <= A.groups) high = mid;
+        else low = mid;
+    }
+    const int parts = max((key_tiles + high - 1) / high, 1);
+    return {tiles, parts, wave_scan_int(tiles * parts) - tiles * parts};
+}
+
+template <bool SPLIT>
 __global__ void __launch_bounds__(kThreads, 2) packed_kernel(PackedArgs A) {
     __shared__ __align__(16) uint16_t s_k[2][kKeys * kDim];
     __shared__ __align__(16) uint16_t s_v[2][kDim * kVPitch];
@@ -113,27 +128,47 @@ __global__ void __launch_bounds__(kThreads, 2) packed_kernel(PackedArgs A) {
     int w = blockIdx.x;
     const int hk = w % A.Hk;
     w /= A.Hk;
-    const int split = w % A.splits, item = w / A.splits;
-    Place at_item;
-    if (A.sequences <= kWave) at_item = place_by_cost(A, item);
-    else at_item = place_in_order(A, item);
-    const Item it = at_item.item;
-    if (it.seq < 0) {
-        // behind the last item (there is always one such): rows of no sequence
-        if (A.clear_rest && split == 0) {
-            const int begin = min(max(A.q_offsets[0], 0), A.Nq);
-            const int end = min(max(A.q_offsets[A.sequences], begin), A.Nq);
-            const int spares = A.items - (item - it.index), rest = begin + A.Nq - end;
-            const int per_row = A.G * 16;  // 16-byte pieces of a query's heads in the group
-            for (long i = (long)it.index * kThreads + tid; i < (long)rest * per_row; i += (long)spares * kThreads) {
-                const int r = (int)(i / per_row), at = (int)(i - (long)r * per_row);
-                const long row = r < begin ? r : end + r - begin;
-                reinterpret_cast<uint4*>(A.out + (row * A.Hq + (long)hk * A.G) * kDim)[at] = make_uint4(0, 0, 0, 0);
-            }
+    auto clear_rest = [&](int spare, int spares) __attribute__((always_inline)) {  // rows of no sequence
+        const int begin = min(max(A.q_offsets[0], 0), A.Nq);
+        const int end = min(max(A.q_offsets[A.sequences], begin), A.Nq);
+        const int rest = begin + A.Nq - end;
+        const int per_row = A.G * 16;  // 16-byte pieces of a query's heads in the group
+        for (long i = (long)spare * kThreads + tid; i < (long)rest * per_row; i += (long)spares * kThreads) {
+            const int r = (int)(i / per_row), at = (int)(i - (long)r * per_row);
+            const long row = r < begin ? r : end + r - begin;
+            reinterpret_cast<uint4*>(A.out + (row * A.Hq + (long)hk * A.G) * kDim)[at] = make_uint4(0, 0, 0, 0);
         }
-        return;
+    };
+    Rows q_rows = {0, 0}, k_rows = {0, 0};  // of sequence `lane`
+    if (A.sequences <= kWave && lane < A.sequences) {
+        q_rows = sequence_rows(A.q_offsets, lane, A.Nq);
+        k_rows = sequence_rows(A.k_offsets, lane, A.Nk);
     }
-    const Rows qr = at_item.q, kr = at_item.k;
+    Item it;
+    Rows qr, kr;  // of the workgroup's sequence, kept in scalar registers
+    int split = 0, parts = 1;
+    if (SPLIT) {
+        if (A.clear_rest) clear_rest(w, A.groups);
+        const Parts p = split_parts(A, q_rows, k_rows);
+        const uint64_t who = ballot(w >= p.first && w < p.first + p.tiles * p.parts);
+        if (who == 0) return;
+        it.seq = __builtin_ctzll(who);
+        parts = __builtin_amdgcn_readlane(p.parts, it.seq);
+        const int n = w - __builtin_amdgcn_readlane(p.first, it.seq);
+        it.index = n / parts;
+        split = n - it.index * parts;
+        qr = {__builtin_amdgcn_readlane(q_rows.first, it.seq), __builtin_amdgcn_readlane(q_rows.count, it.seq)};
+        kr = {__builtin_amdgcn_readlane(k_rows.first, it.seq), __builtin_amdgcn_readlane(k_rows.count, it.seq)};
+    } else {
+        const Place place = A.sequences <= kWave ? place_by_cost(A, w, q_rows, k_rows) : place_in_order(A, w);
+        it = place.item;
+        if (it.seq < 0) {  // behind the last item (there is always one such)
+            if (A.clear_rest) clear_rest(it.index, A.items - (w - it.index));
+            return;
+        }
+        qr = place.q;
+        kr = place.k;
+    }
     const int nk = kr.count, ahead = nk - qr.count;          // query i sees keys up to i + ahead
     const int rows = qr.count * A.G, g0 = it.index * kRows;  // the sequence's rows, the workgroup's first
     const int r0 = g0 + wave * kWaveRows;                    // the wave's first row
@@ -147,7 +182,7 @@ __global__ void __launch_bounds__(kThreads, 2) packed_kernel(PackedArgs A) {
     const int group_all = g0 / A.G + ahead + 1;
     const int group_any = min((min(g0 + kRows, rows) - 1) / A.G + ahead + 1, nk);
     const int tiles = group_any > 0 ? (group_any + kKeys - 1) / kKeys : 0;
-    const int per_split = (tiles + A.splits - 1) / A.splits;
+    const int per_split = (tiles + parts - 1) / parts;
     const int tile0 = split * per_split, tile1 = min(tile0 + per_split, tiles);
 
     // Tiles are fetched through range-checked buffer loads without branches: a row behind the
@@ -348,10 +383,9 @@ __global__ void __launch_bounds__(kThreads, 2) packed_kernel(PackedArgs A) {
     }
     const auto ls = __builtin_amdgcn_permlane32_swap((uint32_t)f2i(l), (uint32_t)f2i(l), false, false);
     const float total = i2f((int)ls[0]) + i2f((int)ls[1]);
-    if (A.splits > 1) {
+    if (SPLIT && parts > 1) {
         if (r0 + col >= rows) return;
-        const long row = ((long)qr.first + query) * A.Hq + head;
-        float* rec = A.part + ((long)split * A.Nq * A.Hq + row) * kRecord;
+        float* rec = A.part + ((long)blockIdx.x * kRows + wave * kWaveRows + col) * kRecord;
 #pragma unroll
         for (int db = 0; db < 4; ++db)
 #pragma unroll
@@ -384,23 +418,38 @@ __global__ void __launch_bounds__(kThreads, 2) packed_kernel(PackedArgs A) {
     }
 }
 
-// Joins the splits: one wave per (query, head) row, two channels per lane.  Rows of no
-// sequence have no records and are left to the attention's own workgroups.
+// Joins the splits: one wave per (query, head) row, two channels per lane.  Rows of no sequence, and of
+// sequences that are not split, are done already.
 __global__ void __launch_bounds__(kThreads) packed_merge_kernel(PackedArgs A) {
     const int lane = threadIdx.x & 63;
-    const long row = (long)blockIdx.x * kWaves + (threadIdx.x >> 6), all = (long)A.Nq * A.Hq;
-    if (row >= all) return;
-    const int query = (int)(row / A.Hq);
-    if (query < A.q_offsets[0] || query >= A.q_offsets[A.sequences]) return;
+    const long row = (long)blockIdx.x * kWaves + (threadIdx.x >> 6);
+    const int query = __builtin_amdgcn_readfirstlane((int)(row / A.Hq)), head = __builtin_amdgcn_readfirstlane((int)(row - (long)query * A.Hq));
+    if (query >= A.Nq) return;
+    Rows q = {0, 0}, k = {0, 0};
+    if (lane < A.sequences) {
+        q = sequence_rows(A.q_offsets, lane, A.Nq);
+        k = sequence_rows(A.k_offsets, lane, A.Nk);
+    }
+    const Parts p = split_parts(A, q, k);
+    const uint64_t who = ballot(query >= q.first && query < q.first + q.count);
+    if (who == 0) return;
+    const int seq = __builtin_ctzll(who), parts = __builtin_amdgcn_readlane(p.parts, seq);
+    if (parts == 1) return;
+    const int hk = head / A.G, r = (query - __builtin_amdgcn_readlane(q.first, seq)) * A.G + head - hk * A.G, tile = r / kRows;
+    // workgroup (first + tile * parts + split) * Hk + hk has the row's record of a split
+    const int group = __builtin_amdgcn_readlane(p.first, seq) + tile * parts;
+    if (group + parts > A.groups) return;
+    const float* const rec = A.part + (((long)group * A.Hk + hk) * kRows + r - tile * kRows) * kRecord;
+    const long apart = (long)A.Hk * kRows * kRecord;
     float top = -__FLT_MAX__;
-    for (int s = 0; s < A.splits; ++s) top = fmaxf(top, A.part[(s * all + row) * kRecord + kDim]);
+    for (int s = lane; s < parts; s += kWave) top = fmaxf(top, rec[s * apart + kDim]);
+    top = wave_max(top);
     float o0 = 0.0f, o1 = 0.0f, total = 0.0f;
-    for (int s = 0; s < A.splits; ++s) {
-        const float* rec = A.part + (s * all + row) * kRecord;
-        const float l = rec[kDim + 1];
-        if (l == 0.0f) continue;  // no keys (a NaN goes on)
-        const float a = __builtin_amdgcn_exp2f(rec[kDim] - top);
-        const float2 o = reinterpret_cast<const float2*>(rec)[lane];
+#pragma unroll 4
+    for (int s = 0; s < parts; ++s) {
+        const float l = rec[s * apart + kDim + 1];
+        const float2 o = reinterpret_cast<const float2*>(rec + s * apart)[lane];
+        const float a = l == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(rec[s * apart + kDim] - top);  // no keys (a NaN goes on)
         o0 += a * o.x;
         o1 += a * o.y;
         total += a * l;
@@ -414,21 +463,22 @@ bool aligned16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
 // Tiles of 256 rows that S sequences of Nq rows in all can bring, and one that is always free.
 long packed_items(int S, long Nq, int G) { return Nq * G / kRows + S + 1; }
 
-// Splits of the keys: none while the rows alone (half a tile more per sequence, as a rule) give
-// every second CU its workgroup, else as many as give every CU one, of at least 512 keys each.
-int packed_splits(int S, long Nq, int Hk, int G, long max_keys) {
-    const long groups = (2 * Nq * G / kRows + S + 1) / 2 * Hk;
-    long splits = groups < 1 ? 256 : 256 / groups;
-    if (splits > max_keys / 512) splits = max_keys / 512;
-    return splits < 1 ? 1 : (int)splits;
+// Whether the keys are split: while the rows alone leave CUs without a workgroup and there are keys for more
+// than one part.  Workgroups of a KV head then (one per CU in all), else 0.  Where the keys are mostly
+// the queries' own, the tiles differ in length and the longest of them bounds the time less than a second
+// pass over the records costs, so that half of the CUs have to be free: one prompt of 1600 tokens (200 workgroups)
+// 50 us whole and 73 split; 20 chunks of 10 tokens after 5000 (160 workgroups) 86 whole and 71 split.
+constexpr int kGroups = 256;
+int split_groups(int S, long Nq, int Hk, int G, long max_keys) {
+    const long groups = packed_items(S, Nq, G) * Hk * (max_keys < 4 * Nq ? 2 : 1);
+    return S <= kWave && groups <= kGroups && max_keys >= 2 * kMinPart * kKeys ? kGroups / Hk : 0;
 }
 
 }  // namespace
 
 extern "C" int64_t reskv_packed_workspace_bytes(int S, int64_t Nq, int Hq, int Hk, int64_t max_keys) {
-    if (S < 1 || Nq < 1 || Hk < 1 || Hq < 1 || Hq % Hk != 0) return 0;
-    const int splits = packed_splits(S, Nq, Hk, Hq / Hk, max_keys);
-    return splits == 1 ? 0 : (int64_t)splits * Nq * Hq * kRecord * 4;
+    if (S < 1 || Nq < 1 || Hk < 1 || Hq < 1 || Hq % Hk != 0 || Nq >= (1LL << 30)) return 0;
+    return (int64_t)split_groups(S, Nq, Hk, Hq / Hk, max_keys) * Hk * kRows * kRecord * 4;
 }
 
 extern "C" int reskv_packed_attention(const void* q, const void* k, const void* v, void* out, const int32_t* q_offsets,
@@ -445,8 +495,8 @@ extern "C" int reskv_packed_attention(const void* q, const void* k, const void* 
     RESKV_REQUIRE(strides[2] < (1 << 23) && strides[4] < (1 << 23), "token strides of k and v must be below 2^23");
     RESKV_REQUIRE(strides[2] >= kDim && strides[4] >= kDim, "rows of k and v must not overlap");
     RESKV_REQUIRE(scaling > 0.0f, "scaling must be positive");
-    const int splits = packed_splits(S, Nq, Hk, G, max_keys);
-    RESKV_REQUIRE(splits == 1 || (workspace && workspace_bytes >= reskv_packed_workspace_bytes(S, Nq, Hq, Hk, max_keys)),
+    const int split = split_groups(S, Nq, Hk, G, max_keys);
+    RESKV_REQUIRE(!split || (workspace && workspace_bytes >= reskv_packed_workspace_bytes(S, Nq, Hq, Hk, max_keys)),
                   "the workspace is too small");
     PackedArgs A{};
     A.q = (const uint16_t*)q;
@@ -469,14 +519,15 @@ extern "C" int reskv_packed_attention(const void* q, const void* k, const void* 
     A.Hk = Hk;
     A.G = G;
     const long items = packed_items(S, Nq, G);
-    RESKV_REQUIRE(items * Hk * splits < (1L << 31), "too many rows");
+    RESKV_REQUIRE(items * Hk < (1L << 31), "too many rows");
     A.items = (int)items;
-    A.splits = splits;
+    A.groups = split;
     A.clear_rest = clear_rest;
     A.c = scaling * 1.4426950408889634f;
-    hipLaunchKernelGGL(packed_kernel, dim3((unsigned)(items * Hk * splits)), dim3(kThreads), 0, (hipStream_t)stream, A);
+    hipLaunchKernelGGL(split ? packed_kernel<true> : packed_kernel<false>, dim3((unsigned)(split ? split * Hk : items * Hk)),
+                       dim3(kThreads), 0, (hipStream_t)stream, A);
     if (reskv_host::check_launch("packed_kernel")) return 1;
-    if (splits == 1) return 0;
+    if (!split) return 0;
     const long rows = (long)Nq * Hq;
     hipLaunchKernelGGL(packed_merge_kernel, dim3((unsigned)((rows + kWaves - 1) / kWaves)), dim3(kThreads), 0,
                        (hipStream_t)stream, A);

@@ -332,9 +332,9 @@ constexpr int kWaves = 4;
 // 16384 tokens 130 us against 124, of 2000 to 8192 tokens 38 against 37.5.
 constexpr int kWavesPerSimd = 2;
 constexpr float kLog2e = 1.4426950408889634f;
-// Weights are exp2(x - m) * 2^10 with m at most 2^4 below the largest score so far: the largest stays below the
+// Weights are exp2(x - m) * 2^11 with m at most 2^4 below the largest score so far: the largest stays below the
 // largest fp16 number, and a weight is lost to fp16 only when it is below 2^-35 of the largest one.
-constexpr float kWeightBits = 10.0f;
+constexpr float kWeightBits = 11.0f;
 constexpr float kSlack = 4.0f;  // how far a score may pass m before m moves up
 
 // Work: a column is (sequence, KV head, set of query heads), `blocks` long; the columns lie one behind the

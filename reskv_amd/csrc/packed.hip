@@ -1,6 +1,6 @@
 // Causal attention of packed sequences of different lengths (include/reskv_serving.h).
 //
-// One workgroup of four waves per 128 rows of one KV head and sequence, where row r is
+// One workgroup of eight waves per 256 rows of one KV head and sequence, where row r is
 // query r / G of query head r % G of the head's group: short sequences and single tokens then fill
 // the matrix cores' columns with the heads of a group, whatever G is.  A wave owns 32
 // rows; keys are taken 64 at a time from double-buffered LDS.
@@ -10,11 +10,24 @@
 //     B operand of
 //   O^T = V^T P^T as they are: its 16-key steps take the keys in the order in which
 //     a lane holds them.
-// The 16-byte pieces of a row of K are staged permuted so that the rows' reads fall on different banks; V is staged transposed, in the order of keys of the weights, so that its operand is one
-// 16-byte read (transposing reads run at half the rate).
+// The 16-byte pieces of a row of K are staged permuted, so that the rows' reads fall on different banks; V is
+// staged transposed, in the order of keys of the weights, so that its operand is one 16-byte read
+// (transposing reads run at half the rate).
+//
+// The two halves of a workgroup, a wave of each on every SIMD, are half a tile apart: one multiplies with K while
+// the other does its softmax and multiplies with V, so that the vector ALU (about 830 cycles a tile and wave, half of
+// them exponentials) works beside the matrix cores (1024).  One workgroup of 256 rows also fetches and stages K and V
+// half as often as two of 128: 16384 tokens, 32 / 8 heads, 2.14 ms (1030 TFLOP/s) against 2.41 with four waves
+// that take no turns; 24 prompts of 16 to 1500 tokens 112 us against 120.
+//
+// Bound: long prompts by the power that the matrix cores may draw: with zeros in K and V the same
+// instructions take 1.75 ms, as a library product of 16384 x 16384 matrices makes 1761 TFLOP/s of zeros and 1277 of
+// random numbers.  Short ones also by what a workgroup does alone on its CU at its start and end (about 6 us: its place
+// among the offsets, the first tiles, its rows' way out).
+//
 // Scores, softmax and sums are fp32.  The weights are rounded to fp16 for the second product, and summed
-// as rounded; they are 2^6 exp2(x - m) with m at most 2^8 below the row's largest score so far, so
-// that a weight is lost only when it is below 2^-30 of the largest.
+// as rounded; they are 2^9 exp2(x - m) with m at most 2^6 below the row's largest score so far, so
+// that a weight is lost only when it is below 2^-33 of the largest.
 #include "serving.h"
 #include "reskv_serving.h"
 
@@ -33,8 +46,8 @@ constexpr int kRows = kWaves * kWaveRows;
 constexpr int kKeys = 64;           // keys per tile
 constexpr int kVPitch = kKeys + 8;  // halves per staged row of V transposed: rows start on different banks
 constexpr int kOutPitch = kDim + 8;
-constexpr float kWeightBits = 6.0f;
-constexpr float kSlack = 8.0f;      // how far a score may pass m before m moves up
+constexpr float kWeightBits = 9.0f;
+constexpr float kSlack = 6.0f;      // how far a score may pass m before m moves up: weights stay within 2^15
 constexpr int kRecord = kDim + 2;
 
 struct PackedArgs {

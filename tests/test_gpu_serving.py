@@ -68,6 +68,8 @@ def packed_inputs(seed, nq, nk, kv, gqa):
     ([50, 9], [20, 8], 1, 2),             # more queries than keys: the first see nothing
     ([2, 1], [1500, 1111], 1, 4),         # keys split over workgroups
     ([130], [900], 2, 5),
+    ([3, 70, 1, 0], [2600, 1030, 700, 512], 3, 4),  # some split, some not
+    ([20], None, 1, 64),
 ])
 def test_packed_attention(device, nq, nk, kv, gqa):
     nk = nq if nk is None else nk
@@ -194,6 +196,21 @@ def test_packed_attention_small_weights_add_up(device):
     want, bound = ref.packed(*(x.astype(np.float64) for x in (q, k, v)), [0, 1], [0, n], 128 ** -0.5)
     assert want.min() > 1e-5
     check(packed_attention(gpu(q), gpu(k), gpu(v), i32([0, 1]), i32([0, n])), want, bound)
+
+
+def test_packed_attention_far_rows(device):
+    """Keys, values and queries behind 2^31 elements of their tensors."""
+    r = rng(50)
+    n, far = 90, (1 << 31) // (2 * 128) + 1000
+    q, k, v = half(r, n, 2, 128), half(r, n, 2, 128), half(r, n, 2, 128)
+    qf, kf, vf = (torch.empty(far + n, 2, 128, dtype=torch.float16, device="cuda") for _ in range(3))
+    for t, x in zip((qf, kf, vf), (q, k, v)):
+        t[far:] = gpu(x)
+    want, bound = ref.packed(*(x.astype(np.float64) for x in (q, k, v)), [0, n], [0, n], 128 ** -0.5)
+    for most in (n, 4096):
+        got = packed_attention(qf, kf, vf, i32([far, far + n]), max_keys=most)
+        check(got[far:], want, bound)
+        assert (got[:5] == 0).all() and (got[far - 5: far] == 0).all()
 
 
 # ---------------------------------------------------------------------------
@@ -450,6 +467,67 @@ def test_int4_attention_lengths_are_clamped(device):
     assert (int4_attention(gpu(q), pool, table, i32([64, 64]), max_length=0) == 0).all()
 
 
+@pytest.mark.parametrize("gqa", [2, 8])
+def test_int4_attention_many_sequences(device, gqa):
+    """More sequences than a wave has lanes, empty ones among them."""
+    r = rng(25)
+    lengths = [int(n) for n in r.integers(0, 90, 150)]
+    lengths[0] = lengths[70] = lengths[71] = lengths[149] = 0
+    pool, table, k, v = filled(r, lengths, 1, 32)
+    q = half(r, 150, gqa, 128)
+    want, bound = expected(q, k, v, lengths)
+    got = int4_attention(gpu(q), pool, table, i32(lengths))
+    check(got, want, bound)
+    assert torch.equal(int4_attention(gpu(q), pool, table, i32(lengths)), got)  # the same every time
+
+
+@pytest.mark.parametrize("gqa,entries", [(4, 200001), (8, 150000)])
+def test_int4_attention_long_tables(device, gqa, entries):
+    """Runs of blocks over more page numbers than a wave holds at a time: a few pages that a long
+    sequence uses again and again, so that a token counts as often as its page is named."""
+    r = rng(26)
+    pages = 40
+    pool, once, k, v = filled(r, [32 * pages], 1, 32)
+    order = once.cpu().numpy()[0]
+    named = r.choice(pages, entries, p=(w := r.random(pages) ** 3) / w.sum())
+    table = gpu(order[named].astype(np.int32)[None])
+    length = 32 * entries - 11
+    q = half(r, 1, gqa, 128)
+    times = np.repeat(np.bincount(named, minlength=pages), 32).astype(np.float64)
+    times[32 * named[-1] + 21: 32 * named[-1] + 32] -= 1  # the last page's last eleven tokens
+    (kd, ka), (vd, va) = ref.stored(k), ref.stored(v)
+    want, bound = np.zeros((1, gqa, 128)), np.zeros((1, gqa, 128))
+    for h in range(gqa):
+        s = 128 ** -0.5 * kd[:, 0] @ q[0, h].astype(np.float64)
+        w = times * np.exp(s - s.max())
+        w /= w.sum()
+        want[0, h] = w @ vd[:, 0]
+        delta = 160 * ref.H32 * 128 ** -0.5 * (ka[:, 0] @ np.abs(q[0, h].astype(np.float64))).max()
+        # as in ref.sequence, with fp32 sums over 2^12 blocks of a wave, whose errors add up at most linearly
+        bound[0, h] = (w @ va[:, 0]) * (2 * ref.H16 + 2 * delta + 2.0 ** -12) * 1.01 + ref.H16 * np.abs(want[0, h]) + 2.0 ** -24
+    check(int4_attention(gpu(q), pool, table, i32([length])), want, bound)
+
+
+def test_far_pages(device):
+    """Pages behind 2^32 bytes of the pool."""
+    r = rng(27)
+    kv, page = 8, 64
+    count = (1 << 32) // (kv * page * 160) + 200
+    pool = torch.zeros(count, kv, page * 160, dtype=torch.uint8, device="cuda")
+    lengths = [100, 64]
+    table = i32([count - 1, 5, count - 7, count - 2]).view(2, 2)
+    k, v = half(r, 164, kv, 128), half(r, 164, kv, 128)
+    off = i32(offsets(lengths))
+    int4_append(pool, table, i32([0, 0]), gpu(k), gpu(v), off)
+    got = int4_gather(pool, table, i32([0, 0]), off, 164)
+    for x, y in zip((k, v), got):
+        assert np.array_equal(y.cpu().numpy(), ref.stored(x)[0].astype(np.float32).astype(np.float16))
+    q = half(r, 2, 32, 128)
+    check(int4_attention(gpu(q), pool, table, i32(lengths)), *expected(q, k, v, lengths))
+    copy_pages(pool, [count - 1, count - 7], [count - 3, 9])
+    assert torch.equal(pool[count - 1], pool[count - 3]) and torch.equal(pool[count - 7], pool[9])
+
+
 # ---------------------------------------------------------------------------
 # page copies, streams, graphs
 # ---------------------------------------------------------------------------
@@ -552,6 +630,30 @@ def test_packed_attention_in_a_graph(device):
             q.copy_(gpu(half(r, 400, 8, 128)))
             graph.replay()
             assert torch.equal(out, packed_attention(q, k, v, off, max_keys=most))
+
+
+def test_two_graphs_share_a_pool(device):
+    """Workspaces of two captured graphs, of one memory pool, replayed in turns."""
+    r = rng(34)
+    lengths = [700, 45]
+    pool, table, k, v = filled(r, lengths, 2, 64)
+    lens, off = i32(lengths), i32([0, 2, 3])
+    qa, qb = (torch.zeros(n, 8, 128, dtype=torch.float16, device="cuda") for n in (2, 3))
+    kg, vg, ko = gpu(k), gpu(v), i32(offsets(lengths))
+    first = lambda: int4_attention(qa, pool, table, lens)  # noqa: E731
+    second = lambda: packed_attention(qb, kg, vg, off, ko, max_keys=4096)  # noqa: E731
+    first(), second()
+    handle, graphs, outs = torch.cuda.graph_pool_handle(), [], []
+    for f in (first, second):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1], pool=handle):
+            outs.append(f())
+    for turn in range(6):
+        for t in (qa, qb):
+            t.copy_(gpu(half(r, *t.shape)))
+        for i in (0, 1) if turn % 2 else (1, 0):
+            graphs[i].replay()
+            assert torch.equal(outs[i], (first, second)[i]())
 
 
 def test_served_batch(device):

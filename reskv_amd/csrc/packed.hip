@@ -431,44 +431,47 @@ __global__ void __launch_bounds__(kThreads, 2) packed_kernel(PackedArgs A) {
     }
 }
 
-// Joins the splits: one wave per (query, head) row, two channels per lane.  Rows of no sequence, and of
+// Joins the splits: four (query, head) rows per wave, two channels per lane.  Rows of no sequence, and of
 // sequences that are not split, are done already.
+constexpr int kMergeRows = 4;
 __global__ void __launch_bounds__(kThreads) packed_merge_kernel(PackedArgs A) {
     const int lane = threadIdx.x & 63;
-    const long row = (long)blockIdx.x * kWaves + (threadIdx.x >> 6);
-    const int query = __builtin_amdgcn_readfirstlane((int)(row / A.Hq)), head = __builtin_amdgcn_readfirstlane((int)(row - (long)query * A.Hq));
-    if (query >= A.Nq) return;
+    const long row0 = ((long)blockIdx.x * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) * kMergeRows;
+    if (row0 >= (long)A.Nq * A.Hq) return;
     Rows q = {0, 0}, k = {0, 0};
     if (lane < A.sequences) {
         q = sequence_rows(A.q_offsets, lane, A.Nq);
         k = sequence_rows(A.k_offsets, lane, A.Nk);
     }
     const Parts p = split_parts(A, q, k);
-    const uint64_t who = ballot(query >= q.first && query < q.first + q.count);
-    if (who == 0) return;
-    const int seq = __builtin_ctzll(who), parts = __builtin_amdgcn_readlane(p.parts, seq);
-    if (parts == 1) return;
-    const int hk = head / A.G, r = (query - __builtin_amdgcn_readlane(q.first, seq)) * A.G + head - hk * A.G, tile = r / kRows;
-    // workgroup (first + tile * parts + split) * Hk + hk has the row's record of a split
-    const int group = __builtin_amdgcn_readlane(p.first, seq) + tile * parts;
-    if (group + parts > A.groups) return;
-    const float* const rec = A.part + (((long)group * A.Hk + hk) * kRows + r - tile * kRows) * kRecord;
-    const long apart = (long)A.Hk * kRows * kRecord;
-    float top = -__FLT_MAX__;
-    for (int s = lane; s < parts; s += kWave) top = fmaxf(top, rec[s * apart + kDim]);
-    top = wave_max(top);
-    float o0 = 0.0f, o1 = 0.0f, total = 0.0f;
-#pragma unroll 4
-    for (int s = 0; s < parts; ++s) {
-        const float l = rec[s * apart + kDim + 1];
-        const float2 o = reinterpret_cast<const float2*>(rec + s * apart)[lane];
-        const float a = l == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(rec[s * apart + kDim] - top);  // no keys (a NaN goes on)
-        o0 += a * o.x;
-        o1 += a * o.y;
-        total += a * l;
+    for (int i = 0; i < kMergeRows; ++i) {
+        const long row = row0 + i;
+        const int query = (int)(row / A.Hq), head = (int)(row - (long)query * A.Hq);
+        const uint64_t who = ballot(query < A.Nq && query >= q.first && query < q.first + q.count);
+        if (who == 0) continue;
+        const int seq = __builtin_ctzll(who), parts = __builtin_amdgcn_readlane(p.parts, seq);
+        const int hk = head / A.G, r = (query - __builtin_amdgcn_readlane(q.first, seq)) * A.G + head - hk * A.G, tile = r / kRows;
+        // workgroup (first + tile * parts + split) * Hk + hk has the row's record of a split
+        const int group = __builtin_amdgcn_readlane(p.first, seq) + tile * parts;
+        if (parts == 1 || group + parts > A.groups) continue;
+        const float* const rec = A.part + (((long)group * A.Hk + hk) * kRows + r - tile * kRows) * kRecord;
+        const long apart = (long)A.Hk * kRows * kRecord;
+        float top = -__FLT_MAX__;
+        for (int s = lane; s < parts; s += kWave) top = fmaxf(top, rec[s * apart + kDim]);
+        top = wave_max(top);
+        float o0 = 0.0f, o1 = 0.0f, total = 0.0f;
+#pragma unroll 8
+        for (int s = 0; s < parts; ++s) {
+            const float l = rec[s * apart + kDim + 1];
+            const float2 o = reinterpret_cast<const float2*>(rec + s * apart)[lane];
+            const float a = l == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(rec[s * apart + kDim] - top);  // no keys (a NaN goes on)
+            o0 += a * o.x;
+            o1 += a * o.y;
+            total += a * l;
+        }
+        const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+        reinterpret_cast<uint32_t*>(A.out + row * kDim)[lane] = (uint32_t)f2h(o0 * inv) | ((uint32_t)f2h(o1 * inv) << 16);
     }
-    const float inv = total == 0.0f ? 0.0f : 1.0f / total;
-    reinterpret_cast<uint32_t*>(A.out + row * kDim)[lane] = (uint32_t)f2h(o0 * inv) | ((uint32_t)f2h(o1 * inv) << 16);
 }
 
 bool aligned16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
@@ -542,7 +545,7 @@ extern "C" int reskv_packed_attention(const void* q, const void* k, const void* 
     if (reskv_host::check_launch("packed_kernel")) return 1;
     if (!split) return 0;
     const long rows = (long)Nq * Hq;
-    hipLaunchKernelGGL(packed_merge_kernel, dim3((unsigned)((rows + kWaves - 1) / kWaves)), dim3(kThreads), 0,
+    hipLaunchKernelGGL(packed_merge_kernel, dim3((unsigned)((rows + kWaves * kMergeRows - 1) / (kWaves * kMergeRows))), dim3(kThreads), 0,
                        (hipStream_t)stream, A);
     return reskv_host::check_launch("packed_merge_kernel");
 }

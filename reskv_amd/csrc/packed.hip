@@ -54,7 +54,9 @@ struct PackedArgs {
     const uint16_t *q, *k, *v;
     uint16_t* out;               // [Nq, Hq, 128]
     const int32_t *q_offsets, *k_offsets;
-    float* part;                 // split keys: [workgroups, 256 rows, 130]: o[128], m, l
+    float* part;                 // split keys: [workgroups, 256 rows, 128]: weighted values
+    float2* stat;                // [workgroups, 256 rows]: reference of the weights, their sum
+    int32_t* length;             // tiles of keys of a part
     long q_token, q_head, k_token, k_head, v_token, v_head;  // strides in halves
     int sequences, Nq, Nk, Hq, Hk, G;
     int items, clear_rest;
@@ -116,15 +118,20 @@ struct Parts {
     int tiles, parts, first;
 };
 constexpr int kMinPart = 8;  // tiles of keys
-__device__ __forceinline__ Parts split_parts(const PackedArgs& A, const Rows& q, const Rows& k) {
-    const int tiles = row_tiles(A, q.count), key_tiles = tiles > 0 ? (k.count + kKeys - 1) / kKeys : 0;
-    int low = kMinPart - 1, high = max(wave_max_int(key_tiles), kMinPart);  // high is long enough, low is not
+__device__ __forceinline__ int key_tiles(const Rows& q, const Rows& k) { return q.count > 0 ? (k.count + kKeys - 1) / kKeys : 0; }
+// Tiles of keys of a part.
+__device__ __forceinline__ int part_length(const PackedArgs& A, const Rows& q, const Rows& k) {
+    const int tiles = row_tiles(A, q.count), keys = key_tiles(q, k);
+    int low = kMinPart - 1, high = max(wave_max_int(keys), kMinPart);  // high is long enough, low is not
     while (high - low > 1) {
         const int mid = low + (high - low) / 2;
-        if (wave_sum_int(tiles * max((key_tiles + mid - 1) / mid, 1)) <= A.groups) high = mid;
+        if (wave_sum_int(tiles * max((keys + mid - 1) / mid, 1)) <= A.groups) high = mid;
         else low = mid;
     }
-    const int parts = max((key_tiles + high - 1) / high, 1);
+    return high;
+}
+__device__ __forceinline__ Parts split_parts(const PackedArgs& A, const Rows& q, const Rows& k, int length) {
+    const int tiles = row_tiles(A, q.count), parts = max((key_tiles(q, k) + length - 1) / length, 1);
     return {tiles, parts, wave_scan_int(tiles * parts) - tiles * parts};
 }
 
@@ -162,7 +169,9 @@ __global__ void __launch_bounds__(kThreads, 2) packed_kernel(PackedArgs A) {
     int split = 0, parts = 1;
     if (SPLIT) {
         if (A.clear_rest) clear_rest(w, A.groups);
-        const Parts p = split_parts(A, q_rows, k_rows);
+        const int length = part_length(A, q_rows, k_rows);
+        if (blockIdx.x == 0 && tid == 0) *A.length = length;  // for the merge
+        const Parts p = split_parts(A, q_rows, k_rows, length);
         const uint64_t who = ballot(w >= p.first && w < p.first + p.tiles * p.parts);
         if (who == 0) return;
         it.seq = __builtin_ctzll(who);
@@ -398,13 +407,14 @@ __global__ void __launch_bounds__(kThreads, 2) packed_kernel(PackedArgs A) {
     const float total = i2f((int)ls[0]) + i2f((int)ls[1]);
     if (SPLIT && parts > 1) {
         if (r0 + col >= rows) return;
-        float* rec = A.part + ((long)blockIdx.x * kRows + wave * kWaveRows + col) * kRecord;
+        const long record = (long)blockIdx.x * kRows + wave * kWaveRows + col;
+        float* rec = A.part + record * kDim;
 #pragma unroll
         for (int db = 0; db < 4; ++db)
 #pragma unroll
             for (int i = 0; i < 16; i += 2)
                 *reinterpret_cast<float2*>(rec + 32 * db + 8 * (i >> 2) + 4 * half + (i & 3)) = make_float2(acc[db][i], acc[db][i + 1]);
-        if (half == 0) *reinterpret_cast<float2*>(rec + kDim) = make_float2(m, total);
+        if (half == 0) A.stat[record] = make_float2(m, total);
         return;
     }
     // through the LDS to whole rows: sixteen lanes write one
@@ -431,9 +441,9 @@ __global__ void __launch_bounds__(kThreads, 2) packed_kernel(PackedArgs A) {
     }
 }
 
-// Joins the splits: four (query, head) rows per wave, two channels per lane.  Rows of no sequence, and of
+// Joins the splits: two (query, head) rows per wave, two channels per lane.  Rows of no sequence, and of
 // sequences that are not split, are done already.
-constexpr int kMergeRows = 4;
+constexpr int kMergeRows = 2;
 __global__ void __launch_bounds__(kThreads) packed_merge_kernel(PackedArgs A) {
     const int lane = threadIdx.x & 63;
     const long row0 = ((long)blockIdx.x * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) * kMergeRows;
@@ -443,7 +453,7 @@ __global__ void __launch_bounds__(kThreads) packed_merge_kernel(PackedArgs A) {
         q = sequence_rows(A.q_offsets, lane, A.Nq);
         k = sequence_rows(A.k_offsets, lane, A.Nk);
     }
-    const Parts p = split_parts(A, q, k);
+    const Parts p = split_parts(A, q, k, *A.length);
     for (int i = 0; i < kMergeRows; ++i) {
         const long row = row0 + i;
         const int query = (int)(row / A.Hq), head = (int)(row - (long)query * A.Hq);
@@ -454,20 +464,28 @@ __global__ void __launch_bounds__(kThreads) packed_merge_kernel(PackedArgs A) {
         // workgroup (first + tile * parts + split) * Hk + hk has the row's record of a split
         const int group = __builtin_amdgcn_readlane(p.first, seq) + tile * parts;
         if (parts == 1 || group + parts > A.groups) continue;
-        const float* const rec = A.part + (((long)group * A.Hk + hk) * kRows + r - tile * kRows) * kRecord;
-        const long apart = (long)A.Hk * kRows * kRecord;
+        const long record = ((long)group * A.Hk + hk) * kRows + r - tile * kRows, apart = (long)A.Hk * kRows;
+        const float2* const rec = reinterpret_cast<const float2*>(A.part) + record * kWave + lane;
         float top = -__FLT_MAX__;
-        for (int s = lane; s < parts; s += kWave) top = fmaxf(top, rec[s * apart + kDim]);
+        for (int s = lane; s < parts; s += kWave) top = fmaxf(top, A.stat[record + s * apart].x);
         top = wave_max(top);
         float o0 = 0.0f, o1 = 0.0f, total = 0.0f;
-#pragma unroll 8
-        for (int s = 0; s < parts; ++s) {
-            const float l = rec[s * apart + kDim + 1];
-            const float2 o = reinterpret_cast<const float2*>(rec + s * apart)[lane];
-            const float a = l == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(rec[s * apart + kDim] - top);  // no keys (a NaN goes on)
-            o0 += a * o.x;
-            o1 += a * o.y;
-            total += a * l;
+        for (int s0 = 0; s0 < parts; s0 += 8) {
+            float2 o[8], ml[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const long at = min(s0 + j, parts - 1) * apart;
+                o[j] = rec[at * kWave];
+                ml[j] = A.stat[record + at];
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                if (s0 + j >= parts || ml[j].y == 0.0f) continue;  // no keys (a NaN goes on)
+                const float a = __builtin_amdgcn_exp2f(ml[j].x - top);
+                o0 += a * o[j].x;
+                o1 += a * o[j].y;
+                total += a * ml[j].y;
+            }
         }
         const float inv = total == 0.0f ? 0.0f : 1.0f / total;
         reinterpret_cast<uint32_t*>(A.out + row * kDim)[lane] = (uint32_t)f2h(o0 * inv) | ((uint32_t)f2h(o1 * inv) << 16);
@@ -494,7 +512,8 @@ int split_groups(int S, long Nq, int Hk, int G, long max_keys) {
 
 extern "C" int64_t reskv_packed_workspace_bytes(int S, int64_t Nq, int Hq, int Hk, int64_t max_keys) {
     if (S < 1 || Nq < 1 || Hk < 1 || Hq < 1 || Hq % Hk != 0 || Nq >= (1LL << 30)) return 0;
-    return (int64_t)split_groups(S, Nq, Hk, Hq / Hk, max_keys) * Hk * kRows * kRecord * 4;
+    const int64_t groups = split_groups(S, Nq, Hk, Hq / Hk, max_keys);
+    return groups == 0 ? 0 : groups * Hk * kRows * kRecord * 4 + 16;  // records, length of a part
 }
 
 extern "C" int reskv_packed_attention(const void* q, const void* k, const void* v, void* out, const int32_t* q_offsets,
@@ -522,6 +541,8 @@ extern "C" int reskv_packed_attention(const void* q, const void* k, const void* 
     A.q_offsets = q_offsets;
     A.k_offsets = k_offsets;
     A.part = (float*)workspace;
+    A.stat = (float2*)(A.part + (long)split * Hk * kRows * kDim);
+    A.length = (int32_t*)(A.stat + (long)split * Hk * kRows);
     A.q_token = strides[0];
     A.q_head = strides[1];
     A.k_token = strides[2];

@@ -38,7 +38,8 @@ extern "C" {
  * [q_offsets[s], q_offsets[s+1]) and the key rows [k_offsets[s], k_offsets[s+1]);
  * with nq and nk of them, query i sees the keys 0 .. i + nk - nq (none: zeros).
  * q fp16 [Nq, Hq, 128], k, v [Nk, Hk, 128]: strides[0..5] are the token and head strides of q,
- * k and v in elements (channel stride 1, rows 16-byte aligned, token strides below 2^23);
+ * k and v in elements (channel stride 1, rows 16-byte aligned, token strides below 2^23, those of k and v
+ * at least 128);
  * out [Nq, Hq, 128] contiguous.  Query rows of no sequence are left as they are, or set to
  * zero with clear_rest.  max_keys bounds the keys of a sequence (it only steers how the work
  * is split); workspace as reskv_packed_workspace_bytes says (may be NULL when that is 0). */
@@ -65,7 +66,7 @@ int reskv_int4_gather(const void* pages, int64_t num_pages, int page_tokens, int
 
 /* One token of each of B sequences: q fp16 [B, Hq, 128] against the first lengths[b] tokens of
  * sequence b, out fp16 [B, Hq, 128] (zeros for a sequence without tokens), both contiguous.
- * max_length bounds the lengths (longer ones are clamped to it). */
+ * max_length bounds the lengths (longer ones are clamped to it); the workspace is always needed. */
 int64_t reskv_int4_workspace_bytes(int B, int Hq, int Hk, int64_t max_length);
 int reskv_int4_attention(const void* q, const void* pages, int64_t num_pages, int page_tokens, const int32_t* table,
                          int table_width, const int32_t* lengths, int B, int Hq, int Hk, float scaling,

@@ -140,7 +140,9 @@ __device__ __forceinline__ void codes_of(const half2_t* x, const Group& g, uint3
 // One workgroup per (block of 32 tokens that gets rows, head); thread (token, part) has 16 channels
 // of K and of V, so that a wave has the eight tokens that share the dwords of V.
 //
-// Bound: the vector ALU, and memory behind it (512 bytes in and 160 out per row).
+// Bound: memory (512 bytes in and 160 out per token and head), with the vector ALU close behind: 37,200 tokens of 8 heads
+// in 47 us (4.2 TB/s; a large copy reaches 4.8).  With a division per code and V transposed byte by byte through the
+// LDS it was 74 us.  32 single tokens: 6 us, a chain of five trips to memory (offsets, page, rows, old nibbles, out).
 __global__ void __launch_bounds__(kThreads) append_kernel(RowArgs A) {
     __shared__ __align__(16) uint32_t s_k[512], s_v[512];  // codes as stored
     __shared__ uint32_t s_kp[128];                         // K scalings as stored
@@ -263,6 +265,7 @@ __device__ void clear_rows(const RowArgs& A, int spare, int spares, int h) {
     }
 }
 
+// The same workgroups the other way.  Bound: memory, 37,200 tokens of 8 heads in 34 us (5.9 TB/s).
 __global__ void __launch_bounds__(kThreads) gather_kernel(RowArgs A) {
     __shared__ __align__(16) uint32_t s_v[512];
     __shared__ uint32_t s_vp[128];
@@ -426,6 +429,12 @@ __device__ __forceinline__ void load_block(Block& b, const char* p, int lane) {
 // share one set of accumulators (32 registers otherwise, a quarter of them used).  The lowest values are one
 // more product, with P alone.  The product P s is relative to a power of two `e2` not below any scale so far,
 // kept like the softmax's maximum.
+//
+// The matrix cores have rows to spare (16 for 4 heads), which is why a group's place among the rows costs nothing:
+// a block of 32 tokens takes 17 products, about 220 vector instructions and 5 KB.  Bound: memory for large
+// batches (32 sequences of 16384 tokens, 32 / 8 heads: 118 us, 5.7 TB/s, where a kernel that only reads such pieces
+// reaches 6.0), the start of a wave and the merge for small ones (1000 tokens: 4.5 + 4 us), and the chain of a block's steps
+// for 8 query heads (5 sequences of 17 to 65001: 24 us, of which 17 would be memory's).
 template <int HB>
 __device__ __forceinline__ void work_on_column(const AttnArgs& A, uint16_t* s_p, int b, int column, int begin, int end) {
     constexpr int kHeads = 4 * HB;
@@ -670,7 +679,7 @@ __global__ void __launch_bounds__(kWave, kWavesPerSimd) attention_kernel(AttnArg
 
 // Joins the records of a query head: one workgroup per (sequence, query head).  Lanes take the records'
 // maxima and sums, 64 at a time; the waves then take every fourth record's 128 channels, two per lane,
-// with eight loads under way (one after the other a record costs a trip to memory: 51 of them took 28 us).
+// with eight loads under way (one after the other a record costs a trip to memory: 51 of them took 28 us, now 4).
 __global__ void __launch_bounds__(kThreads) merge_kernel(AttnArgs A) {
     __shared__ float2 s_o[kWaves][kWave];
     const long row = blockIdx.x;
@@ -726,6 +735,8 @@ __global__ void __launch_bounds__(kThreads) merge_kernel(AttnArgs A) {
 // page copies
 // ---------------------------------------------------------------------------
 
+// 16 KB per workgroup through the registers.  Bound: memory, 300 pages of 32 layers (1.57 GB read and written) in
+// 304 us (5.2 TB/s), 3 pages in 4 us.
 constexpr int kPairs = 384;  // per launch: the numbers travel with the kernel's arguments
 struct CopyArgs {
     uint4* pages;

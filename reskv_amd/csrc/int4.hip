@@ -872,6 +872,7 @@ extern "C" int reskv_int4_attention(const void* q, const void* pages, int64_t nu
     if (!pool_ok(pages, num_pages, page_tokens, Hk, table, table_width)) return 1;
     RESKV_REQUIRE(B > 0 && Hq > 0 && Hq % Hk == 0, "bad sizes (sequences %d, query heads %d, KV heads %d)", B, Hq, Hk);
     RESKV_REQUIRE(max_length >= 0, "max_length must not be negative");
+    RESKV_REQUIRE(scaling > -1e30f && scaling < 1e30f, "scaling must lie between -1e30 and 1e30");
     RESKV_REQUIRE(aligned16(q) && aligned16(out) && aligned16(workspace), "tensors must be 16-byte aligned");
     const long most = (long)table_width * page_tokens;
     if (max_length > most) max_length = most;

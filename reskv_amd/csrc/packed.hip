@@ -529,7 +529,7 @@ extern "C" int reskv_packed_attention(const void* q, const void* k, const void* 
     for (int i = 0; i < 6; ++i) RESKV_REQUIRE(strides[i] >= 0 && strides[i] % 8 == 0, "rows must be 16-byte aligned");
     RESKV_REQUIRE(strides[2] < (1 << 23) && strides[4] < (1 << 23), "token strides of k and v must be below 2^23");
     RESKV_REQUIRE(strides[2] >= kDim && strides[4] >= kDim, "rows of k and v must not overlap");
-    RESKV_REQUIRE(scaling > 0.0f, "scaling must be positive");
+    RESKV_REQUIRE(scaling > 0.0f && scaling < 1e30f, "scaling must be positive and below 1e30");
     const int split = split_groups(S, Nq, Hk, G, max_keys);
     RESKV_REQUIRE(!split || (workspace && workspace_bytes >= reskv_packed_workspace_bytes(S, Nq, Hq, Hk, max_keys)),
                   "the workspace is too small");

@@ -132,7 +132,7 @@ def int4_attention(q, pages, table, lengths, *, scaling=None, max_length=None, o
 
     Hq is any multiple of the pool's KV heads.  A sequence without tokens gives zeros.  ``max_length`` bounds
     the lengths (default: what the table can hold; a longer length is cut to it) and steers how the work
-    is split over the GPU.  Scores, softmax and sums are fp32; the weights are rounded to fp16 for the
+    is split over the GPU; a captured call keeps it.  Scores, softmax and sums are fp32; the weights are rounded to fp16 for the
     product with V.
     """
     count, tokens, kv_heads = _pool(pages)
@@ -203,8 +203,9 @@ class Int4Cache:
             out = cache.attend(layer, q)       # rotated Q [sequences, Hq, 128]
 
     Which page belongs to whom is kept on the host; ``table``, ``starts`` (of the reserved tokens) and
-    ``lengths`` (with them) are its copies on the GPU, at fixed addresses.  Sequences that were forked
-    share pages; ``reserve`` gives a sequence a copy of its last page before it writes to a shared one.
+    ``lengths`` (with them) are its copies on the GPU, at fixed addresses, so that appends and attention
+    may be captured into a graph and replayed after every ``reserve``, which itself stays outside.  Sequences that
+    were forked share pages; ``reserve`` gives a sequence a copy of its last page before it writes to a shared one.
     """
 
     def __init__(self, layers, kv_heads, sequences, max_length, *, page_tokens=64, pages=None, device="cuda"):
@@ -221,6 +222,7 @@ class Int4Cache:
         self._pages = [[] for _ in range(int(sequences))]
         self._lengths = [0] * int(sequences)
         self._counts = [0] * int(sequences)          # tokens reserved last
+        self._forked = False                         # rows may share pages that the reserved tokens lie in
         self._users = [0] * self.pool.shape[1]       # sequences that have a page
         self._free = list(range(self.pool.shape[1] - 1, -1, -1))  # the lowest number last
 
@@ -269,6 +271,8 @@ class Int4Cache:
         """Makes room for ``counts`` more tokens (one number for every sequence, or one for each); the
         appends that follow fill it.  Raises before any change when a sequence would pass
         ``max_length`` or the pool has too few free pages."""
+        _require(not (self.pool.is_cuda and torch.cuda.is_current_stream_capturing()),
+                 "reserve works on the host and cannot be captured")
         same = isinstance(counts, int)
         counts = [counts] * self.sequences if same else [int(c) for c in counts]
         _require(len(counts) == self.sequences and min(counts) >= 0, "reserve needs a count of tokens for every sequence")
@@ -301,7 +305,7 @@ class Int4Cache:
                 self._pages[s].append(p)
                 changed.add(s)
         self._publish(sorted(changed))
-        self._lengths, self._counts = ends, counts
+        self._lengths, self._counts, self._forked = ends, counts, False
         if same:
             self.starts.copy_(self.lengths)
             self.lengths.add_(counts[0])
@@ -309,13 +313,14 @@ class Int4Cache:
             self._publish_lengths()
 
     def append(self, layer, k, v, offsets=None):
-        """The reserved tokens of one layer (``int4_append``): one row per sequence, or rows packed by ``offsets``."""
+        """The reserved tokens of one layer (``int4_append``): one row per sequence, or rows packed by ``offsets``
+        (on the GPU, so that their counts are not compared with the reserved ones)."""
+        _require(not self._forked, "sequences were forked: reserve tokens before the next append")
         int4_append(self.pool[layer], self.table, self.starts, k, v, offsets)
 
     def attend(self, layer, q, *, scaling=None, out=None):
         """Attention of one token per sequence over all its tokens (``int4_attention``)."""
-        return int4_attention(q, self.pool[layer], self.table, self.lengths, scaling=scaling,
-                              max_length=max(self._lengths), out=out)
+        return int4_attention(q, self.pool[layer], self.table, self.lengths, scaling=scaling, out=out)
 
     def gather(self, layer):
         """(k, v, offsets): the stored values of all tokens, packed (``int4_gather``), as
@@ -334,6 +339,7 @@ class Int4Cache:
         for row in pages:
             for p in row:
                 self._users[p] += 1
+        self._forked |= len(set(index)) < len(index)
         old, self._pages = self._pages, pages
         self._drop(p for row in old for p in row)
         self._lengths = [self._lengths[s] for s in index]

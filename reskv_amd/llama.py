@@ -415,7 +415,9 @@ class GreedyDecoder:
         if self.mode == "reskv":
             self.caches[layer].update(rot_k, v, {"raw_keys": raw_k})
         elif self.mode == "int4":
-            if layer == 0:
+            if layer == 0:  # a new prompt takes the place of what was there
+                for b in range(self.batch):
+                    self.pages.release(b)
                 self.pages.reserve(t)
             ends = torch.arange(0, (self.batch + 1) * t, t, dtype=torch.int32, device=v.device)
             rows = [y.transpose(1, 2).reshape(-1, *y.shape[1::2]) for y in (rot_k, v)]

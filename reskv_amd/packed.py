@@ -98,7 +98,7 @@ def packed_attention(q, k, v, q_offsets, k_offsets=None, *, scaling=None, max_ke
 
     ``scaling`` (positive) defaults to 128 ** -0.5; ``max_keys`` bounds the keys of a sequence
     (default: all of k) and only steers how the work is split.  Returns fp16 [Nq, Hq, 128],
-    ``out`` when given (contiguous); rows of no sequence are zero, or left as they are in ``out``.
+    ``out`` when given (contiguous, apart from k and v); rows of no sequence are zero, or left as they are in ``out``.
 
     Scores and sums are fp32; the softmax weights are rounded to fp16 for the product with V.  Offsets
     are not read on the host: values outside the tensors are clamped into them.

@@ -83,6 +83,36 @@ def test_cache_through_prompt_forks_beams_and_compaction(device):
         assert np.array_equal(got.cpu().numpy(), ref.stored(want)[0].astype(np.float32).astype(np.float16))
 
 
+def test_captured_steps_over_the_cache(device):
+    """One captured append and attention, replayed while the cache grows (across pages, after a
+    fork), equals the eager calls on a cache of its own."""
+    g = torch.Generator().manual_seed(3)
+    own, other = (Int4Cache(1, 2, 3, 300, page_tokens=32) for _ in range(2))
+    first, at = [rows(g, 46, 2) for _ in range(2)], torch.tensor([0, 5, 14, 46], dtype=torch.int32, device="cuda")
+    for c in (own, other):
+        c.reserve([5, 9, 32])
+        c.append(0, *first, at)
+    q, k, v = rows(g, 3, 8), rows(g, 3, 2), rows(g, 3, 2)
+    own.attend(0, q)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        own.append(0, k, v)
+        out = own.attend(0, q)
+        with pytest.raises(RuntimeError, match="cannot be captured"):
+            own.reserve(1)
+    for step in range(150):
+        for x in (q, k, v):
+            x.copy_(rows(g, *x.shape[:2]))
+        for c in (own, other):
+            if step == 70:
+                c.fork(2, 0)
+            c.reserve(1)
+        graph.replay()
+        other.append(0, k, v)
+        assert torch.equal(out, other.attend(0, q)), step
+    assert own.get_seq_length(0) == 32 + 150 and own.get_seq_length(1) == 9 + 150
+
+
 def test_a_prompt_in_chunks_attends_what_it_stored(device):
     """Chunked prompt: gather the cached tokens, put the chunk's own keys behind them, attend packed."""
     g = torch.Generator().manual_seed(2)
@@ -149,6 +179,8 @@ def test_greedy_decoder_over_the_4_bit_cache(device):
     tokens = torch.stack([dec.step().clone() for _ in range(8)])
     assert checked == [0, 1] * 8 and dec.pages.get_seq_length() == 68
     assert 0 <= int(tokens.min()) and int(tokens.max()) < TINY.vocab and torch.isfinite(dec.x.float()).all()
+    model.prefill(ids, dec.absorb)  # a new prompt takes the place of the old one
+    assert dec.pages.get_seq_length() == 60
     ended = GreedyDecoder(model, 2, 4, 0, "int4")
     with pytest.raises(RuntimeError, match="capacity exhausted"):
         ended.step()

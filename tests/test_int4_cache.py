@@ -113,6 +113,20 @@ def test_refusals_change_nothing(copies):
     consistent(c)
 
 
+def test_no_append_between_a_fork_and_the_next_reservation(copies):
+    """Rows that share the page of reserved tokens would write to one place."""
+    c, kv = cache(2, 64), torch.zeros(2, 1, 128, dtype=torch.float16)
+    c.reserve(1)
+    for forked in (lambda: c.fork(0, 1), lambda: c.reorder([1, 1])):
+        forked()
+        with pytest.raises(RuntimeError, match="reserve tokens before"):
+            c.append(0, kv, kv)
+        c.reserve([0, 1])
+        c.reorder([1, 0])
+        with pytest.raises(RuntimeError, match="CUDA tensor"):
+            c.append(0, kv, kv)
+
+
 @pytest.mark.parametrize("kw", [dict(layers=0), dict(sequences=0), dict(max_length=0), dict(page_tokens=48),
                                 dict(kv_heads=0), dict(pages=0)])
 def test_constructor_refusals(kw):

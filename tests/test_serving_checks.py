@@ -169,6 +169,8 @@ def test_entry_points_refuse_bad_arguments_without_a_gpu():
         return lib.reskv_packed_attention(q, p, p, out, p, p, S, Nq, Nk, Hq, Hk, strides, scaling, most, 0, work, nbytes, None)
 
     assert "null" in _err(packed(q=None))
+    for scaling in (0.0, 1e300, float("nan")):  # 1e300 is infinite in 32 bits
+        assert "scaling must be positive" in _err(packed(scaling=scaling))
     assert "bad sizes" in _err(packed(S=0)) and "bad sizes" in _err(packed(Hq=5)) and "bad sizes" in _err(packed(Nk=0))
     assert "aligned" in _err(packed(out=odd))
     assert "aligned" in _err(packed(strides=(ctypes.c_int64 * 6)(512, 128, 256, 100, 256, 128)))

@@ -334,6 +334,7 @@ constexpr int kWaves = 4;
 // Waves at work on each SIMD.  Three of them fit with 4 query heads, and are no faster: 32 sequences of
 // 16384 tokens 130 us against 124, of 2000 to 8192 tokens 38 against 37.5.
 constexpr int kWavesPerSimd = 2;
+constexpr int kMostWaves = 1024 * kWavesPerSimd;  // 256 CUs of 4 SIMDs
 constexpr float kLog2e = 1.4426950408889634f;
 // Weights are exp2(x - m) * 2^14, m the largest score so far: the largest stays below the largest fp16 number, and a
 // weight is lost to fp16 only when it is below 2^-39 of it.  The largest weight itself is exact, which matters
@@ -677,14 +678,22 @@ __global__ void __launch_bounds__(kWave, kWavesPerSimd) attention_kernel(AttnArg
     }
 }
 
-// Joins the records of a query head: one workgroup per (sequence, query head).  Lanes take the records'
-// maxima and sums, 64 at a time; the waves then take every fourth record's 128 channels, two per lane,
-// with eight loads under way (one after the other a record costs a trip to memory: 51 of them took 28 us, now 4).
+// Joins the records of a query head: PIECES workgroups per (sequence, query head), each with as many
+// of its channels.  The threads take a record's maximum and sum each, and the weights from them into the LDS; the
+// waves then take records' channels, two per lane, with eight loads under way, the first of them before the weights
+// are known: a merge is a chain of trips to memory, of which each costs more than what it brings.  51 records
+// one after the other took 28 us; 5 sequences of 17 to 65001 tokens and 32 heads, 8.4 us with one workgroup
+// each and the maxima read twice, and 4.8 like this.
+template <int PIECES>
 __global__ void __launch_bounds__(kThreads) merge_kernel(AttnArgs A) {
-    __shared__ float2 s_o[kWaves][kWave];
-    const long row = blockIdx.x;
-    const int b = (int)(row / A.Hq), hq = (int)(row - (long)b * A.Hq), lane = threadIdx.x & 63;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    constexpr int kLanes = kWave / PIECES;     // of a record's piece: PIECES records per load
+    constexpr int kStep = kWaves * PIECES;     // records that the waves take with one load
+    __shared__ float2 s_record[kMostWaves];    // maximum (then weight) and sum; a wave leaves one record in a column at most
+    __shared__ float2 s_o[kWaves][kLanes];
+    __shared__ float s_top[kWaves], s_total[kWaves];
+    const long row = blockIdx.x / PIECES;
+    const int b = (int)(row / A.Hq), hq = (int)(row - (long)b * A.Hq), tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int heads = A.G <= 4 ? 4 : 8;  // of a set
     const int hk = hq / A.G, set = (hq - hk * A.G) / heads, column = hk * A.sets + set;
     const Sums sums = sum_blocks(A, b);
@@ -692,43 +701,69 @@ __global__ void __launch_bounds__(kThreads) merge_kernel(AttnArgs A) {
     const int start = sums.before * A.columns + column * blocks, first = start / run;
     const int records = blocks == 0 ? 0 : (start + blocks - 1) / run - first + 1;
     const long at = ((long)first + (long)b * A.columns + column) * heads + (hq - hk * A.G - set * heads);
+    const int of = lane / kLanes, channel = (int)blockIdx.x % PIECES * kLanes + lane % kLanes;  // record of a load, channel pair
     const float2* const stat = A.stat + at;  // a record's every `heads`
-    const float2* const part = reinterpret_cast<const float2*>(A.part) + at * kWave + lane;
-    float top = -__FLT_MAX__;
-    for (int s = lane; s < records; s += kWave) top = fmaxf(top, stat[(long)s * heads].x);
+    const float2* const part = reinterpret_cast<const float2*>(A.part) + at * kWave + channel;
+    uint32_t* const out = reinterpret_cast<uint32_t*>(A.out + row * kDim) + channel;
+    if (records == 0) {
+        if (tid < kLanes) *out = 0;
+        return;
+    }
+    float2 r[8], o = make_float2(0.0f, 0.0f);
+    auto load = [&](int i0) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) r[i] = part[(long)min(i0 + kStep * i + of, records - 1) * heads * kWave];
+    };
+    load(wave * PIECES);
+    float top = -__FLT_MAX__, total = 0.0f;
+    for (int s = tid; s < records; s += kThreads) {
+        const float2 ml = stat[(long)s * heads];
+        s_record[s] = ml;
+        top = fmaxf(top, ml.x);
+    }
     top = wave_max(top);
-    float2 o = make_float2(0.0f, 0.0f);
-    float total = 0.0f;
-    for (int s0 = 0; s0 < records; s0 += kWave) {
-        const float2 ml = s0 + lane < records ? stat[(long)(s0 + lane) * heads] : make_float2(0.0f, 0.0f);
+    if (lane == 0) s_top[wave] = top;
+    __syncthreads();
+    top = fmaxf(fmaxf(s_top[0], s_top[1]), fmaxf(s_top[2], s_top[3]));
+    for (int s = tid; s < records; s += kThreads) {
+        const float2 ml = s_record[s];
         const float weight = ml.y == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(ml.x - top);  // no tokens (a NaN goes on)
-        total += wave_sum(weight * ml.y);
-        const int n = min(kWave, records - s0);
-        for (int i0 = wave; i0 < n; i0 += 8 * kWaves) {
-            float2 r[8];
+        s_record[s].x = weight;
+        total += weight * ml.y;
+    }
+    total = wave_sum(total);
+    if (lane == 0) s_total[wave] = total;
+    __syncthreads();
+    total = (s_total[0] + s_total[1]) + (s_total[2] + s_total[3]);
+    for (int i0 = wave * PIECES;;) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) r[i] = part[(long)(s0 + min(i0 + kWaves * i, n - 1)) * heads * kWave];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int at = i0 + kWaves * i;
-                const float a = readlane(weight, at & 63);
-                if (at < n) {
-                    o.x += a * r[i].x;
-                    o.y += a * r[i].y;
-                }
+        for (int i = 0; i < 8; ++i) {
+            const int n = i0 + kStep * i + of;
+            if (n < records) {
+                const float weight = s_record[n].x;
+                o.x += weight * r[i].x;
+                o.y += weight * r[i].y;
             }
         }
+        i0 += 8 * kStep;
+        if (i0 >= records) break;
+        load(i0);
     }
-    s_o[wave][lane] = o;
+#pragma unroll
+    for (int i = kLanes; i < kWave; i *= 2) {
+        o.x += __shfl_xor(o.x, i);
+        o.y += __shfl_xor(o.y, i);
+    }
+    if (lane < kLanes) s_o[wave][lane] = o;
     __syncthreads();
-    if (wave != 0) return;
+    if (tid >= kLanes) return;
 #pragma unroll
     for (int i = 1; i < kWaves; ++i) {
         o.x += s_o[i][lane].x;
         o.y += s_o[i][lane].y;
     }
     const float inv = total == 0.0f ? 0.0f : 1.0f / total;
-    reinterpret_cast<uint32_t*>(A.out + row * kDim)[lane] = pack_halves(o.x * inv, o.y * inv);
+    *out = pack_halves(o.x * inv, o.y * inv);
 }
 
 // ---------------------------------------------------------------------------
@@ -798,11 +833,10 @@ long row_items(const int32_t* offsets, int S, long N) { return offsets ? N / kBl
 int head_sets(int G) { return G <= 4 ? 1 : (G + 7) / 8; }
 int set_heads(int G) { return G <= 4 ? 4 : 8; }
 
-// Waves: as many as the chip holds at once (256 CUs of 4 SIMDs), or one per block when there are fewer.
+// Waves: as many as the chip holds at once, or one per block when there are fewer.
 long attention_waves(int B, int Hk, int G, long max_length) {
     const long blocks = (max_length + kBlock - 1) / kBlock * B * Hk * head_sets(G);
-    const long most = 1024L * kWavesPerSimd;
-    return blocks < 1 ? 1 : blocks < most ? blocks : most;
+    return blocks < 1 ? 1 : blocks < kMostWaves ? blocks : kMostWaves;
 }
 long attention_records(int B, int Hk, int G, long max_length) {
     return attention_waves(B, Hk, G, max_length) + (long)B * Hk * head_sets(G);
@@ -901,7 +935,12 @@ extern "C" int reskv_int4_attention(const void* q, const void* pages, int64_t nu
     hipLaunchKernelGGL(G <= 4 ? attention_kernel<1> : attention_kernel<2>, dim3((unsigned)A.waves), dim3(kWave), 0,
                        (hipStream_t)stream, A);
     if (reskv_host::check_launch("int4 attention_kernel")) return 1;
-    hipLaunchKernelGGL(merge_kernel, dim3((unsigned)(B * Hq)), dim3(kThreads), 0, (hipStream_t)stream, A);
+    // Query heads in pieces while there are fewer than CUs: their records come from the whole chip.  One sequence of 30000
+    // tokens and 32 heads 16 us with four pieces and 20 with one, 4 of 1000 to 9000 13.6 and 14.3, 8 of them (256 heads) 18.0
+    // and 17.8, 24 of 4000 35 and 28.
+    const int pieces = (long)B * Hq < 256 ? 4 : 1;
+    hipLaunchKernelGGL(pieces == 4 ? merge_kernel<4> : merge_kernel<1>, dim3((unsigned)(B * Hq * pieces)), dim3(kThreads), 0,
+                       (hipStream_t)stream, A);
     return reskv_host::check_launch("int4 merge_kernel");
 }
 

@@ -445,6 +445,28 @@ __device__ __forceinline__ void work_on_column(const AttnArgs& A, uint16_t* s_p,
     const int heads = min(kHeads, A.G - h0), length = A.tokens(b);
     const long row0 = (long)b * A.Hq + hk * A.G + h0;
 
+    // The wave's blocks, one after the other, each fetched while the one before is worked on.  Page
+    // numbers come 64 at a time, one per lane.
+    int entry0 = begin / A.pool.blocks, entry = 0, inside = begin - entry0 * A.pool.blocks, numbers = 0;
+    auto fetch_numbers = [&]() { numbers = A.pool.table[(long)b * A.pool.width + min(entry0 + lane, A.pool.width - 1)]; };
+    // next block's data, and whether its page is there
+    auto fetch = [&](Block& x) {
+        const char* p = A.pool.in_page(__builtin_amdgcn_readlane(numbers, entry), inside, hk);
+        load_block(x, p ? p : A.pool.pages, lane);
+        if (++inside == A.pool.blocks) {
+            inside = 0;
+            if (++entry == kWave) {
+                entry0 += kWave;
+                entry = 0;
+                fetch_numbers();
+            }
+        }
+        return p != nullptr;
+    };
+    Block x0, x1;
+    fetch_numbers();
+    bool there0 = fetch(x0);  // before Q, so that the first block does not wait for it
+
     // Q: lane (n = 4 g + h, quarter): channels 32 g + 8 quarter + [0, 8) of head h, brought to a common power
     // of two so that the sixteenth of an element keeps its bits
     half8_t qa[HB][4];
@@ -499,24 +521,6 @@ __device__ __forceinline__ void work_on_column(const AttnArgs& A, uint16_t* s_p,
     float e2 = 0x1p-14f;  // not below any scale so far
     half2_t f1 = {(_Float16)0x1p14f, (_Float16)0x1p14f}, f16 = {(_Float16)0x1p10f, (_Float16)0x1p10f};  // its reciprocal, and a sixteenth
 
-    // The wave's blocks, one after the other, each fetched while the one before is worked on.  Page
-    // numbers come 64 at a time, one per lane.
-    int entry0 = begin / A.pool.blocks, entry = 0, inside = begin - entry0 * A.pool.blocks, numbers = 0;
-    auto fetch_numbers = [&]() { numbers = A.pool.table[(long)b * A.pool.width + min(entry0 + lane, A.pool.width - 1)]; };
-    // next block's data, and whether its page is there
-    auto fetch = [&](Block& x) {
-        const char* p = A.pool.in_page(__builtin_amdgcn_readlane(numbers, entry), inside, hk);
-        load_block(x, p ? p : A.pool.pages, lane);
-        if (++inside == A.pool.blocks) {
-            inside = 0;
-            if (++entry == kWave) {
-                entry0 += kWave;
-                entry = 0;
-                fetch_numbers();
-            }
-        }
-        return p != nullptr;
-    };
     auto work = [&](Block& x, int blk, bool there) {
         const int valid = there ? min(kBlock, length - blk * kBlock) : 0;
         if (valid < kBlock) {  // what lies behind the last token may be anything
@@ -618,9 +622,7 @@ __device__ __forceinline__ void work_on_column(const AttnArgs& A, uint16_t* s_p,
         }
         wave_sync();
     };
-    Block x0, x1;
-    fetch_numbers();
-    bool there0 = fetch(x0), there1 = false;
+    bool there1 = false;
     for (int blk = begin; blk < end; blk += 2) {
         if (blk + 1 < end) there1 = fetch(x1);
         work(x0, blk, there0);

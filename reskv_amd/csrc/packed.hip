@@ -545,7 +545,7 @@ extern "C" int reskv_packed_attention(const void* q, const void* k, const void* 
                   "bad sizes (sequences %d, Nq %ld, Nk %ld, Hq %d, Hk %d)", S, (long)Nq, (long)Nk, Hq, Hk);
     const int G = Hq / Hk;
     RESKV_REQUIRE(Nq * G < (1LL << 30) && Nk < (1LL << 30), "too many rows");
-    RESKV_REQUIRE(aligned16(q) && aligned16(k) && aligned16(v) && aligned16(out), "tensors must be 16-byte aligned");
+    RESKV_REQUIRE(aligned16(q) && aligned16(k) && aligned16(v) && aligned16(out) && aligned16(workspace), "tensors must be 16-byte aligned");
     for (int i = 0; i < 6; ++i) RESKV_REQUIRE(strides[i] >= 0 && strides[i] % 8 == 0, "rows must be 16-byte aligned");
     RESKV_REQUIRE(strides[2] < (1 << 23) && strides[4] < (1 << 23), "token strides of k and v must be below 2^23");
     RESKV_REQUIRE(strides[2] >= kDim && strides[4] >= kDim, "rows of k and v must not overlap");

@@ -172,7 +172,7 @@ def test_entry_points_refuse_bad_arguments_without_a_gpu():
     for scaling in (0.0, 1e300, float("nan")):  # 1e300 is infinite in 32 bits
         assert "scaling must be positive" in _err(packed(scaling=scaling))
     assert "bad sizes" in _err(packed(S=0)) and "bad sizes" in _err(packed(Hq=5)) and "bad sizes" in _err(packed(Nk=0))
-    assert "aligned" in _err(packed(out=odd))
+    assert "aligned" in _err(packed(out=odd)) and "aligned" in _err(packed(work=odd))
     assert "aligned" in _err(packed(strides=(ctypes.c_int64 * 6)(512, 128, 256, 100, 256, 128)))
     assert "2^23" in _err(packed(strides=(ctypes.c_int64 * 6)(512, 128, 1 << 23, 128, 256, 128)))
     assert "scaling" in _err(packed(scaling=0.0)) and "scaling" in _err(packed(scaling=float("nan")))

@@ -336,11 +336,20 @@ constexpr int kWaves = 4;
 constexpr int kWavesPerSimd = 2;
 constexpr int kMostWaves = 1024 * kWavesPerSimd;  // 256 CUs of 4 SIMDs
 constexpr float kLog2e = 1.4426950408889634f;
-// Weights are exp2(x - m) * 2^14, m the largest score so far: the largest stays below the largest fp16 number, and a
-// weight is lost to fp16 only when it is below 2^-39 of it.  The largest weight itself is exact, which matters
-// where one token outweighs the others: letting scores pass m by up to 2^4 saved up to 3% of the time (32.9 ->
-// 31.9 us), and took the error of such outputs from 2.3e-4 to 3.0e-4 (2.1e-4 is their own rounding's).
-constexpr float kWeightBits = 14.0f;
+// What is rounded to fp16 is a weight times a V scale, once, as an operand of the matrix cores, times the power of two
+// that brings the reference of its query head and channel group to [kTop, 2 kTop).  The reference is a product so far,
+// relative to the largest weight, and follows when one is more than kMost.  It follows the products, not the scales, so
+// that a token of large values and no weight takes no bits from the others, and each head and group has its own: a
+// product keeps fp16's eleven bits down to 2^-20 of the reference, and is lost at 2^-31.  (Scales relative to one power
+// of two above all of a run's scales took 28.8 us instead of 30.7 for 8 query heads, and lost what was 2^-14 below it.)
+// A power of two, as the largest weight is 1 and its products then exact, which matters where one token outweighs the
+// others: with kTop / reference itself such outputs were off by 3.3e-4 instead of 2.25e-4 (2.1e-4 is their own rounding's).
+constexpr float kTop = 0x1p10f, kMost = 0x1p15f;
+constexpr float kLeastReference = 0x1p-24f;  // the smallest scale: a largest weight (1) without any product needs no more
+__device__ __forceinline__ float up_of(float reference) {  // kTop over the power of two not above a reference of kLeastReference or more
+    return i2f(((127 + 10 + 127) << 23) - (f2i(reference) & 0x7F800000));
+}
+__device__ __forceinline__ float quotient(float a, float b) { return i2f((127 << 23) + f2i(a) - f2i(b)); }  // of powers of two
 
 // Work: a column is (sequence, KV head, set of query heads), `blocks` long; the columns lie one behind the
 // other and every wave takes an equal run of blocks, across columns where it has to, so that lengths may
@@ -387,6 +396,13 @@ __device__ __forceinline__ float swap_sum16(float a, float b) {
     const auto r = __builtin_amdgcn_permlane16_swap((uint32_t)f2i(a), (uint32_t)f2i(b), false, false);
     return i2f((int)r[0]) + i2f((int)r[1]);
 }
+// Maximum over the four quarters of the wave.
+__device__ __forceinline__ float swap_max(float a) {
+    const auto r = __builtin_amdgcn_permlane16_swap((uint32_t)f2i(a), (uint32_t)f2i(a), false, false);
+    a = fmaxf(i2f((int)r[0]), i2f((int)r[1]));
+    const auto s = __builtin_amdgcn_permlane32_swap((uint32_t)f2i(a), (uint32_t)f2i(a), false, false);
+    return fmaxf(i2f((int)s[0]), i2f((int)s[1]));
+}
 
 // The operand register pair (elements 0 .. 7) of a dword of codes: elements 0, 1, 4, 5 times
 // 2^-24 and 2, 3, 6, 7 times 2^-20.
@@ -395,6 +411,8 @@ __device__ __forceinline__ half8_t operand(uint32_t d) {
     const uint4 w = make_uint4(d & 0x000F000Fu, d & 0x00F000F0u, e & 0x000F000Fu, e & 0x00F000F0u);
     return __builtin_bit_cast(half8_t, w);
 }
+
+constexpr int kPitch = kBlock + 16;  // fp32 weights of a head in the LDS: the four quarters' writes fall on different banks
 
 // One block's codes and scalings as a lane takes them.
 struct Block {
@@ -427,19 +445,17 @@ __device__ __forceinline__ void load_block(Block& b, const char* p, int lane) {
 // three lane swaps add the groups and leave head h's score of token n in lane (h, n).
 // Values: D[row 4 g + h][16 channels] += (P s_g) V over 32 tokens for each group's two sets of channels, the
 // weights times the scale of group g in rows 4 g + h and zeros elsewhere, so that the four groups
-// share one set of accumulators (32 registers otherwise, a quarter of them used).  The lowest values are one
-// more product, with P alone.  The product P s is relative to a power of two `e2` not below any scale so far,
-// kept like the softmax's maximum.
+// share one set of accumulators (32 registers otherwise, a quarter of them used).  A lane has the weights of head h in
+// fp32 from the LDS, multiplies them with group g's scales, and adds up the lowest values' share in fp32 itself.
 //
 // The matrix cores have rows to spare (16 for 4 heads), which is why a group's place among the rows costs nothing:
-// a block of 32 tokens takes 17 products, about 220 vector instructions and 5 KB.  Bound: memory for large
+// a block of 32 tokens takes 16 products, about 180 vector instructions and 5 KB.  Bound: memory for large
 // batches (32 sequences of 16384 tokens, 32 / 8 heads: 118 us, 5.7 TB/s, where a kernel that only reads such pieces
 // reaches 6.0), the start of a wave and the merge for small ones (1000 tokens: 4.5 + 4 us), and the chain of a block's steps
 // for 8 query heads (5 sequences of 17 to 65001: 24 us, of which 17 would be memory's).
 template <int HB>
-__device__ __forceinline__ void work_on_column(const AttnArgs& A, uint16_t* s_p, int b, int column, int begin, int end) {
+__device__ __forceinline__ void work_on_column(const AttnArgs& A, float* s_p, int b, int column, int begin, int end) {
     constexpr int kHeads = 4 * HB;
-    constexpr int kPitch = kBlock + 8;
     const int lane = threadIdx.x, n = lane & 15, quarter = lane >> 4;
     const int hk = column / A.sets, h0 = (column - hk * A.sets) * kHeads;  // KV head, first query head of the set within it
     const int heads = min(kHeads, A.G - h0), length = A.tokens(b);
@@ -508,18 +524,19 @@ __device__ __forceinline__ void work_on_column(const AttnArgs& A, uint16_t* s_p,
         }
     }
 
-    float4_t acc[HB][2], accl[HB];  // acc: channels 32 quarter + 16 i + n of the four heads
-    float m[HB], l[HB];  // head 4 hb + quarter; l: this lane's tokens
+    float4_t acc[HB][2];  // channels 32 quarter + 16 i + n of the four heads, times their rows' `up`
+    float m[HB], l[HB];   // head 4 hb + quarter; l: this lane's tokens
+    // of row n = 4 g + h: the reference of the products; its power of two; the lowest values' share of this lane's tokens
+    float reference[HB], up[HB], lows[HB];
 #pragma unroll
     for (int hb = 0; hb < HB; ++hb) {
         m[hb] = -__FLT_MAX__;
-        l[hb] = 0.0f;
-        accl[hb] = {0.0f, 0.0f, 0.0f, 0.0f};
+        l[hb] = lows[hb] = 0.0f;
+        reference[hb] = kLeastReference;
+        up[hb] = up_of(kLeastReference);
 #pragma unroll
         for (int i = 0; i < 2; ++i) acc[hb][i] = {0.0f, 0.0f, 0.0f, 0.0f};
     }
-    float e2 = 0x1p-14f;  // not below any scale so far
-    half2_t f1 = {(_Float16)0x1p14f, (_Float16)0x1p14f}, f16 = {(_Float16)0x1p10f, (_Float16)0x1p10f};  // its reciprocal, and a sixteenth
 
     auto work = [&](Block& x, int blk, bool there) {
         const int valid = there ? min(kBlock, length - blk * kBlock) : 0;
@@ -555,36 +572,22 @@ __device__ __forceinline__ void work_on_column(const AttnArgs& A, uint16_t* s_p,
                 score[hb][tile] = 16 * tile + n < valid ? s : -INFINITY;
             }
         }
-        half2_t tops = {(_Float16)0.0f, (_Float16)0.0f};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) tops = __builtin_elementwise_max(tops, __builtin_bit_cast(half2_t, x.vs[i]));
-        const float top_scale = fmaxf((float)tops[0], (float)tops[1]);
-        bool grow = top_scale > e2;
+        bool grow = false;
 #pragma unroll
         for (int hb = 0; hb < HB; ++hb) grow |= fmaxf(score[hb][0], score[hb][1]) > m[hb];
-        if (ballot(grow) != 0) {
-            const float ts = wave_max(top_scale);
-            float shrink = 1.0f;
-            if (ts > e2) {
-                const float up = ldexpf(1.0f, ilogbf(ts) + 1), down = ldexpf(1.0f, -1 - ilogbf(ts));
-                shrink = e2 * down;
-                e2 = up;
-                f1[0] = f1[1] = (_Float16)down;
-                f16[0] = f16[1] = (_Float16)(0.0625f * down);
-            }
+        float kept[HB];  // of row n's sums, where m moves
+#pragma unroll
+        for (int hb = 0; hb < HB; ++hb) kept[hb] = 1.0f;
+        const bool moved = ballot(grow) != 0;
+        if (moved) {
 #pragma unroll
             for (int hb = 0; hb < HB; ++hb) {
                 const float mn = fmaxf(m[hb], row_max16(fmaxf(score[hb][0], score[hb][1])));
                 const float alpha = __builtin_amdgcn_exp2f(m[hb] - mn);
                 m[hb] = mn;
                 l[hb] *= alpha;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float a = readlane(alpha, 16 * i);
-                    accl[hb][i] *= a;
-#pragma unroll
-                    for (int j = 0; j < 2; ++j) acc[hb][j][i] *= a * shrink;
-                }
+                kept[hb] = __shfl(alpha, 16 * (n & 3));
+                lows[hb] *= kept[hb];
             }
         }
         // weights to LDS as [head][token]
@@ -592,20 +595,56 @@ __device__ __forceinline__ void work_on_column(const AttnArgs& A, uint16_t* s_p,
         for (int hb = 0; hb < HB; ++hb)
 #pragma unroll
             for (int tile = 0; tile < 2; ++tile) {
-                const float p = __builtin_amdgcn_exp2f(score[hb][tile] - m[hb] + kWeightBits);
+                const float p = __builtin_amdgcn_exp2f(score[hb][tile] - m[hb]);
                 l[hb] += p;
-                s_p[(4 * hb + quarter) * kPitch + 16 * tile + n] = f2h(p);
+                s_p[(4 * hb + quarter) * kPitch + 16 * tile + n] = p;
             }
         wave_sync();
-        const half8_t factor = {f1[0], f1[1], f16[0], f16[1], f1[0], f1[1], f16[0], f16[1]};
-        const half8_t vscale = __builtin_bit_cast(half8_t, make_uint4(x.vs[0], x.vs[1], x.vs[2], x.vs[3])) * factor;
-        const half8_t vlow = __builtin_bit_cast(half8_t, make_uint4(x.vl[0], x.vl[1], x.vl[2], x.vl[3]));
-        uint4 ps[HB];
+        half2_t vs[4], vl[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            vs[i] = __builtin_bit_cast(half2_t, x.vs[i]);
+            vl[i] = __builtin_bit_cast(half2_t, x.vl[i]);
+        }
+        float product[HB][8], top[HB];
+        bool raise = moved;
 #pragma unroll
         for (int hb = 0; hb < HB; ++hb) {
-            const half8_t pw = *reinterpret_cast<const half8_t*>(&s_p[(4 * hb + (n & 3)) * kPitch + 8 * quarter]);
-            accl[hb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(pw, vlow, accl[hb], 0, 0, 0);
-            ps[hb] = __builtin_bit_cast(uint4, pw * vscale);
+            const float4_t* const row = reinterpret_cast<const float4_t*>(&s_p[(4 * hb + (n & 3)) * kPitch + 8 * quarter]);
+            const float4_t w[2] = {row[0], row[1]};
+            float low[2] = {0.0f, 0.0f};
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                product[hb][e] = __builtin_fmaf(w[e >> 2][e & 3], (float)vs[e >> 1][e & 1], 0.0f);
+                low[e >> 2] = __builtin_fmaf(w[e >> 2][e & 3], (float)vl[e >> 1][e & 1], low[e >> 2]);
+            }
+            lows[hb] += low[0] + low[1];
+            top[hb] = product[hb][0];
+#pragma unroll
+            for (int e = 1; e < 8; ++e) top[hb] = fmaxf(top[hb], product[hb][e]);
+            raise |= top[hb] * up[hb] > kMost;
+        }
+        if (ballot(raise) != 0) {
+#pragma unroll
+            for (int hb = 0; hb < HB; ++hb) {
+                reference[hb] = fmaxf(fmaxf(reference[hb] * kept[hb], swap_max(top[hb])), kLeastReference);
+                const float next = up_of(reference[hb]), shrink = kept[hb] * quotient(next, up[hb]);
+                up[hb] = next;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float a = __shfl(shrink, 4 * quarter + i);
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) acc[hb][j][i] *= a;
+                }
+            }
+        }
+        half2_t ps[HB][4];
+#pragma unroll
+        for (int hb = 0; hb < HB; ++hb) {
+            const float sixteenth = up[hb] * 0.0625f;  // elements 2, 3, 6, 7 meet codes times 2^-20
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                ps[hb][e >> 1][e & 1] = (_Float16)__builtin_fmaf(product[hb][e], e & 2 ? sixteenth : up[hb], 0.0f);  // one instruction
         }
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
@@ -614,8 +653,8 @@ __device__ __forceinline__ void work_on_column(const AttnArgs& A, uint16_t* s_p,
             const uint32_t rows = (n >> 2) == g ? ~0u : 0u;
 #pragma unroll
             for (int hb = 0; hb < HB; ++hb) {
-                const half8_t pg = __builtin_bit_cast(half8_t, make_uint4(ps[hb].x & rows, ps[hb].y & rows, ps[hb].z & rows,
-                                                                          ps[hb].w & rows));
+                const uint4 p = __builtin_bit_cast(uint4, ps[hb]);
+                const half8_t pg = __builtin_bit_cast(half8_t, make_uint4(p.x & rows, p.y & rows, p.z & rows, p.w & rows));
                 acc[hb][0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(pg, v0, acc[hb][0], 0, 0, 0);
                 acc[hb][1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(pg, v1, acc[hb][1], 0, 0, 0);
             }
@@ -632,19 +671,18 @@ __device__ __forceinline__ void work_on_column(const AttnArgs& A, uint16_t* s_p,
     }
 
     // lane (quarter g, n): channels 32 g + n and 32 g + 16 + n of the four heads
-    const float back = e2 * 0x1p24f;
     const long record = (long)blockIdx.x + (long)b * A.columns + column;
     float* const part = A.part + record * kHeads * kDim;
 #pragma unroll
     for (int hb = 0; hb < HB; ++hb) {
-        const float total = row_sum16(l[hb]);
+        const float total = row_sum16(l[hb]), sum16 = swap_sum16(lows[hb], lows[hb]), low_sum = swap_sum32(sum16, sum16);
         if (n == 0) A.stat[record * kHeads + 4 * hb + quarter] = make_float2(m[hb], total);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const float lows = __shfl(accl[hb][i], 16 * quarter + 4 * quarter);  // row 4 g + i, column of group g
+            const float low = __shfl(low_sum, 4 * quarter + i), back = __shfl(quotient(0x1p24f, up[hb]), 4 * quarter + i);
 #pragma unroll
             for (int j = 0; j < 2; ++j)
-                part[(4 * hb + i) * kDim + 32 * quarter + 16 * j + n] = __builtin_fmaf(acc[hb][j][i], back, lows);
+                part[(4 * hb + i) * kDim + 32 * quarter + 16 * j + n] = __builtin_fmaf(acc[hb][j][i], back, low);
         }
     }
     wave_sync();
@@ -653,8 +691,7 @@ __device__ __forceinline__ void work_on_column(const AttnArgs& A, uint16_t* s_p,
 template <int HB>
 __global__ void __launch_bounds__(kWave, kWavesPerSimd) attention_kernel(AttnArgs A) {
     constexpr int kHeads = 4 * HB;
-    constexpr int kPitch = kBlock + 8;
-    __shared__ __align__(16) uint16_t s_p[kHeads * kPitch];
+    __shared__ __align__(16) float s_p[kHeads * kPitch];
     const int all = sum_blocks(A, 0).all, run = run_length(A, all);
     const int start = (int)blockIdx.x * run;
     int left = min(run, all * A.columns - start);

@@ -132,8 +132,9 @@ def int4_attention(q, pages, table, lengths, *, scaling=None, max_length=None, o
 
     Hq is any multiple of the pool's KV heads.  A sequence without tokens gives zeros.  ``max_length`` bounds
     the lengths (default: what the table can hold; a longer length is cut to it) and steers how the work
-    is split over the GPU; a captured call keeps it.  Scores, softmax and sums are fp32; the weights are rounded to fp16 for the
-    product with V.
+    is split over the GPU; a captured call keeps it.  Scores, softmax and sums are fp32; a weight times a scale of V is
+    rounded to fp16, once, for the product with V's codes (where it is 2^-20 of the largest such product of its query head and
+    channel group, or less, to 2^-31 of that).
     """
     count, tokens, kv_heads = _pool(pages)
     sequences, width = _table(table)

@@ -483,40 +483,39 @@ __device__ __forceinline__ void work_on_column(const AttnArgs& A, float* s_p, in
     fetch_numbers();
     bool there0 = fetch(x0);  // before Q, so that the first block does not wait for it
 
-    // Q: lane (n = 4 g + h, quarter): channels 32 g + 8 quarter + [0, 8) of head h, brought to a common power
-    // of two so that the sixteenth of an element keeps its bits
+    // Q: lane (n = 4 g + h, quarter): channels 32 g + 8 quarter + [0, 8) of head h, each head brought to its own
+    // power of two so that the sixteenth of an element keeps its bits.  One power for all heads of the set
+    // took the bits of a head whose channels are 2^-25 of another's.
     half8_t qa[HB][4];
-    float qs[HB][4], c24;
+    float qs[HB][4], back_q[HB];  // sums of a group's channels; what brings head 4 hb + quarter's scores back
     {
         const int g = n >> 2;
-        float x[HB][8], top = 0.0f, sum[HB];
 #pragma unroll
         for (int hb = 0; hb < HB; ++hb) {
+            float x[8], top = 0.0f, sum = 0.0f;
             const int h = 4 * hb + (n & 3);
             uint4 r = {};
             if (h < heads) r = reinterpret_cast<const uint4*>(A.q + (row0 + h) * kDim)[4 * g + quarter];
             const uint32_t words[4] = {r.x, r.y, r.z, r.w};
-            sum[hb] = 0.0f;
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                x[hb][e] = h2f((uint16_t)(words[e >> 1] >> (16 * (e & 1))));
-                top = fmaxf(top, fabsf(x[hb][e]));
-                sum[hb] += x[hb][e];
+                x[e] = h2f((uint16_t)(words[e >> 1] >> (16 * (e & 1))));
+                top = fmaxf(top, fabsf(x[e]));
+                sum += x[e];
             }
-            sum[hb] += __shfl_xor(sum[hb], 16);
-            sum[hb] += __shfl_xor(sum[hb], 32);
+            top = fmaxf(top, dpp<0x124>(top));  // over the groups (row_ror 4, 8) and quarters
+            top = fmaxf(top, dpp<0x128>(top));
+            top = swap_max(top);
+            // 2^e with top * 2^e in [2^14, 2^15); 1 where there is nothing to scale, or no number
+            const float up = top > 0.0f && top < INFINITY ? ldexpf(1.0f, 14 - ilogbf(top)) : 1.0f;
+            sum = swap_sum16(sum, sum);
+            sum = swap_sum32(sum, sum) * up * 0x1p-24f;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) qs[hb][i] = __shfl(sum[hb], 4 * quarter + i) * A.c;
-        }
-        top = wave_max(top);
-        // 2^e with top * 2^e in [2^11, 2^12); 1 where there is nothing to scale, or no number
-        const float up = top > 0.0f && top < INFINITY ? ldexpf(1.0f, 11 - ilogbf(top)) : 1.0f;
-        c24 = A.c * 0x1p24f / up;
-#pragma unroll
-        for (int hb = 0; hb < HB; ++hb) {
+            for (int i = 0; i < 4; ++i) qs[hb][i] = __shfl(sum, 4 * quarter + i);
+            back_q[hb] = A.c * (0x1p24f / __shfl(up, quarter));
             half8_t mine;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) mine[e] = (_Float16)(x[hb][e] * (e & 2 ? up * 0.0625f : up));
+            for (int e = 0; e < 8; ++e) mine[e] = (_Float16)(x[e] * (e & 2 ? up * 0.0625f : up));
 #pragma unroll
             for (int gg = 0; gg < 4; ++gg)
 #pragma unroll
@@ -562,13 +561,13 @@ __device__ __forceinline__ void work_on_column(const AttnArgs& A, float* s_p, in
 #pragma unroll
                 for (int hb = 0; hb < HB; ++hb) d[hb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(qa[hb][g], kf, d[hb], 0, 0, 0);
             }
-            const float scale = h2f((uint16_t)x.ks[tile]) * c24, low = h2f((uint16_t)(x.ks[tile] >> 16));
+            const float scale = h2f((uint16_t)x.ks[tile]), low = h2f((uint16_t)(x.ks[tile] >> 16));
 #pragma unroll
             for (int hb = 0; hb < HB; ++hb) {
                 float t[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) t[i] = __builtin_fmaf(d[hb][i], scale, low * qs[hb][i]);
-                const float s = swap_sum16(swap_sum32(t[0], t[2]), swap_sum32(t[1], t[3]));
+                const float s = swap_sum16(swap_sum32(t[0], t[2]), swap_sum32(t[1], t[3])) * back_q[hb];
                 score[hb][tile] = 16 * tile + n < valid ? s : -INFINITY;
             }
         }

@@ -116,3 +116,26 @@ def test_values_without_a_scale(device, n, gqa):
     v[n // 2:: 3] = -0.25
     v[1::5, :, :64] *= 2.0 ** -20
     check(q, k, v)
+
+
+@SIZES
+def test_query_heads_of_different_size(device, n, gqa):
+    """Heads at both ends of fp16, each with scores of its own over large keys."""
+    q, k, v = inputs(7, n, gqa)
+    q *= (2.0 ** np.array([14, -14, 0, -9]))[np.arange(gqa) % 4, None]
+    check(q, k * 2.0 ** 13, v)
+    check(q, k * 2.0 ** -8, v)
+
+
+@pytest.mark.parametrize("bad", [np.inf, np.nan])
+@pytest.mark.parametrize("gqa", [4, 8, 16])
+def test_a_query_head_that_is_no_number(device, bad, gqa):
+    """The other heads are as they are without it."""
+    q, k, v = (x.astype(np.float16) for x in inputs(8, 400, gqa, 2.0))
+    q, k = q * np.float16(2.0 ** -12), k * np.float16(2.0 ** 11)
+    want, bound = expected(q, k, v)
+    q[0, 2, 5] = bad
+    got = attend(q, k, v)
+    assert np.isnan(got[0, 2]).all()
+    excess = (np.abs(got - want) - bound)[0, [h for h in range(gqa) if h != 2]]
+    assert excess.max() <= 0, f"{(excess > 0).sum()} values past their bound"

@@ -340,6 +340,7 @@ __global__ void __launch_bounds__(kThreads, 2) packed_kernel(PackedArgs A) {
                 for (int i = 0; i < 16; ++i) acc[db][i] *= alpha;
         }
         const float shift = kWeightBits - m;
+        float sum = 0.0f;  // of the tile: adding each pair of weights to l itself loses small ones against a large one
         const uint16_t* const sv = s_v[buf] + col * kVPitch + 8 * half;
 #pragma unroll
         for (int st = 0; st < 4; ++st) {
@@ -348,7 +349,7 @@ __global__ void __launch_bounds__(kThreads, 2) packed_kernel(PackedArgs A) {
             for (int i = 0; i < 8; i += 2) {
                 const half2_t p = {(_Float16)__builtin_amdgcn_exp2f(__builtin_fmaf(s[st >> 1][8 * (st & 1) + i], A.c, shift)),
                                    (_Float16)__builtin_amdgcn_exp2f(__builtin_fmaf(s[st >> 1][8 * (st & 1) + i + 1], A.c, shift))};
-                l = __builtin_amdgcn_fdot2(p, ones, l, false);
+                sum = __builtin_amdgcn_fdot2(p, ones, sum, false);
                 pf[i] = p[0];
                 pf[i + 1] = p[1];
             }
@@ -358,6 +359,7 @@ __global__ void __launch_bounds__(kThreads, 2) packed_kernel(PackedArgs A) {
                 acc[db] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pf, acc[db], 0, 0, 0);
             }
         }
+        l += sum;
         // a step's weights between the products of the step before
         __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
 #pragma unroll

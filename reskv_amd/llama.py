@@ -415,7 +415,10 @@ class GreedyDecoder:
         if self.mode == "reskv":
             self.caches[layer].update(rot_k, v, {"raw_keys": raw_k})
         elif self.mode == "int4":
-            if layer == 0:  # a new prompt takes the place of what was there
+            if layer == 0:  # a new prompt takes the place of what was there; decoding goes on behind it
+                if t > self.max_pos:
+                    raise RuntimeError(f"a prompt of {t} tokens passes the decoder's capacity of {self.max_pos}")
+                self.pos = t
                 for b in range(self.batch):
                     self.pages.release(b)
                 self.pages.reserve(t)

@@ -344,7 +344,8 @@ class RandomLlama:
     def prefill_packed(self, ids, lengths, sink, logits=False):
         """``prefill`` of prompts of different lengths: ids [N] one prompt behind the other,
         ``lengths`` their token counts (host numbers, at least 1, N in all).  ``sink(layer, raw_k,
-        rot_k, v)`` receives [1, Hk, N, 128]; returns the next token of each prompt [S]
+        rot_k, v)`` receives [1, Hk, N, 128], as ``Int4Cache.append`` takes it with offsets once it is
+        [N, Hk, 128] (not ``GreedyDecoder.absorb``, whose prompts have one length); returns the next token of each prompt [S]
         (or, with ``logits``, its last position's logits [S, vocab])."""
         s = self.shape
         lengths = [int(n) for n in lengths]
@@ -410,11 +411,14 @@ class GreedyDecoder:
 
     # -- prefill hand-off ----------------------------------------------------
     def absorb(self, layer, raw_k, rot_k, v):
-        """Takes one layer's prompt keys/values (the prefill sink)."""
+        """Takes one layer's prompt keys/values (the sink of ``prefill``: prompts of one length)."""
         t = raw_k.shape[2]
         if self.mode == "reskv":
             self.caches[layer].update(rot_k, v, {"raw_keys": raw_k})
         elif self.mode == "int4":
+            if raw_k.shape[0] != self.batch:
+                raise RuntimeError(f"the decoder takes {self.batch} prompts of one length, not {raw_k.shape[0]}"
+                                   " (packed prompts of different lengths go into an Int4Cache)")
             if layer == 0:  # a new prompt takes the place of what was there; decoding goes on behind it
                 if t > self.max_pos:
                     raise RuntimeError(f"a prompt of {t} tokens passes the decoder's capacity of {self.max_pos}")

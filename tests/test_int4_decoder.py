@@ -45,3 +45,16 @@ def test_a_prompt_past_the_capacity_changes_nothing(appended):
     prompt(model, 2, 10, dec.absorb)
     with pytest.raises(RuntimeError, match="capacity exhausted"):
         dec.step()
+
+
+def test_packed_prompts_are_refused(appended):
+    """``prefill_packed`` hands all prompts on in one row: not one prompt per row of the decoder."""
+    model = RandomLlama(SHAPE, "cpu", seed=3)
+    dec = GreedyDecoder(model, 2, 6, 4, "int4")
+    prompt(model, 2, 5, dec.absorb)
+    ids = torch.arange(9)
+    with pytest.raises(RuntimeError, match="takes 2 prompts of one length, not 1"):
+        model.prefill_packed(ids, [6, 3], dec.absorb)
+    with pytest.raises(RuntimeError, match="takes 2 prompts of one length, not 3"):
+        prompt(model, 3, 4, dec.absorb)
+    assert dec.pos == 5 and dec.pages.get_seq_length(0) == dec.pages.get_seq_length(1) == 5 and len(appended) == 2

@@ -323,10 +323,16 @@ class Int4Cache:
         """Attention of one token per sequence over all its tokens (``int4_attention``)."""
         return int4_attention(q, self.pool[layer], self.table, self.lengths, scaling=scaling, out=out)
 
-    def gather(self, layer):
+    def gather(self, layer, *, reserved=True):
         """(k, v, offsets): the stored values of all tokens, packed (``int4_gather``), as
-        ``packed_attention`` takes them for a prompt that continues."""
-        ends = torch.tensor([0, *self._lengths], dtype=torch.int64).cumsum(0)
+        ``packed_attention`` takes them for a prompt that continues.
+
+        The tokens reserved last are among them, so they have to be appended to this layer first.  With
+        ``reserved=False`` they are left out: what the cache held before, for a chunk whose own fp16 rows
+        are put behind each sequence's.
+        """
+        ends = self._lengths if reserved else [n - c for n, c in zip(self._lengths, self._counts)]
+        ends = torch.tensor([0, *ends], dtype=torch.int64).cumsum(0)
         offsets = ends.to(torch.int32).to(self.table.device)
         k, v = int4_gather(self.pool[layer], self.table, torch.zeros_like(self.starts), offsets, int(ends[-1]))
         return k, v, offsets

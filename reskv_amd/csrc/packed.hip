@@ -54,13 +54,14 @@ struct PackedArgs {
     const uint16_t *q, *k, *v;
     uint16_t* out;               // [Nq, Hq, 128]
     const int32_t *q_offsets, *k_offsets;
-    float* part;                 // split keys: [workgroups, 256 rows, 128]: weighted values
-    float2* stat;                // [workgroups, 256 rows]: reference of the weights, their sum
+    float* part;                 // split keys: [workgroups, record_rows, 128]: weighted values
+    float2* stat;                // [workgroups, record_rows]: reference of the weights, their sum
     int32_t* length;             // tiles of keys of a part
     long q_token, q_head, k_token, k_head, v_token, v_head;  // strides in halves
     int sequences, Nq, Nk, Hq, Hk, G;
     int items, clear_rest;
     int groups;                  // split keys: workgroups of a KV head
+    int record_rows;             // rows that a workgroup can have
     float c;                     // scaling * log2(e)
 };
 
@@ -409,7 +410,7 @@ __global__ void __launch_bounds__(kThreads, 2) packed_kernel(PackedArgs A) {
     const float total = i2f((int)ls[0]) + i2f((int)ls[1]);
     if (SPLIT && parts > 1) {
         if (r0 + col >= rows) return;
-        const long record = (long)blockIdx.x * kRows + wave * kWaveRows + col;
+        const long record = (long)blockIdx.x * A.record_rows + wave * kWaveRows + col;
         float* rec = A.part + record * kDim;
 #pragma unroll
         for (int db = 0; db < 4; ++db)
@@ -479,7 +480,7 @@ __global__ void __launch_bounds__(kThreads) packed_merge_kernel(PackedArgs A) {
         }
     }
     if (most_parts == 1) return;
-    const long record = (long)group * kRows + r, apart = (long)A.Hk * kRows;
+    const long record = (long)group * A.record_rows + r, apart = (long)A.Hk * A.record_rows;
     const float4* const rec = reinterpret_cast<const float4*>(A.part) + record * 32 + (lane & 31);
     float top = -__FLT_MAX__, o0 = 0.0f, o1 = 0.0f, o2 = 0.0f, o3 = 0.0f, total = 0.0f;
     for (int s0 = 0; s0 < most_parts; s0 += 8) {
@@ -530,12 +531,15 @@ int split_groups(int S, long Nq, int Hk, int G, long max_keys) {
     return S <= kWave && groups <= kGroups && max_keys >= 2 * kMinPart * kKeys ? kGroups / Hk : 0;
 }
 
+// Rows of a workgroup that can hold a record: no sequence has more than all rows.
+long record_rows(long Nq, int G) { return Nq * G < kRows ? Nq * G : kRows; }
+
 }  // namespace
 
 extern "C" int64_t reskv_packed_workspace_bytes(int S, int64_t Nq, int Hq, int Hk, int64_t max_keys) {
     if (S < 1 || Nq < 1 || Hk < 1 || Hq < 1 || Hq % Hk != 0 || Nq >= (1LL << 30)) return 0;
     const int64_t groups = split_groups(S, Nq, Hk, Hq / Hk, max_keys);
-    return groups == 0 ? 0 : groups * Hk * kRows * kRecord * 4 + 16;  // records, length of a part
+    return groups == 0 ? 0 : groups * Hk * record_rows(Nq, Hq / Hk) * kRecord * 4 + 16;  // records, length of a part
 }
 
 extern "C" int reskv_packed_attention(const void* q, const void* k, const void* v, void* out, const int32_t* q_offsets,
@@ -563,8 +567,9 @@ extern "C" int reskv_packed_attention(const void* q, const void* k, const void* 
     A.q_offsets = q_offsets;
     A.k_offsets = k_offsets;
     A.part = (float*)workspace;
-    A.stat = (float2*)(A.part + (long)split * Hk * kRows * kDim);
-    A.length = (int32_t*)(A.stat + (long)split * Hk * kRows);
+    A.record_rows = (int)record_rows(Nq, G);
+    A.stat = (float2*)(A.part + (long)split * Hk * A.record_rows * kDim);
+    A.length = (int32_t*)(A.stat + (long)split * Hk * A.record_rows);
     A.q_token = strides[0];
     A.q_head = strides[1];
     A.k_token = strides[2];

@@ -139,3 +139,15 @@ def test_a_query_head_that_is_no_number(device, bad, gqa):
     assert np.isnan(got[0, 2]).all()
     excess = (np.abs(got - want) - bound)[0, [h for h in range(gqa) if h != 2]]
     assert excess.max() <= 0, f"{(excess > 0).sum()} values past their bound"
+
+
+@pytest.mark.parametrize("gqa", [4, 8])
+def test_a_group_of_values_that_is_no_number(device, gqa):
+    """It shows in its 32 channels of the heads that see it, and nowhere else."""
+    q, k, v = (x.astype(np.float16) for x in inputs(9, 700, gqa, 3.0))
+    want, bound = expected(q, k, v)
+    v[300, 0, 70] = np.inf
+    got = attend(q, k, v)
+    assert np.isnan(got[:, :, 64:96]).all()
+    rest = np.r_[0:64, 96:128]
+    assert (np.abs(got - want) <= bound)[:, :, rest].all()

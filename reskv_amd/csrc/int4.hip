@@ -347,9 +347,9 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kTop = 0x1p10f, kMost = 0x1p15f;
 constexpr float kLeastReference = 0x1p-24f;  // the smallest scale: a largest weight (1) without any product needs no more
 __device__ __forceinline__ float up_of(float reference) {  // kTop over the power of two not above a reference of kLeastReference or more
-    return i2f(((127 + 10 + 127) << 23) - (f2i(reference) & 0x7F800000));
+    return i2f((127 + 10 + 127 - (f2i(reference) >> 23)) << 23);
 }
-__device__ __forceinline__ float quotient(float a, float b) { return i2f((127 << 23) + f2i(a) - f2i(b)); }  // of powers of two
+__device__ __forceinline__ float quotient(float a, float b) { return i2f(f2i(a) - f2i(b) + (127 << 23)); }  // of powers of two
 
 // Work: a column is (sequence, KV head, set of query heads), `blocks` long; the columns lie one behind the
 // other and every wave takes an equal run of blocks, across columns where it has to, so that lengths may

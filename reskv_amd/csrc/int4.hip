@@ -344,6 +344,7 @@ constexpr float kLog2e = 1.4426950408889634f;
 // of two above all of a run's scales took 28.8 us instead of 30.7 for 8 query heads, and lost what was 2^-14 below it.)
 // A power of two, as the largest weight is 1 and its products then exact, which matters where one token outweighs the
 // others: with kTop / reference itself such outputs were off by 3.3e-4 instead of 2.25e-4 (2.1e-4 is their own rounding's).
+// Rounding the products in two parts (22 bits) gave 2.12e-4, for 2% more time with 4 query heads and 11% with 8.
 constexpr float kTop = 0x1p10f, kMost = 0x1p15f;
 constexpr float kLeastReference = 0x1p-24f;  // the smallest scale: a largest weight (1) without any product needs no more
 __device__ __forceinline__ float up_of(float reference) {  // kTop over the power of two not above a reference of kLeastReference or more
@@ -450,9 +451,9 @@ __device__ __forceinline__ void load_block(Block& b, const char* p, int lane) {
 //
 // The matrix cores have rows to spare (16 for 4 heads), which is why a group's place among the rows costs nothing:
 // a block of 32 tokens takes 16 products, about 180 vector instructions and 5 KB.  Bound: memory for large
-// batches (32 sequences of 16384 tokens, 32 / 8 heads: 118 us, 5.7 TB/s, where a kernel that only reads such pieces
-// reaches 6.0), the start of a wave and the merge for small ones (1000 tokens: 4.5 + 4 us), and the chain of a block's steps
-// for 8 query heads (5 sequences of 17 to 65001: 24 us, of which 17 would be memory's).
+// batches (32 sequences of 16384 tokens, 32 / 8 heads: 119 us, 5.6 TB/s, where a kernel that only reads such pieces
+// reaches 6.0), the start of a wave and the merge for small ones (1000 tokens: 4.6 + 4 us), and the chain of a block's steps
+// for 8 query heads (5 sequences of 17 to 65001: 27 us, of which 17 would be memory's).
 template <int HB>
 __device__ __forceinline__ void work_on_column(const AttnArgs& A, float* s_p, int b, int column, int begin, int end) {
     constexpr int kHeads = 4 * HB;
@@ -721,7 +722,7 @@ __global__ void __launch_bounds__(kWave, kWavesPerSimd) attention_kernel(AttnArg
 // waves then take records' channels, two per lane, with eight loads under way, the first of them before the weights
 // are known: a merge is a chain of trips to memory, of which each costs more than what it brings.  51 records
 // one after the other took 28 us; 5 sequences of 17 to 65001 tokens and 32 heads, 8.4 us with one workgroup
-// each and the maxima read twice, and 4.8 like this.
+// each and the maxima read twice, and 5.0 like this.
 template <int PIECES>
 __global__ void __launch_bounds__(kThreads) merge_kernel(AttnArgs A) {
     constexpr int kLanes = kWave / PIECES;     // of a record's piece: PIECES records per load

@@ -892,7 +892,7 @@ extern "C" int reskv_int4_append(void* pages, int64_t num_pages, int page_tokens
     RESKV_REQUIRE(aligned16(k) && aligned16(v), "rows must be 16-byte aligned");
     for (int i = 0; i < 4; ++i) RESKV_REQUIRE(strides[i] >= 0 && strides[i] % 8 == 0, "rows must be 16-byte aligned");
     const long items = row_items(offsets, S, N) * Hk;
-    RESKV_REQUIRE(items < (1L << 31), "too many rows");
+    RESKV_REQUIRE(items < kLaunchThreads / kThreads, "too many rows or sequences");
     RowArgs A{};
     A.pool = make_pool(pages, num_pages, page_tokens, Hk, table, table_width);
     A.starts = starts;
@@ -917,7 +917,7 @@ extern "C" int reskv_int4_gather(const void* pages, int64_t num_pages, int page_
     RESKV_REQUIRE(S > 0 && N > 0 && N < (1LL << 30) && (offsets || N == S), "bad sizes (sequences %d, rows %ld)", S, (long)N);
     RESKV_REQUIRE(aligned16(k_out) && aligned16(v_out), "rows must be 16-byte aligned");
     const long items = row_items(offsets, S, N) * Hk;
-    RESKV_REQUIRE(items < (1L << 31), "too many rows");
+    RESKV_REQUIRE(items < kLaunchThreads / kThreads, "too many rows or sequences");
     RowArgs A{};
     A.pool = make_pool(pages, num_pages, page_tokens, Hk, table, table_width);
     A.starts = starts;
@@ -953,7 +953,7 @@ extern "C" int reskv_int4_attention(const void* q, const void* pages, int64_t nu
     RESKV_REQUIRE(workspace && workspace_bytes >= reskv_int4_workspace_bytes(B, Hq, Hk, max_length), "the workspace is too small");
     const long columns = (long)Hk * head_sets(G), blocks = (max_length + kBlock - 1) / kBlock;
     // blocks, records and rows are counted in 32 bits; the last wave's run may end behind the last block
-    RESKV_REQUIRE((long)B * columns * (blocks + 1) < (1L << 30) && (long)B * Hq < (1L << 31),
+    RESKV_REQUIRE((long)B * columns * (blocks + 1) < (1L << 30) && (long)B * Hq < kLaunchThreads / kThreads,
                   "too many tokens: sequences x KV heads x blocks of %d must stay below 2^30", kBlock);
     const long records = attention_records(B, Hk, G, max_length);
     AttnArgs A{};
@@ -997,7 +997,7 @@ extern "C" int reskv_copy_pages(void* pages, int layers, int64_t num_pages, int6
     A.pieces = page_bytes / 16;
     A.layer = A.pieces * num_pages;
     const long groups = (A.pieces + kCopyPieces - 1) / kCopyPieces;
-    RESKV_REQUIRE(groups < (1L << 31), "pages are too large");
+    RESKV_REQUIRE(groups < kLaunchThreads / kThreads, "pages are too large");
     for (int first = 0; first < n; first += kPairs) {
         const int count = n - first < kPairs ? n - first : kPairs;
         for (int i = 0; i < count; ++i) {

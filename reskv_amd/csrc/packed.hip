@@ -586,7 +586,7 @@ extern "C" int reskv_packed_attention(const void* q, const void* k, const void* 
     A.Hk = Hk;
     A.G = G;
     const long items = packed_items(S, Nq, G);
-    RESKV_REQUIRE(items * Hk < (1L << 31), "too many rows");
+    RESKV_REQUIRE(items * Hk < kLaunchThreads / kThreads, "too many rows or sequences");
     A.items = (int)items;
     A.groups = split;
     A.clear_rest = clear_rest;

@@ -37,6 +37,8 @@ __device__ __forceinline__ int wave_scan_int(int v) {
     return v;
 }
 
+constexpr long kLaunchThreads = 1L << 32;  // a launch has fewer: the grid is counted in threads, in 32 bits
+
 struct Item {
     int seq;    // -1: behind the last sequence's items
     int index;  // item within the sequence

@@ -11,7 +11,7 @@ from pathlib import Path
 _HERE = Path(__file__).resolve().parent
 LIB_PATH = _HERE / "libreskv_hip.so"
 
-_vp, _i, _i64, _f = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_float
+_vp, _i, _i64, _f, _d = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_float, ctypes.c_double
 
 # reskv_abi_version() of the library these signatures describe
 ABI_VERSION = 7
@@ -77,6 +77,16 @@ SIGNATURES = {
     "reskv_int4_workspace_bytes": (_i64, [_i, _i, _i, _i64]),
     "reskv_int4_attention": (_i, [_vp, _vp, _i64, _i, _vp, _i, _vp, _i, _i, _i, _f, _i64, _vp, _vp, _i64, _vp]),
     "reskv_copy_pages": (_i, [_vp, _i, _i64, _i64, _vp, _vp, _i, _vp]),
+    # include/reskv_drafts.h: trees of drafted tokens over the 4-bit cache
+    "reskv_int4_append_rope": (_i, [_vp, _i64, _i, _i, _vp, _i, _i] + [_vp] * 4 + [_i, _vp, _vp, _i64] + [_vp] * 3
+                               + [_i, _i, _i, _vp, _i, _vp]),
+    "reskv_draft_tree": (_i, [_vp, _vp, _vp, _i, _i64, _vp, _vp, _vp]),
+    "reskv_int4_tree_workspace_bytes": (_i64, [_i, _i64, _i, _i, _i64, _i]),
+    "reskv_int4_tree_attention": (_i, [_vp, _vp, _i64, _i, _vp, _i, _vp, _vp, _vp, _i, _i64, _i, _i, _f, _i64, _i, _i, _vp,
+                                       _vp, _i64, _vp]),
+    "reskv_verify_workspace_bytes": (_i64, [_i, _i64, _i64]),
+    "reskv_verify_drafts": (_i, [_vp, _i, _i64] + [_vp] * 6 + [_i64, _d, _i, _i64, _i64] + [_vp] * 4 + [_i64, _vp]),
+    "reskv_int4_keep": (_i, [_vp, _i, _i64, _i, _i, _vp, _i, _i, _vp, _vp, _i, _vp, _vp]),
     # include/reskv_llama.h: fused steps of the end-to-end decode harness
     "reskv_llama_rmsnorm": (_i, [_vp, _vp, _vp, _i, _i, _f, _vp]),
     "reskv_llama_silu_mul": (_i, [_vp, _vp, _i, _i, _vp]),

@@ -16,7 +16,7 @@ HERE = Path(__file__).resolve().parent
 CSRC = HERE / "csrc"
 LIB_NAME = "libreskv_hip.so"
 SOURCES = ("capi.hip", "encode.hip", "kmeans.hip", "decode.hip", "cache.hip", "llama_ops.hip", "prefill.hip",
-           "int4.hip", "packed.hip")
+           "int4.hip", "packed.hip", "int4_tree.hip", "drafts.hip")
 
 
 def library_path() -> Path:

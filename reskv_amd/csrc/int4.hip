@@ -8,82 +8,16 @@
 // masking alone: the bits 0 .. 15 of a nibble at bit 0 are the denormal code * 2^-24, at
 // bit 4 the number code * 2^-20 (the matrix cores keep denormals); the other operand carries
 // the factor 16 and the result the factor 2^24, both exact.
-#include "serving.h"
-#include "reskv_serving.h"
+#include "int4.h"
+#include "reskv_drafts.h"
 
 using namespace reskv;
 
 namespace {
 
-typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
-typedef _Float16 half8_t __attribute__((ext_vector_type(8)));
-typedef float float4_t __attribute__((ext_vector_type(4)));
-
-constexpr int kBlock = 32;  // tokens (>> 5 below)
-constexpr int kBlockBytes = RESKV_INT4_BLOCK_BYTES;
-constexpr int kKScale = 2048, kVCodes = 2560, kVScale = 4608, kVLow = 4864;  // byte offsets in a block
-constexpr int kThreads = 256;
-
-struct Pool {
-    char* pages;
-    const int32_t* table;  // [sequences, width]
-    long num_pages;
-    int blocks;  // per page
-    int width, heads;
-
-    // Block `block` of sequence s and head h, null where the table holds no page for it.
-    __device__ __forceinline__ char* at(int s, int block, int h) const {
-        const int entry = block / blocks;
-        if (block < 0 || entry >= width) return nullptr;
-        const int page = table[(long)s * width + entry];
-        return in_page(page, block - entry * blocks, h);
-    }
-    __device__ __forceinline__ char* in_page(int page, int block, int h) const {
-        if (page < 0 || page >= num_pages) return nullptr;
-        return pages + (((long)page * heads + h) * blocks + block) * kBlockBytes;
-    }
-};
-
-// Position of the nibble of element e = 0 .. 7 in its dword, in bits.  Elements 2 i and
-// 2 i + 1 are 16 bits apart, so that one mask makes an operand register of both.
-__host__ __device__ constexpr int nibble(int e) { return 4 * (e / 2 + 4 * (e % 2)); }
-
 // ---------------------------------------------------------------------------
 // rows into pages and back
 // ---------------------------------------------------------------------------
-
-struct RowArgs {
-    Pool pool;
-    const int32_t* starts;
-    const int32_t* offsets;  // null: row s is the one row of sequence s
-    const uint16_t *k, *v;   // append: rows
-    uint16_t *k_out, *v_out; // gather: rows [N, heads, 128]
-    long k_token, k_head, v_token, v_head;  // strides of k, v in halves
-    int sequences, N, clear_rest;
-};
-
-// The tokens [lo, hi) of block `block` of sequence seq that this workgroup handles, and the row of the first.
-struct Part {
-    int seq, block, lo, hi;
-    long row;
-};
-
-__device__ __forceinline__ Part row_part(const RowArgs& A, int item) {
-    if (!A.offsets) {
-        const int start = A.starts[item], lead = start & (kBlock - 1);
-        return {item, start >> 5, lead, lead + 1, item};
-    }
-    const Item it = find_item(item, A.sequences, [&](int s) {
-        const int n = sequence_rows(A.offsets, s, A.N).count, lead = A.starts[s] & (kBlock - 1);
-        return n == 0 ? 0 : (lead + n + kBlock - 1) / kBlock;
-    });
-    if (it.seq < 0) return {-1, it.index, 0, 0, 0};
-    const Rows r = sequence_rows(A.offsets, it.seq, A.N);
-    const int start = A.starts[it.seq], lead = start & (kBlock - 1);  // before token 0: a block without a page
-    const int lo = it.index == 0 ? lead : 0, hi = min(kBlock, lead + r.count - it.index * kBlock);
-    if (it.index < 0 || hi <= lo) return {-1, 0, 0, 0, 0};
-    return {it.seq, (start >> 5) + it.index, lo, hi, (long)r.first + it.index * kBlock + lo - lead};
-}
 
 // Range of a group of 32 channels, of which this lane has 16 and the lane next to it the others.
 // `maximum` and `minimum` hand a NaN on.
@@ -137,29 +71,133 @@ __device__ __forceinline__ void codes_of(const half2_t* x, const Group& g, uint3
     }
 }
 
+// Rotation of K and Q to their positions on the way into the pages.
+struct Turn {
+    const uint16_t* q;         // [N, heads * G, 128], null: K and V alone
+    uint16_t* q_out;           // [N, heads * G, 128]
+    const int32_t* positions;  // per row; null: the token's place in its sequence
+    const float *cos, *sin;    // [rows, half]
+    long q_token, q_head;      // strides of q in halves
+    int G, rows, half, interleaved;
+};
+
+// Channels [at, at + 8) of a head whose rotated channels come in pairs: (i, i + half), or (2 i, 2 i + 1) when
+// interleaved.  Products and sums are rounded to fp32 one by one and the result to fp16, as the torch formula does it
+// and reskv_llama_qkv_rope: pages hold the same bits whichever way a token came.
+__device__ __forceinline__ uint4 turned_piece(const Turn& R, const uint16_t* head, int at, int position) {
+#pragma clang fp contract(off)
+    const uint4 x = *reinterpret_cast<const uint4*>(head + at);
+    if (at >= 2 * R.half) return x;
+    const uint32_t xw[4] = {x.x, x.y, x.z, x.w};
+    uint32_t out[4];
+    const long table = (long)position * R.half;
+    auto times = [](uint32_t w, int upper) { return h2f((uint16_t)(upper ? w >> 16 : w)); };
+    if (R.interleaved) {
+        const float4 c = *reinterpret_cast<const float4*>(R.cos + table + at / 2), s = *reinterpret_cast<const float4*>(R.sin + table + at / 2);
+        const float cs[4] = {c.x, c.y, c.z, c.w}, sn[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float a = times(xw[i], 0), b = times(xw[i], 1);
+            out[i] = pack_halves(a * cs[i] - b * sn[i], b * cs[i] + a * sn[i]);
+        }
+    } else {
+        const bool second = at >= R.half;
+        const int i0 = second ? at - R.half : at;
+        const uint4 y = *reinterpret_cast<const uint4*>(head + (second ? i0 : at + R.half));
+        const uint32_t yw[4] = {y.x, y.y, y.z, y.w};
+        const float4* const c = reinterpret_cast<const float4*>(R.cos + table + i0);
+        const float4* const s = reinterpret_cast<const float4*>(R.sin + table + i0);
+        const float4 c0 = c[0], c1 = c[1], s0 = s[0], s1 = s[1];
+        const float cs[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w}, sn[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            float r[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const float mine = times(xw[i], e) * cs[2 * i + e], other = times(yw[i], e) * sn[2 * i + e];
+                r[e] = second ? mine + other : mine - other;
+            }
+            out[i] = pack_halves(r[0], r[1]);
+        }
+    }
+    return make_uint4(out[0], out[1], out[2], out[3]);
+}
+
+// The rows' queries of KV head h: eight threads per (row, query head), 16 channels each.
+__device__ __forceinline__ void turn_queries(const RowArgs& A, const Turn& R, const Part& P, int h) {
+    const int at = 16 * ((int)threadIdx.x & 7);
+    for (int u = (int)threadIdx.x >> 3; u < (P.hi - P.lo) * R.G; u += kThreads / 8) {
+        const int t = u / R.G, head = h * R.G + u - t * R.G;
+        const long row = P.row + t;
+        const int position = R.positions ? R.positions[row] : P.block * kBlock + P.lo + t;
+        uint4* const dst = reinterpret_cast<uint4*>(R.q_out + (row * A.pool.heads * R.G + head) * kDim + at);
+        if (position >= 0 && position < R.rows) {
+            const uint16_t* const src = R.q + row * R.q_token + head * R.q_head;
+            const uint4 x0 = turned_piece(R, src, at, position), x1 = turned_piece(R, src, at + 8, position);
+            dst[0] = x0;
+            dst[1] = x1;
+        } else if (A.clear_rest) {
+            dst[0] = dst[1] = make_uint4(0, 0, 0, 0);
+        }
+    }
+}
+
+// Queries of no sequence get zeros from the workgroups behind the last item (there is always one).
+__device__ void clear_queries(const RowArgs& A, const Turn& R, int spare, int spares, int h) {
+    const int begin = min(max(A.offsets[0], 0), A.N), end = min(max(A.offsets[A.sequences], begin), A.N);
+    const long pieces = (long)R.G * (kDim / 8), rest = (begin + A.N - end) * pieces;
+    for (long i = (long)spare * kThreads + threadIdx.x; i < rest; i += (long)spares * kThreads) {
+        const long r = i / pieces, row = r < begin ? r : end + r - begin;
+        reinterpret_cast<uint4*>(R.q_out + (row * A.pool.heads + h) * R.G * kDim)[i - r * pieces] = make_uint4(0, 0, 0, 0);
+    }
+}
+
 // One workgroup per (block of 32 tokens that gets rows, head); thread (token, part) has 16 channels
-// of K and of V, so that a wave has the eight tokens that share the dwords of V.
+// of K and of V, so that a wave has the eight tokens that share the dwords of V.  With TURN, K is rotated before it is
+// quantised, the KV head's queries are rotated beside it, and a row whose position lies outside the tables is left out.
 //
 // Bound: memory (512 bytes in and 160 out per token and head), with the vector ALU close behind: 37,200 tokens of 8 heads
 // in 47 us (4.2 TB/s; a large copy reaches 4.8).  With a division per code and V transposed byte by byte through the
 // LDS it was 74 us.  32 single tokens: 6 us, a chain of five trips to memory (offsets, page, rows, old nibbles, out).
-__global__ void __launch_bounds__(kThreads) append_kernel(RowArgs A) {
+template <bool TURN>
+__global__ void __launch_bounds__(kThreads) append_kernel(RowArgs A, Turn R) {
     __shared__ __align__(16) uint32_t s_k[512], s_v[512];  // codes as stored
     __shared__ uint32_t s_kp[128];                         // K scalings as stored
     __shared__ uint16_t s_vp[256];                         // V scales and lowest values as stored
-    const int h = (int)blockIdx.x % A.pool.heads;
-    const Part P = row_part(A, (int)blockIdx.x / A.pool.heads);
-    if (P.seq < 0) return;
+    __shared__ bool s_in[kBlock];                          // TURN: tokens whose position is in the tables
+    const int h = (int)blockIdx.x % A.pool.heads, item = (int)blockIdx.x / A.pool.heads;
+    const Part P = row_part(A, item);
+    if (P.seq < 0) {
+        if (TURN && A.clear_rest && R.q && A.offsets && P.block >= 0 && P.hi == 0) {
+            const int first = item - P.block;  // the number of items
+            clear_queries(A, R, P.block, (int)gridDim.x / A.pool.heads - first, h);
+        }
+        return;
+    }
+    if (TURN && R.q) turn_queries(A, R, P, h);
     const int tid = threadIdx.x, token = tid >> 3, part = tid & 7, group = part >> 1;
-    const bool mine = token >= P.lo && token < P.hi;
+    bool mine = token >= P.lo && token < P.hi;
     uint4 kw[2] = {}, vw[2] = {};
     if (mine) {
         const long row = P.row + token - P.lo;
-        const uint4* ks = reinterpret_cast<const uint4*>(A.k + row * A.k_token + h * A.k_head) + 2 * part;
+        const uint16_t* const key = A.k + row * A.k_token + h * A.k_head;
+        const uint4* ks = reinterpret_cast<const uint4*>(key) + 2 * part;
         const uint4* vs = reinterpret_cast<const uint4*>(A.v + row * A.v_token + h * A.v_head) + 2 * part;
-        kw[0] = ks[0], kw[1] = ks[1];
         vw[0] = vs[0], vw[1] = vs[1];
+        if (TURN) {
+            const int position = R.positions ? R.positions[row] : P.block * kBlock + token;
+            mine = position >= 0 && position < R.rows;
+            if (mine) {
+                kw[0] = turned_piece(R, key, 16 * part, position);
+                kw[1] = turned_piece(R, key, 16 * part + 8, position);
+            }
+        } else {
+            kw[0] = ks[0], kw[1] = ks[1];
+        }
     }
+    if (TURN && part == 0) s_in[token] = mine;
+    // whether token t of the block is stored (TURN: behind the barrier)
+    auto stored = [&](int t) { return t >= P.lo && t < P.hi && (!TURN || s_in[t]); };
     char* const block = A.pool.at(P.seq, P.block, h);
     if (!block) return;
     uint32_t code[16];
@@ -220,27 +258,25 @@ __global__ void __launch_bounds__(kThreads) append_kernel(RowArgs A) {
     __syncthreads();
     if (tid < 128) {
         const int t = (tid >> 6) * 16 + (tid & 15);  // the token of both: piece (tile, quarter, token), dword (tile, group, token)
-        if (t >= P.lo && t < P.hi) {
+        if (stored(t)) {
             reinterpret_cast<uint4*>(block)[tid] = reinterpret_cast<const uint4*>(s_k)[tid];
             reinterpret_cast<uint32_t*>(block + kKScale)[tid] = s_kp[tid];
         }
     }
-    {
-        const int t = tid & 31;  // half (scale or low, group, token)
-        if (t >= P.lo && t < P.hi) reinterpret_cast<uint16_t*>(block + kVScale)[tid] = s_vp[tid];
-    }
+    if (stored(tid & 31))  // half (scale or low, group, token)
+        reinterpret_cast<uint16_t*>(block + kVScale)[tid] = s_vp[tid];
     // V codes: dword (c / 64, t / 8, c % 16, c / 16 % 4) has the eight tokens of a channel; of a dword whose
     // tokens are not all new the others' nibbles stay
     if (tid < 128) {
         const int t0 = 8 * ((tid >> 4) & 3);
-        if (t0 + 8 <= P.lo || t0 >= P.hi) return;
+        uint32_t fresh = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (stored(t0 + i)) fresh |= 15u << nibble(i);
+        if (fresh == 0) return;
         uint4* const dst = reinterpret_cast<uint4*>(block + kVCodes) + tid;
         uint4 w = reinterpret_cast<const uint4*>(s_v)[tid];
-        if (t0 < P.lo || t0 + 8 > P.hi) {
-            uint32_t fresh = 0;
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-                if (t0 + i >= P.lo && t0 + i < P.hi) fresh |= 15u << nibble(i);
+        if (fresh != ~0u) {
             const uint4 old = *dst;
             w.x = (w.x & fresh) | (old.x & ~fresh);
             w.y = (w.y & fresh) | (old.y & ~fresh);
@@ -250,8 +286,6 @@ __global__ void __launch_bounds__(kThreads) append_kernel(RowArgs A) {
         *dst = w;
     }
 }
-
-__device__ __forceinline__ uint32_t pack_halves(float a, float b) { return (uint32_t)f2h(a) | ((uint32_t)f2h(b) << 16); }
 
 // Rows of no sequence get zeros from the workgroups behind the last item (there is always one).
 __device__ void clear_rows(const RowArgs& A, int spare, int spares, int h) {
@@ -388,30 +422,6 @@ __device__ __forceinline__ Sums sum_blocks(const AttnArgs& A, int b) {
 }
 // Blocks of a wave's run.
 __device__ __forceinline__ int run_length(const AttnArgs& A, int all) { return max((all * A.columns + A.waves - 1) / A.waves, 1); }
-
-__device__ __forceinline__ float swap_sum32(float a, float b) {
-    const auto r = __builtin_amdgcn_permlane32_swap((uint32_t)f2i(a), (uint32_t)f2i(b), false, false);
-    return i2f((int)r[0]) + i2f((int)r[1]);
-}
-__device__ __forceinline__ float swap_sum16(float a, float b) {
-    const auto r = __builtin_amdgcn_permlane16_swap((uint32_t)f2i(a), (uint32_t)f2i(b), false, false);
-    return i2f((int)r[0]) + i2f((int)r[1]);
-}
-// Maximum over the four quarters of the wave.
-__device__ __forceinline__ float swap_max(float a) {
-    const auto r = __builtin_amdgcn_permlane16_swap((uint32_t)f2i(a), (uint32_t)f2i(a), false, false);
-    a = fmaxf(i2f((int)r[0]), i2f((int)r[1]));
-    const auto s = __builtin_amdgcn_permlane32_swap((uint32_t)f2i(a), (uint32_t)f2i(a), false, false);
-    return fmaxf(i2f((int)s[0]), i2f((int)s[1]));
-}
-
-// The operand register pair (elements 0 .. 7) of a dword of codes: elements 0, 1, 4, 5 times
-// 2^-24 and 2, 3, 6, 7 times 2^-20.
-__device__ __forceinline__ half8_t operand(uint32_t d) {
-    const uint32_t e = d >> 8;
-    const uint4 w = make_uint4(d & 0x000F000Fu, d & 0x00F000F0u, e & 0x000F000Fu, e & 0x00F000F0u);
-    return __builtin_bit_cast(half8_t, w);
-}
 
 constexpr int kPitch = kBlock + 16;  // fp32 weights of a head in the LDS: the four quarters' writes fall on different banks
 
@@ -839,35 +849,6 @@ __global__ void __launch_bounds__(kThreads) copy_kernel(CopyArgs A) {
 // host side
 // ---------------------------------------------------------------------------
 
-bool aligned16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
-
-bool pool_ok(const void* pages, int64_t num_pages, int page_tokens, int Hk, const int32_t* table, int width) {
-    if (!pages || !table) {
-        reskv_host::set_error("null pointer");
-        return false;
-    }
-    if (num_pages < 1 || num_pages >= (1LL << 31) || Hk < 1 || width < 1) {
-        reskv_host::set_error("bad pool sizes (pages %ld, KV heads %d, table width %d)", (long)num_pages, Hk, width);
-        return false;
-    }
-    if (page_tokens < kBlock || page_tokens % kBlock != 0 || (long)width * page_tokens >= (1L << 31)) {
-        reskv_host::set_error("a page holds a multiple of %d tokens, a sequence fewer than 2^31", kBlock);
-        return false;
-    }
-    if (!aligned16(pages)) {
-        reskv_host::set_error("pages must be 16-byte aligned");
-        return false;
-    }
-    return true;
-}
-
-Pool make_pool(const void* pages, int64_t num_pages, int page_tokens, int Hk, const int32_t* table, int width) {
-    return Pool{(char*)pages, table, (long)num_pages, page_tokens / kBlock, width, Hk};
-}
-
-// Blocks that N rows of S sequences can touch: a sequence of n rows touches at most n / 32 + 2.
-long row_items(const int32_t* offsets, int S, long N) { return offsets ? N / kBlock + 2L * S + 1 : (long)S; }
-
 // Sets of query heads of a KV head: of 4, or of 8 when there are more.
 int head_sets(int G) { return G <= 4 ? 1 : (G + 7) / 8; }
 int set_heads(int G) { return G <= 4 ? 4 : 8; }
@@ -905,8 +886,53 @@ extern "C" int reskv_int4_append(void* pages, int64_t num_pages, int page_tokens
     A.v_head = strides[3];
     A.sequences = S;
     A.N = (int)N;
-    hipLaunchKernelGGL(append_kernel, dim3((unsigned)items), dim3(kThreads), 0, (hipStream_t)stream, A);
+    hipLaunchKernelGGL(append_kernel<false>, dim3((unsigned)items), dim3(kThreads), 0, (hipStream_t)stream, A, Turn{});
     return reskv_host::check_launch("append_kernel");
+}
+
+extern "C" int reskv_int4_append_rope(void* pages, int64_t num_pages, int page_tokens, int Hk, const int32_t* table,
+                                      int table_width, int S, const int32_t* starts, const int32_t* offsets,
+                                      const int32_t* positions, const void* q, int Hq, const void* k, const void* v,
+                                      int64_t N, const int64_t* strides, const float* cos, const float* sin, int rows,
+                                      int rotary, int interleaved, void* q_out, int clear_rest, void* stream) {
+    RESKV_REQUIRE(starts && k && v && strides && cos && sin && (!q || q_out), "null pointer");
+    if (!pool_ok(pages, num_pages, page_tokens, Hk, table, table_width)) return 1;
+    RESKV_REQUIRE(S > 0 && N > 0 && N < (1LL << 30) && (offsets || N == S), "bad sizes (sequences %d, rows %ld)", S, (long)N);
+    RESKV_REQUIRE(!q || (Hq > 0 && Hq % Hk == 0 && Hq < (1 << 20)), "the query heads (%d) must be a multiple of the KV heads (%d)", Hq, Hk);
+    RESKV_REQUIRE(rows > 0 && rotary >= 16 && rotary <= kDim && rotary % 16 == 0,
+                  "the rotated channels (%d) must be a multiple of 16 up to 128, and the tables have rows", rotary);
+    RESKV_REQUIRE(aligned16(q) && aligned16(k) && aligned16(v) && aligned16(q_out) && aligned16(cos) && aligned16(sin),
+                  "tensors must be 16-byte aligned");
+    for (int i = q ? 0 : 2; i < 6; ++i) RESKV_REQUIRE(strides[i] >= 0 && strides[i] % 8 == 0, "rows must be 16-byte aligned");
+    const long items = row_items(offsets, S, N) * Hk;
+    RESKV_REQUIRE(items < kLaunchThreads / kThreads, "too many rows or sequences");
+    RowArgs A{};
+    A.pool = make_pool(pages, num_pages, page_tokens, Hk, table, table_width);
+    A.starts = starts;
+    A.offsets = offsets;
+    A.k = (const uint16_t*)k;
+    A.v = (const uint16_t*)v;
+    A.k_token = strides[2];
+    A.k_head = strides[3];
+    A.v_token = strides[4];
+    A.v_head = strides[5];
+    A.sequences = S;
+    A.N = (int)N;
+    A.clear_rest = clear_rest;
+    Turn R{};
+    R.q = (const uint16_t*)q;
+    R.q_out = (uint16_t*)q_out;
+    R.positions = positions;
+    R.cos = cos;
+    R.sin = sin;
+    R.q_token = strides[0];
+    R.q_head = strides[1];
+    R.G = q ? Hq / Hk : 0;
+    R.rows = rows;
+    R.half = rotary / 2;
+    R.interleaved = interleaved;
+    hipLaunchKernelGGL(append_kernel<true>, dim3((unsigned)items), dim3(kThreads), 0, (hipStream_t)stream, A, R);
+    return reskv_host::check_launch("append_rope_kernel");
 }
 
 extern "C" int reskv_int4_gather(const void* pages, int64_t num_pages, int page_tokens, int Hk, const int32_t* table,

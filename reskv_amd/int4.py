@@ -7,13 +7,16 @@ the group's smallest value and ``scale`` a fifteenth of its range, both fp16, an
 nearest of the sixteen values ``code * scale + low``.
 
 * ``int4_append`` puts rows of K and V into pages, prompts and single tokens alike;
+* ``int4_append_rope`` does the same with keys that are not rotated yet, and rotates them and the queries on the way;
 * ``int4_gather`` gives them back in fp16, for a prompt that continues on cached tokens;
 * ``int4_attention`` attends one token of every sequence over its pages;
+* ``int4_tree_attention`` attends several, the nodes of a chain or tree of drafted tokens;
+* ``int4_keep`` moves the drafted tokens that were accepted together, in every layer's pool at once;
 * ``copy_pages`` copies pages in every layer's pool at once;
 * ``Int4Cache`` keeps the pages of a decoder stack: which sequence has which, forks that share
   them, their release and compaction.
 
-K is stored as it is given: rotated keys, as the dense ring of ``ResKVLayerCache`` has them.
+``int4_append`` stores K as it is given: rotated keys, as the dense ring of ``ResKVLayerCache`` has them.
 Like ``attention`` these are inference operators: no gradient is recorded.  Page tables, positions and
 lengths stay on the GPU and are not read on the host: a page number outside the pool, or a position outside
 the table, stands for a token that is not there, which appends leave out and reads pass over.
@@ -29,6 +32,7 @@ from ._extension import _require, _workspace
 from .packed import _INF, _int32, _kernel_rows, _launch, _new, _rows, _same_gpu, _strides
 
 BLOCK_TOKENS = 32
+TREE_NODES = 64  # drafted tokens of a sequence, at most
 TOKEN_BYTES = 160  # of one KV head, K and V
 
 
@@ -88,6 +92,70 @@ def int4_append(pages, table, starts, k, v, offsets=None):
     _launch("reskv_int4_append", index, pages.data_ptr(), count, tokens, heads, table.data_ptr(), width, sequences,
             starts.data_ptr(), None if offsets is None else offsets.data_ptr(), k.data_ptr(), v.data_ptr(), n,
             _strides(k, v))
+
+
+def _rotation(cos, sin):
+    """(rows, rotated channels) of the tables."""
+    for name, t in (("cos", cos), ("sin", sin)):
+        if t.dtype is not torch.float32 or t.dim() != 2 or not t.is_contiguous():
+            raise RuntimeError(f"{name} must be a contiguous fp32 matrix [positions, half of the rotated channels]")
+    _require(cos.shape == sin.shape, "cos and sin must have the same shape")
+    _require(0 < cos.shape[0] < 1 << 31, "cos and sin must have a row for every position")
+    _require(cos.shape[1] in range(8, 65, 8), "the rotated channels must be a multiple of 16, up to 128")
+    return cos.shape[0], 2 * cos.shape[1]
+
+
+def int4_append_rope(pages, table, starts, q, k, v, cos, sin, offsets=None, *, positions=None, interleaved=False, out=None):
+    """``int4_append`` of keys that are not rotated yet: k goes to its position on the way into the pages, and the
+    queries q, fp16 [N, Hq, 128] (None: keys and values alone), beside it.  Returns the rotated queries, ``out`` when given
+    (contiguous, apart from q).
+
+    cos and sin, fp32 [positions, R / 2], hold what a position turns the first R channels of a head by (R a
+    multiple of 16, up to 128; the others stay): ``fp16(a c - b s), fp16(b c + a s)`` of the pairs (i, i + R / 2), or (2 i, 2 i + 1) when
+    ``interleaved``, products and sums rounded to fp32, as ``fused_qkv_rope`` does it: pages and queries get the same bits as
+    by that and ``int4_append``.  A row's position is its token's place in the sequence, or ``positions[row]`` (int32 [N]), as
+    the nodes of a tree need it.  Rows whose position is outside the tables are not stored; their queries and
+    those of no sequence are zero, or left as they are in ``out``.
+    """
+    count, tokens, heads = _pool(pages)
+    sequences, width = _table(table)
+    _int32("starts", starts, sequences)
+    _rows("k", k, heads)
+    _rows("v", v, heads)
+    n = k.shape[0]
+    _require(v.shape[0] == n, "k and v must have the same number of rows")
+    q_heads = 0
+    if q is not None:
+        _rows("q", q)
+        q_heads = q.shape[1]
+        _require(q.shape[0] == n, "q and k must have the same number of rows")
+        _require(q_heads > 0 and q_heads % heads == 0, "the query heads must be a multiple of the KV heads")
+    if offsets is None:
+        _require(n == sequences, "without offsets there must be one row for every sequence")
+    else:
+        _int32("offsets", offsets, sequences + 1)
+    if positions is not None:
+        _int32("positions", positions, n)
+    rows, rotated = _rotation(cos, sin)
+    if out is not None:
+        _require(q is not None, "out is for the queries, of which there are none")
+        _rows("out", out, q_heads)
+        _require(out.shape[0] == n and out.is_contiguous(), "out must be contiguous and shaped like q")
+    index = _same_gpu(pages, table, starts, k, v, cos, sin, q, offsets, positions, out)
+    clear = out is None
+    if q is not None and clear:
+        out = _new(q, (n, q_heads, 128))
+    if n == 0 or sequences == 0:
+        return out.zero_() if clear and out is not None else out
+    k, v = _kernel_rows(k), _kernel_rows(v)
+    q = k if q is None else _kernel_rows(q)
+    cos, sin = (t if not t.data_ptr() & 15 else t.detach().clone() for t in (cos, sin))
+    _launch("reskv_int4_append_rope", index, pages.data_ptr(), count, tokens, heads, table.data_ptr(), width, sequences,
+            starts.data_ptr(), None if offsets is None else offsets.data_ptr(),
+            None if positions is None else positions.data_ptr(), q.data_ptr() if q_heads else None, q_heads, k.data_ptr(),
+            v.data_ptr(), n, _strides(q, k, v), cos.data_ptr(), sin.data_ptr(), rows, rotated, bool(interleaved),
+            out.data_ptr() if q_heads else None, clear)
+    return out
 
 
 def int4_gather(pages, table, starts, offsets, rows, out=None):
@@ -166,6 +234,86 @@ def int4_attention(q, pages, table, lengths, *, scaling=None, max_length=None, o
     return out
 
 
+@lru_cache(4096)  # a function of the sizes alone
+def _tree_workspace(sequences, rows, heads, kv_heads, most, nodes):
+    return _lib.lib().reskv_int4_tree_workspace_bytes(sequences, rows, heads, kv_heads, most, nodes)
+
+
+def int4_tree_attention(q, pages, table, lengths, offsets, seen=None, *, scaling=None, max_length=None,
+                        max_nodes=TREE_NODES, out=None):
+    """Attention of several tokens of every sequence, the nodes of a chain or tree of drafts: rows ``offsets[s]`` to
+    ``offsets[s + 1]`` (int32 [S + 1]) of q fp16 [N, Hq, 128] (rotated) are the nodes of sequence s, and its last tokens in the
+    pages: of its first ``lengths[s]`` (int32 [S]) tokens, those before the nodes are seen by every node, and the
+    token of node j by those nodes i whose mask ``seen[row i]`` (int64 [N]) has bit j set: ``draft_tree`` makes the masks of trees,
+    None is a chain (a node sees itself and the nodes before it).  What a node does not see does not matter to it, NaN and
+    infinities included; a node that sees nothing gives zeros.
+
+    Hq is any multiple of the pool's KV heads.  ``max_length`` bounds the lengths as in ``int4_attention``; ``max_nodes``
+    (up to 64) bounds the nodes of a sequence: both steer how the work is split.  Returns fp16 [N, Hq, 128], ``out``
+    when given (contiguous); rows of no sequence and nodes from ``max_nodes`` on are zero, or left as they are in ``out``.
+
+    Scores, softmax and sums are fp32; V is rounded to fp16 (what ``int4_gather`` gives) and so are the softmax weights, for
+    their product.
+    """
+    count, tokens, kv_heads = _pool(pages)
+    sequences, width = _table(table)
+    _int32("lengths", lengths, sequences)
+    _int32("offsets", offsets, sequences + 1)
+    _rows("q", q)
+    n, heads, _ = q.shape
+    _require(heads > 0 and heads % kv_heads == 0, "the query heads must be a multiple of the KV heads")
+    if seen is not None and not (seen.dtype is torch.int64 and seen.dim() == 1 and seen.is_contiguous() and seen.shape[0] == n):
+        raise RuntimeError("seen must be a contiguous int64 vector with a mask for every row of q")
+    scaling = 128 ** -0.5 if scaling is None else float(scaling)
+    _require(0.0 < scaling < _INF, "scaling must be positive")
+    most = width * tokens if max_length is None else int(max_length)
+    _require(most >= 0, "max_length must not be negative")
+    nodes = int(max_nodes)
+    _require(1 <= nodes <= TREE_NODES, f"max_nodes must be in 1 .. {TREE_NODES}")
+    clear = out is None
+    if not clear:
+        _rows("out", out, heads)
+        _require(out.shape[0] == n and out.is_contiguous(), "out must be contiguous and shaped like q")
+    index = _same_gpu(q, pages, table, lengths, offsets, seen, out)
+    if clear:
+        out = _new(q, (n, heads, 128))
+    if n == 0 or sequences == 0:
+        return out.zero_() if clear else out
+    if not q.is_contiguous() or q.data_ptr() & 15:
+        q = q.detach().clone(memory_format=torch.contiguous_format)
+    most, nodes = min(most, width * tokens), min(nodes, n)
+    nbytes = _tree_workspace(sequences, n, heads, kv_heads, most, nodes)
+    work = _workspace(nbytes, q.device)
+    _launch("reskv_int4_tree_attention", index, q.data_ptr(), pages.data_ptr(), count, tokens, table.data_ptr(), width,
+            lengths.data_ptr(), offsets.data_ptr(), None if seen is None else seen.data_ptr(), sequences, n, heads, kv_heads,
+            scaling, most, nodes, clear, out.data_ptr(), work.data_ptr(), nbytes)
+    return out
+
+
+def int4_keep(pages, table, starts, path, counts):
+    """Moves accepted tokens together: token ``starts[s] + path[s, j]`` of sequence s becomes its token ``starts[s] + j``, for
+    j below ``counts[s]``, all of them at once, in a pool [pages, ...] or in every layer's pool [layers, pages, KV heads, bytes].
+
+    ``starts`` and ``counts`` are int32 [S], ``path`` int32 [S, up to 64], as ``verify_drafts`` gives them.  Entries outside
+    0 .. 63 and tokens without a page are left out.  No two sequences of a call may have these tokens in one page.
+    """
+    _require(pages.dtype is torch.uint8 and pages.dim() in (3, 4) and pages.is_contiguous(),
+             "pages must be a contiguous uint8 tensor [pages, KV heads, bytes] or [layers, pages, KV heads, bytes]")
+    layers = 1 if pages.dim() == 3 else pages.shape[0]
+    if layers:
+        count, tokens, heads = _pool(pages if pages.dim() == 3 else pages[0])
+    sequences, width = _table(table)
+    _int32("starts", starts, sequences)
+    _int32("counts", counts, sequences)
+    _require(path.dtype is torch.int32 and path.dim() == 2 and path.is_contiguous() and path.shape[0] == sequences
+             and path.shape[1] <= TREE_NODES, f"path must be a contiguous int32 matrix [sequences, up to {TREE_NODES}]")
+    index = _same_gpu(pages, table, starts, path, counts)
+    if sequences == 0 or layers == 0 or path.shape[1] == 0:
+        return
+    _launch("reskv_int4_keep", index, pages.data_ptr(), layers, count, tokens, heads, table.data_ptr(), width, sequences,
+            starts.data_ptr(), path.data_ptr(), path.shape[1], counts.data_ptr())
+
+
 def copy_pages(pages, source, target):
     """Copies page ``source[i]`` to page ``target[i]`` (host sequences of page numbers) in a pool [pages, ...]
     or in every layer's pool [layers, pages, KV heads, bytes], in one launch per 384 pages.
@@ -205,8 +353,9 @@ class Int4Cache:
 
     Which page belongs to whom is kept on the host; ``table``, ``starts`` (of the reserved tokens) and
     ``lengths`` (with them) are its copies on the GPU, at fixed addresses, so that appends and attention
-    may be captured into a graph and replayed after every ``reserve``, which itself stays outside.  Sequences that
-    were forked share pages; ``reserve`` gives a sequence a copy of its last page before it writes to a shared one.
+    may be captured into a graph and replayed after every ``reserve``, which itself stays outside.  Drafted
+    tokens are reserved like others, appended (``append_rope``), attended as chains or trees (``attend_tree``), and cut to those that
+    were accepted (``keep``).  Sequences that were forked share pages; ``reserve`` gives a sequence a copy of its last page before it writes to a shared one.
     """
 
     def __init__(self, layers, kv_heads, sequences, max_length, *, page_tokens=64, pages=None, device="cuda"):
@@ -322,6 +471,43 @@ class Int4Cache:
     def attend(self, layer, q, *, scaling=None, out=None):
         """Attention of one token per sequence over all its tokens (``int4_attention``)."""
         return int4_attention(q, self.pool[layer], self.table, self.lengths, scaling=scaling, out=out)
+
+    def append_rope(self, layer, q, k, v, cos, sin, offsets=None, *, positions=None, interleaved=False, out=None):
+        """The reserved tokens of one layer with keys that are not rotated yet; returns the rotated queries
+        (``int4_append_rope``)."""
+        _require(not self._forked, "sequences were forked: reserve tokens before the next append")
+        return int4_append_rope(self.pool[layer], self.table, self.starts, q, k, v, cos, sin, offsets, positions=positions,
+                                interleaved=interleaved, out=out)
+
+    def attend_tree(self, layer, q, offsets, seen=None, *, scaling=None, max_nodes=TREE_NODES, out=None):
+        """Attention of the reserved tokens, the nodes of a chain or tree of drafts (``int4_tree_attention``)."""
+        return int4_tree_attention(q, self.pool[layer], self.table, self.lengths, offsets, seen, scaling=scaling,
+                                   max_nodes=max_nodes, out=out)
+
+    def keep(self, path, counts):
+        """Of the tokens reserved last, drafts by now appended to every layer, row s keeps the ``counts[s]`` that ``path[s]`` (int32
+        [sequences, up to 64]) lists, in that order behind what it had before them; the others are gone and their pages
+        free.  ``counts`` (int32 on the GPU, as ``verify_drafts`` gives it) is read on the host, so that this stays outside
+        captured graphs; returns it as a list."""
+        _require(not (self.pool.is_cuda and torch.cuda.is_current_stream_capturing()),
+                 "keep works on the host and cannot be captured")
+        _require(not self._forked, "sequences were forked: the drafts of rows that share pages cannot be kept apart")
+        _int32("counts", counts, self.sequences)
+        kept = counts.tolist()
+        _require(all(0 <= k <= c for k, c in zip(kept, self._counts)), "a row keeps between none and all of the tokens reserved last")
+        int4_keep(self.pool, self.table, self.starts, path, counts)
+        changed = []
+        for s, (k, c) in enumerate(zip(kept, self._counts)):
+            self._lengths[s] += k - c
+            need = -(-self._lengths[s] // self.page_tokens)
+            if need < len(self._pages[s]):
+                rest, self._pages[s] = self._pages[s][need:], self._pages[s][:need]
+                self._drop(rest)
+                changed.append(s)
+        self._counts = kept
+        self._publish(changed)
+        self._publish_lengths()
+        return kept
 
     def gather(self, layer, *, reserved=True):
         """(k, v, offsets): the stored values of all tokens, packed (``int4_gather``), as

@@ -35,7 +35,8 @@ from . import _lib
 from ._extension import dense_decode, eager
 from .cache import ResKVLayerCache
 from .config import ResKVKernelConfig
-from .int4 import Int4Cache
+from .drafts import draft_tree, verify_drafts
+from .int4 import TREE_NODES, Int4Cache
 from .packed import packed_attention
 
 
@@ -538,6 +539,9 @@ class GreedyDecoder:
             return self._step(events)
 
     def _step(self, events):
+        if self.mode == "int4" and len(set(self.pages._lengths)) > 1:  # rows that kept different numbers of drafts
+            self._nodes(self.tok[:, None], [], 0.0, None, None, None, events)
+            return self.tok
         if self.graphs is None:
             self.capture()
         self._set_slots()
@@ -558,3 +562,73 @@ class GreedyDecoder:
         head.replay()
         self.pos += 1
         return self.tok
+
+    # -- drafts ------------------------------------------------------------------
+    def step_drafts(self, drafts, parents=None, *, temperature=0.0, accept=None, sample=None, draft=None):
+        """One decoding step that checks drafted tokens (4-bit mode): ``drafts`` int64 [B, m] on the GPU, m up to 63, are
+        nodes 1 .. m of every row's tree, whose root, node 0, is the token that the last step returned; ``parents`` (m host numbers, the
+        same for every row) names each draft's parent, a node before it (default: a chain).  Temperature 0
+        decodes greedily; otherwise ``accept`` (fp32 [B, m + 1]), ``sample`` (fp32 [B]) and ``draft`` (fp32 [B, m + 1, vocab] or None) are
+        as ``verify_drafts`` takes them.
+
+        Returns (tokens, counts): the new tokens of every row, the accepted drafts and the one behind them, int64 [B, m + 1] with
+        -1 behind, and how many they are, a list.  Rows may keep different numbers: later steps go on
+        behind each row's own tokens."""
+        _need(self.mode == "int4", "drafts need the 4-bit cache")
+        _need(drafts.dtype == torch.int64 and drafts.dim() == 2 and drafts.shape[0] == self.batch,
+              f"drafts must be an int64 matrix with a row for each of the {self.batch} sequences")
+        m = drafts.shape[1]
+        _need(m < TREE_NODES, f"a tree has up to {TREE_NODES} nodes, the root among them")
+        parents = list(range(m)) if parents is None else [int(p) for p in parents]
+        _need(len(parents) == m and all(0 <= p <= i for i, p in enumerate(parents)),
+              "parents must name a node before it for every draft")
+        for name, t, shape in (("accept", accept, (self.batch, m + 1)), ("sample", sample, (self.batch,)),
+                               ("draft", draft, (self.batch, m + 1, self.model.shape.vocab))):
+            _need(t is None or tuple(t.shape) == shape, f"{name} must be {list(shape)}")
+        _need(temperature == 0.0 or (accept is not None and sample is not None), "sampling needs random numbers")
+        _on_gpu(drafts)
+        with torch.cuda.device(self.x.device):
+            return self._nodes(torch.cat([self.tok[:, None], drafts], dim=1), parents, temperature, accept, sample, draft, None)
+
+    def _nodes(self, ids, parents, temperature, accept, sample, draft, events):
+        s, dev = self.model.shape, self.model.device
+        n = ids.shape[1]
+        if max(self.pages._lengths) + n > self.max_pos:
+            raise RuntimeError("decoder capacity exhausted")
+        self.pages.reserve(n)
+        offsets = torch.arange(0, (self.batch + 1) * n, n, dtype=torch.int32, device=dev)
+        above = torch.tensor([-1, *parents] * self.batch, dtype=torch.int32).to(dev)
+        seen, positions = draft_tree(above, offsets, self.pages.starts)
+        x = self.model.embed[ids.clamp(0, s.vocab - 1)].view(-1, s.hidden)  # a draft outside the vocabulary is passed over
+        heads, kv = s.heads, s.kv_heads
+        h, act = torch.empty_like(x), torch.empty(x.shape[0], s.ffn, dtype=x.dtype, device=dev)
+        for li, p in enumerate(self.model.layers):
+            qkv = F.linear(fused_rmsnorm(x, p["n1"], s.rms_eps, h), p["wqkv"]).view(-1, heads + 2 * kv, s.head_dim)
+            marks = None if events is None else [torch.cuda.Event(enable_timing=True) for _ in range(2)]
+            if marks:
+                marks[0].record()
+            q = self.pages.append_rope(li, qkv[:, :heads], qkv[:, heads: heads + kv], qkv[:, heads + kv:], self.cos, self.sin,
+                                       offsets, positions=positions)
+            attn = self.pages.attend_tree(li, q, offsets, seen, scaling=self.model.scaling, max_nodes=n)
+            if marks:
+                marks[1].record()
+                events.append(tuple(marks))
+            x.addmm_(attn.view(-1, s.hidden), p["wo"].t())
+            fused_rmsnorm(x, p["n2"], s.rms_eps, h)
+            x.addmm_(fused_silu_mul(F.linear(h, p["wgu"]), act), p["wd"].t())
+        logits = F.linear(fused_rmsnorm(x, self.model.norm, s.rms_eps, h), self.model.lm_head)
+        path, counts, token = verify_drafts(logits, ids.reshape(-1), above, offsets, None if accept is None else accept.reshape(-1),
+                                            sample, draft=None if draft is None else draft.flatten(0, 1),
+                                            temperature=temperature)
+        kept = self.pages.keep(path, counts)
+        if bool((token < 0).any()):
+            raise RuntimeError("the model's logits hold a NaN or an infinity")
+        self.tok.copy_(token)
+        self.x.copy_(self.model.embed[self.tok])
+        self.pos = max(self.pages._lengths)
+        # the accepted drafts are the path's nodes behind the root
+        place = torch.arange(1, n + 1, device=dev)
+        accepted = torch.gather(ids, 1, path[:, 1: n].clamp(min=0).long())
+        out = torch.cat([accepted, token[:, None]], dim=1)
+        out = torch.where(place == counts[:, None], token[:, None], torch.where(place < counts[:, None], out, -1))
+        return out, kept

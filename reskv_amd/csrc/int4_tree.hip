@@ -25,21 +25,22 @@ namespace {
 constexpr int kNodes = RESKV_DRAFT_NODES;
 constexpr int kWavesPerSimd = 2;
 constexpr int kMostWaves = 1024 * kWavesPerSimd;  // 256 CUs of 4 SIMDs
-constexpr float kWeightBits = 9.0f, kSlack = 6.0f;
+constexpr float kWeightBits = 8.0f, kSlack = 6.0f;
 constexpr int kTileRows = 16;
 
 // Work: a column is (sequence, KV head, chunk of rows), as many blocks of 32 tokens long as the sequence; the columns
-// lie one behind the other and every wave takes an equal run of blocks.  A column that lies in one run is written
-// out at once; of the others every wave leaves a record, of its first column at 2 wave, of its last at 2 wave + 1.
+// lie one behind the other and every workgroup takes an equal run of blocks.  A column that lies in one run is written
+// out at once; of the others every workgroup leaves a record, of its first column at 2 w, of its last at 2 w + 1.
 struct TreeArgs {
     Pool pool;
     const uint16_t* q;       // [N, Hq, 128]
     const int32_t *lengths, *offsets;
     const uint64_t* seen;    // [N] or null
     uint16_t* out;           // [N, Hq, 128]
-    float* part;             // [2 waves, rows, 128]: weighted values
-    float2* stat;            // [2 waves, rows]: reference of the weights, their sum
-    int S, N, Hq, G, waves, max_length, max_nodes, clear_rest;
+    float* part;             // [2 groups, rows, 128]: weighted values
+    float2* stat;            // [2 groups, rows]: reference of the weights, their sum
+    int S, N, Hq, G, groups, max_length, max_nodes, clear_rest;
+    int rows_of_chunk;
     float c;                 // scaling * log2(e)
 
     __device__ __forceinline__ int tokens(int s) const { return min(max(lengths[s], 0), max_length); }
@@ -48,61 +49,47 @@ struct TreeArgs {
         const Rows r = sequence_rows(offsets, s, N);
         return {r.first, min(r.count, max_nodes)};
     }
-    template <int ROWS>
-    __device__ __forceinline__ int chunks(int s) const { return (rows(s).count * G + ROWS - 1) / ROWS; }
-    template <int ROWS>
-    __device__ __forceinline__ int units(int s) const { return blocks(s) * chunks<ROWS>(s) * pool.heads; }
+    __device__ __forceinline__ int chunks(int s, int rows_each) const { return (rows(s).count * G + rows_each - 1) / rows_each; }
+    __device__ __forceinline__ int units(int s, int rows_each) const { return blocks(s) * chunks(s, rows_each) * pool.heads; }
 };
 
 // Units (blocks of columns) of the sequences before s, and of all.
 struct Sums {
     int before, all;
 };
-template <int ROWS>
-__device__ __forceinline__ Sums sum_units(const TreeArgs& A, int s) {
+__device__ __forceinline__ Sums sum_units(const TreeArgs& A, int s, int rows_each) {
     int before = 0, all = 0;
     for (int i = lane_id(); i < A.S; i += kWave) {
-        const int n = A.units<ROWS>(i);
+        const int n = A.units(i, rows_each);
         all += n;
         before += i < s ? n : 0;
     }
     return {wave_sum_int(before), wave_sum_int(all)};
 }
-__device__ __forceinline__ int run_length(const TreeArgs& A, int all) { return max((all + A.waves - 1) / A.waves, 1); }
+__device__ __forceinline__ int run_length(const TreeArgs& A, int all) { return max((all + A.groups - 1) / A.groups, 1); }
 
-// One block as a lane takes it.
-struct TreeBlock {
-    uint4 k[2];      // tokens token_of(j), channels 8 quarter + [0, 8) of the four groups
-    uint32_t ks[2];  // their scale and low of group `quarter`
-    uint4 v[2];      // channels 16 (4 i + j) + lane % 16 (dword j), tokens 8 quarter + [0, 8)
-    uint32_t vs, vl; // scales and lowest values of group lane / 16, tokens 2 (lane % 16) + [0, 2)
-};
 // Token of a lane's row in tile j of K: rows 4 q .. 4 q + 3 are the tokens 8 q + 4 j .. + 3.
 __device__ __forceinline__ int token_of(int n, int j) { return 8 * (n >> 2) + 4 * j + (n & 3); }
 
-__device__ __forceinline__ void load_block(TreeBlock& b, const char* p, int lane) {
-    const int n = lane & 15, quarter = lane >> 4;
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-        const int t = token_of(n, j);
-        b.k[j] = reinterpret_cast<const uint4*>(p)[(t >> 4) * 64 + quarter * 16 + (t & 15)];
-        b.ks[j] = reinterpret_cast<const uint32_t*>(p + kKScale)[((t >> 4) * 4 + quarter) * 16 + (t & 15)];
+// The masks of the nibbles, in vector registers: an and with an or takes one instruction then, which has no room for two
+// constants.
+struct Masks {
+    uint32_t low, high;
+    __device__ __forceinline__ Masks() : low(0x000F000Fu), high(0x00F000F0u) {
+        asm("" : "+v"(low));
+        asm("" : "+v"(high));
     }
-    b.v[0] = reinterpret_cast<const uint4*>(p + kVCodes)[lane];
-    b.v[1] = reinterpret_cast<const uint4*>(p + kVCodes)[64 + lane];
-    b.vs = reinterpret_cast<const uint32_t*>(p + kVScale)[lane];
-    b.vl = reinterpret_cast<const uint32_t*>(p + kVLow)[lane];
-}
+};
 
 // Eight values code * scale + low in fp16 of a dword of codes, `s` and `l` being the scales and lowest values of its
 // elements: the codes become 1024 + code, or 1024 + 16 code, by masking, and code exactly from that.
-__device__ __forceinline__ half8_t values_of(uint32_t d, const uint4& s, const uint4& l) {
+__device__ __forceinline__ half8_t values_of(const Masks& M, uint32_t d, const uint4& s, const uint4& l) {
     const half2_t sixteenth = {(_Float16)0.0625f, (_Float16)0.0625f}, back = {(_Float16)-64.0f, (_Float16)-64.0f};
     const half2_t base = {(_Float16)1024.0f, (_Float16)1024.0f};
     const uint32_t e = d >> 8, m = 0x64006400u;
-    const half2_t c0 = __builtin_bit_cast(half2_t, (d & 0x000F000Fu) | m) - base, c2 = __builtin_bit_cast(half2_t, (e & 0x000F000Fu) | m) - base;
-    const half2_t c1 = __builtin_elementwise_fma(__builtin_bit_cast(half2_t, (d & 0x00F000F0u) | m), sixteenth, back);
-    const half2_t c3 = __builtin_elementwise_fma(__builtin_bit_cast(half2_t, (e & 0x00F000F0u) | m), sixteenth, back);
+    const half2_t c0 = __builtin_bit_cast(half2_t, (d & M.low) | m) - base, c2 = __builtin_bit_cast(half2_t, (e & M.low) | m) - base;
+    const half2_t c1 = __builtin_elementwise_fma(__builtin_bit_cast(half2_t, (d & M.high) | m), sixteenth, back);
+    const half2_t c3 = __builtin_elementwise_fma(__builtin_bit_cast(half2_t, (e & M.high) | m), sixteenth, back);
     auto h = [](uint32_t w) __attribute__((always_inline)) { return __builtin_bit_cast(half2_t, w); };
     const half2_t r0 = __builtin_elementwise_fma(c0, h(s.x), h(l.x)), r1 = __builtin_elementwise_fma(c1, h(s.y), h(l.y));
     const half2_t r2 = __builtin_elementwise_fma(c2, h(s.z), h(l.z)), r3 = __builtin_elementwise_fma(c3, h(s.w), h(l.w));
@@ -117,163 +104,148 @@ __device__ __forceinline__ half8_t within_fp16(half8_t v) {
     return __builtin_elementwise_maximum(__builtin_elementwise_minimum(v, most), -most);
 }
 
+// Tokens t0 and t0 + 1 of a dword: the halves of those below `valid`.
+__device__ __forceinline__ uint32_t halves_below(int t0, int valid) { return (t0 < valid ? 0xFFFFu : 0u) | (t0 + 1 < valid ? 0xFFFF0000u : 0u); }
+// The larger of each of two numbers in a dword, not negative in fp16.
+__device__ __forceinline__ uint32_t pair_max(uint32_t a, uint32_t b) {
+    typedef unsigned short ushort2_t __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(ushort2_t, a), __builtin_bit_cast(ushort2_t, b)));
+}
+// Scales of 2^12 and more, NaN and infinity among them: values may pass fp16's largest.
+__device__ __forceinline__ bool is_odd(uint32_t scales) { return (scales & 0xFFFFu) >= 0x6C00u || scales >= 0x6C000000u; }
+
+// Two results in fp16; one past fp16's largest is that largest, as a value may be (a NaN goes on).
+__device__ __forceinline__ float within(float x) { return x > 65504.0f ? 65504.0f : x < -65504.0f ? -65504.0f : x; }
+__device__ __forceinline__ uint32_t pack_results(float a, float b) { return pack_halves(within(a), within(b)); }
+
+// What a wave needs of a column, and its rows' state.
 template <int RT>
-__device__ __forceinline__ void work_on_column(const TreeArgs& A, uint32_t* s_ks, uint32_t* s_vs, int s, int column, int begin,
-                                               int end, int record) {
-    constexpr int kRows = RT * kTileRows;
-    const int lane = threadIdx.x, n = lane & 15, quarter = lane >> 4;
-    const Rows rows = A.rows(s);
-    const int chunks = A.chunks<kRows>(s), hk = column / chunks, r0 = (column - hk * chunks) * kRows;
-    const int total_rows = rows.count * A.G, length = A.tokens(s), context = length - rows.count;
-
-    int entry0 = begin / A.pool.blocks, entry = 0, inside = begin - entry0 * A.pool.blocks, numbers = 0;
-    auto fetch_numbers = [&]() { numbers = A.pool.table[(long)s * A.pool.width + min(entry0 + lane, A.pool.width - 1)]; };
-    auto fetch = [&](TreeBlock& x) {
-        const char* p = A.pool.in_page(__builtin_amdgcn_readlane(numbers, entry), inside, hk);
-        load_block(x, p ? p : A.pool.pages, lane);
-        if (++inside == A.pool.blocks) {
-            inside = 0;
-            if (++entry == kWave) {
-                entry0 += kWave;
-                entry = 0;
-                fetch_numbers();
-            }
-        }
-        return p != nullptr;
-    };
-    TreeBlock x0, x1;
-    fetch_numbers();
-    bool there0 = fetch(x0);
-
-    // Q: lane (row n, quarter): channels 32 g + 8 quarter + [0, 8) of each group, brought to the row's own power of two so
-    // that the sixteenth of an element, which meets codes times 2^-20, keeps its bits
-    half8_t qf[RT][4];
-    float qs[RT], back[RT];  // sum of group `quarter`'s channels; what brings the row's scores back
+struct RowState {
+    half8_t q[RT][4];        // lane (row n, quarter): channels 32 g + 8 quarter + [0, 8) of each group
+    float sum[RT], back[RT]; // sum of group `quarter`'s channels; what brings the row's scores back
     uint64_t sees[RT];       // the row's nodes
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-        const int r = r0 + rt * kTileRows + n, node = r / A.G;
-        const bool real = r < total_rows;
-        const long row = (long)(rows.first + node) * A.Hq + hk * A.G + r - node * A.G;
-        float top = 0.0f, sum[4];
-        uint4 raw[4] = {};
-        if (real) {
-#pragma unroll
-            for (int g = 0; g < 4; ++g) raw[g] = reinterpret_cast<const uint4*>(A.q + row * kDim)[4 * g + quarter];
-        }
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            const uint32_t w[4] = {raw[g].x, raw[g].y, raw[g].z, raw[g].w};
-            sum[g] = 0.0f;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const float x = h2f((uint16_t)(w[e >> 1] >> (16 * (e & 1))));
-                top = fmaxf(top, fabsf(x));
-                sum[g] += x;
-            }
-        }
-        top = swap_max(top);
-        const float up = top > 0.0f && top < INFINITY ? ldexpf(1.0f, 14 - ilogbf(top)) : 1.0f;
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            const uint32_t w[4] = {raw[g].x, raw[g].y, raw[g].z, raw[g].w};
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-                qf[rt][g][e] = (_Float16)(h2f((uint16_t)(w[e >> 1] >> (16 * (e & 1)))) * (e & 2 ? up * 0.0625f : up));
-            sum[g] = swap_sum16(sum[g], sum[g]);
-            sum[g] = swap_sum32(sum[g], sum[g]);
-        }
-        qs[rt] = (quarter == 0 ? sum[0] : quarter == 1 ? sum[1] : quarter == 2 ? sum[2] : sum[3]) * (up * 0x1p-24f);
-        back[rt] = A.c * (0x1p24f / up);
+    float4_t acc[RT][8];     // channels 16 ct + 4 quarter + i of row n
+    float m[RT], l[RT];      // reference of the row's weights, this lane's share of their sum
+
+    // Rows r0 .. of the sequence and KV head.  Each is brought to its own power of two, so that the sixteenth of an element,
+    // which meets codes times 2^-20, keeps its bits.
+    __device__ __forceinline__ void start(const TreeArgs& A, const Rows& rows, int hk, int r0, int lane) {
+        const int n = lane & 15, quarter = lane >> 4, total = rows.count * A.G;
         const uint64_t all = rows.count < 64 ? (1ull << rows.count) - 1 : ~0ull;
-        sees[rt] = !real ? 0 : (A.seen ? A.seen[rows.first + node] : (2ull << node) - 1) & all;
-    }
-
-    float4_t acc[RT][8];  // channels 16 ct + 4 quarter + i of row n
-    float m[RT], l[RT];   // reference of the row's weights, this lane's share of their sum
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-        m[rt] = -__FLT_MAX__;
-        l[rt] = 0.0f;
+        for (int rt = 0; rt < RT; ++rt) {
+            const int r = r0 + rt * kTileRows + n, node = r / A.G;
+            const bool real = r < total;
+            const long row = (long)(rows.first + node) * A.Hq + hk * A.G + r - node * A.G;
+            float top = 0.0f, part[4];
+            uint4 raw[4] = {};
+            if (real) {
 #pragma unroll
-        for (int ct = 0; ct < 8; ++ct) acc[rt][ct] = {0.0f, 0.0f, 0.0f, 0.0f};
-    }
-
-    auto work = [&](TreeBlock& x, int blk, bool there) __attribute__((always_inline)) {
-        if (!there) return;  // its tokens are not there
-        const int valid = min(kBlock, length - blk * kBlock), tree = context - blk * kBlock;  // tokens; where the nodes begin
-        const bool edge = tree < kBlock;  // some tokens are nodes, or none
-        if (valid < kBlock) {  // what lies behind the last token may be anything
-            const int t = 2 * n;
-            const uint32_t keep = (t < valid ? 0xFFFFu : 0u) | (t + 1 < valid ? 0xFFFF0000u : 0u);
-            x.vs &= keep;
-            x.vl &= keep;
-        }
-        // Scales of 2^12 and more, NaN and infinity among them: values may pass fp16's largest
-        const bool odd = ballot((x.vs & 0xFFFFu) >= 0x6C00u || x.vs >= 0x6C000000u) != 0;
-        uint64_t bad0 = 0, bad1 = 0;  // nodes (even and odd tokens, 16 a group) whose values are no numbers
-        if (odd && edge) {
-            const int t = 2 * n;
-            const bool b0 = t >= tree && (x.vs & 0xFFFFu) >= 0x7C00u, b1 = t + 1 >= tree && x.vs >= 0x7C000000u;
-            bad0 = ballot(b0);
-            bad1 = ballot(b1);
-            const uint32_t keep = (b0 ? 0u : 0xFFFFu) | (b1 ? 0u : 0xFFFF0000u);
-            x.vs &= keep;  // zeros to the rows that do not see them, added apart to the others
-            x.vl &= keep;
-        }
+                for (int g = 0; g < 4; ++g) raw[g] = reinterpret_cast<const uint4*>(A.q + row * kDim)[4 * g + quarter];
+            }
 #pragma unroll
-        for (int j = 0; j < 2; ++j) s_ks[quarter * kBlock + token_of(n, j)] = x.ks[j];
-        s_vs[lane] = x.vs;
-        s_vs[64 + lane] = x.vl;
-        wave_sync();
-
-        float4_t score[RT][2];
+            for (int g = 0; g < 4; ++g) {
+                const uint32_t w[4] = {raw[g].x, raw[g].y, raw[g].z, raw[g].w};
+                part[g] = 0.0f;
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            const float low = h2f((uint16_t)(x.ks[j] >> 16));
-#pragma unroll
-            for (int rt = 0; rt < RT; ++rt)
-                score[rt][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(low, qs[rt], float4_t{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
-        }
-#pragma unroll
-        for (int g = 0; g < 4; ++g)
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                const uint32_t kd = g == 0 ? x.k[j].x : g == 1 ? x.k[j].y : g == 2 ? x.k[j].z : x.k[j].w;
-                const half8_t kf = operand(kd);
-                const uint4 sc = *reinterpret_cast<const uint4*>(&s_ks[g * kBlock + 8 * quarter + 4 * j]);
-                const uint32_t w[4] = {sc.x, sc.y, sc.z, sc.w};
-#pragma unroll
-                for (int rt = 0; rt < RT; ++rt) {
-                    const float4_t d = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[rt][g], float4_t{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) score[rt][j][i] = __builtin_fmaf(d[i], h2f((uint16_t)w[i]), score[rt][j][i]);
+                for (int e = 0; e < 8; ++e) {
+                    const float x = h2f((uint16_t)(w[e >> 1] >> (16 * (e & 1))));
+                    top = fmaxf(top, fabsf(x));
+                    part[g] += x;
                 }
             }
-
-        uint32_t sees_block[RT];
-        if (edge || valid < kBlock) {
+            top = swap_max(top);
+            const float up = top > 0.0f && top < INFINITY ? ldexpf(1.0f, 14 - ilogbf(top)) : 1.0f;
 #pragma unroll
-            for (int rt = 0; rt < RT; ++rt) {
-                uint32_t bits = tree <= 0 ? (tree > -64 ? (uint32_t)(sees[rt] >> -tree) : 0u)
-                                          : tree < kBlock ? (uint32_t)(sees[rt] << tree) | ((1u << tree) - 1u) : ~0u;
-                if (valid < kBlock) bits &= (1u << valid) - 1u;
-                sees_block[rt] = bits;
-                const uint32_t mine = bits >> (8 * quarter);
+            for (int g = 0; g < 4; ++g) {
+                const uint32_t w[4] = {raw[g].x, raw[g].y, raw[g].z, raw[g].w};
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    q[rt][g][e] = (_Float16)(h2f((uint16_t)(w[e >> 1] >> (16 * (e & 1)))) * (e & 2 ? up * 0.0625f : up));
+                part[g] = swap_sum16(part[g], part[g]);
+                part[g] = swap_sum32(part[g], part[g]);
+            }
+            sum[rt] = (quarter == 0 ? part[0] : quarter == 1 ? part[1] : quarter == 2 ? part[2] : part[3]) * (up * 0x1p-24f);
+            back[rt] = A.c * (0x1p24f / up);
+            sees[rt] = !real ? 0 : (A.seen ? A.seen[rows.first + node] : (2ull << node) - 1) & all;
+            m[rt] = -__FLT_MAX__;
+            l[rt] = 0.0f;
+#pragma unroll
+            for (int ct = 0; ct < 8; ++ct) acc[rt][ct] = {0.0f, 0.0f, 0.0f, 0.0f};
+        }
+    }
+
+    // The weights of NB blocks, as operands.  key(b, j, g): the K operand of tile j and group g of block b; scale(b, g): the
+    // scales of the tokens 8 quarter .. + 7; low(b, j): the lowest value of the lane's K row and group.  Of block b valid[b] tokens
+    // are there, from tree[b] on they are nodes; `visible` gets the tokens that a row sees where some do not.
+    template <int NB, bool SHARED, class Key, class Scale, class Low, class Before, class Between>
+    __device__ __forceinline__ void weights(half8_t (*p)[RT], uint32_t (*visible)[RT], const int* valid, const int* tree, int quarter, Key key,
+                                            Scale scale, Low low, Before before_softmax, Between between) {
+        float4_t score[NB][RT][2];
+        const float4_t zero = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            if (SHARED) __builtin_amdgcn_s_setprio(1);
+            float lows[2];
+            half8_t scales[4], keys[4][2];
+            auto read = [&](int g) __attribute__((always_inline)) {
+#pragma unroll
+                for (int j = 0; j < 2; ++j) keys[g][j] = key(b, j, g);
+                scales[g] = __builtin_bit_cast(half8_t, scale(b, g));
+            };
+#pragma unroll
+            for (int j = 0; j < 2; ++j) lows[j] = low(b, j);
+            read(0);
+            read(1);
+            float4_t d[2][2][RT];
+            auto multiply = [&](int g, int j, int rt) __attribute__((always_inline)) {
+                d[g & 1][j][rt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(keys[g][j], q[rt][g], zero, 0, 0, 0);
+            };
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt) multiply(0, j, rt);
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                if (g < 2) read(g + 2);
 #pragma unroll
                 for (int j = 0; j < 2; ++j)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        if (!((mine >> (4 * j + i)) & 1u)) score[rt][j][i] = -INFINITY;
+                    for (int rt = 0; rt < RT; ++rt) {
+                        if (g < 3) multiply(g + 1, j, rt);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const float x = d[g & 1][j][rt][i], sc = (float)scales[g][4 * j + i];
+                            score[b][rt][j][i] = __builtin_fmaf(x, sc, g == 0 ? 0.0f : score[b][rt][j][i]);  // one instruction
+                        }
+                        if (g == 3) score[b][rt][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(lows[j], sum[rt], score[b][rt][j], 0, 0, 0);
+                    }
             }
         }
+        if (SHARED) __builtin_amdgcn_s_setprio(0);
+        before_softmax();
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+            if (tree[b] < kBlock || valid[b] < kBlock) {
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt) {
+                    uint32_t bits = tree[b] <= 0 ? (tree[b] > -64 ? (uint32_t)(sees[rt] >> -tree[b]) : 0u)
+                                                 : tree[b] < kBlock ? (uint32_t)(sees[rt] << tree[b]) | ((1u << tree[b]) - 1u) : ~0u;
+                    if (valid[b] < kBlock) bits &= (1u << valid[b]) - 1u;
+                    visible[b][rt] = bits;
+                    const uint32_t mine = bits >> (8 * quarter);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        if (!((mine >> e) & 1u)) score[b][rt][e >> 2][e & 3] = -INFINITY;
+                }
+            }
         bool grow = false;
         float top[RT];
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
-            top[rt] = score[rt][0][0];
+            top[rt] = score[0][rt][0][0];
 #pragma unroll
-            for (int i = 1; i < 8; ++i) top[rt] = fmaxf(top[rt], score[rt][i >> 2][i & 3]);
+            for (int i = 1; i < 8 * NB; ++i) top[rt] = fmaxf(top[rt], score[i >> 3][rt][i >> 2 & 1][i & 3]);
             top[rt] *= back[rt];
             grow |= top[rt] > m[rt] + kSlack;
         }
@@ -289,93 +261,416 @@ __device__ __forceinline__ void work_on_column(const TreeArgs& A, uint32_t* s_ks
                     for (int i = 0; i < 4; ++i) acc[rt][ct][i] *= alpha;
             }
         }
-        half8_t p[RT];
         const half2_t ones = {(_Float16)1.0f, (_Float16)1.0f};
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-            const float shift = kWeightBits - m[rt];
-            float sum = 0.0f;
+        for (int b = 0; b < NB; ++b)
 #pragma unroll
-            for (int e = 0; e < 8; e += 2) {
-                const half2_t w = {(_Float16)__builtin_amdgcn_exp2f(__builtin_fmaf(score[rt][e >> 2][e & 3], back[rt], shift)),
-                                   (_Float16)__builtin_amdgcn_exp2f(__builtin_fmaf(score[rt][e >> 2][(e & 3) + 1], back[rt], shift))};
-                sum = __builtin_amdgcn_fdot2(w, ones, sum, false);
-                p[rt][e] = w[0];
-                p[rt][e + 1] = w[1];
+            for (int rt = 0; rt < RT; ++rt) {
+                const float shift = kWeightBits - m[rt];
+                float total = 0.0f;
+#pragma unroll
+                for (int e = 0; e < 8; e += 2) {
+                    if (rt > 0) between(b, rt - 1, e >> 1);
+                    const half2_t w = {(_Float16)__builtin_amdgcn_exp2f(__builtin_fmaf(score[b][rt][e >> 2][e & 3], back[rt], shift)),
+                                       (_Float16)__builtin_amdgcn_exp2f(__builtin_fmaf(score[b][rt][e >> 2][(e & 3) + 1], back[rt], shift))};
+                    total = __builtin_amdgcn_fdot2(w, ones, total, false);
+                    p[b][rt][e] = w[0];
+                    p[b][rt][e + 1] = w[1];
+                }
+                l[rt] += total;
             }
-            l[rt] += sum;
-        }
-#pragma unroll
-        for (int ct = 0; ct < 8; ++ct) {
-            const uint4 sc = *reinterpret_cast<const uint4*>(&s_vs[(ct >> 1) * 16 + 4 * quarter]);
-            const uint4 lo = *reinterpret_cast<const uint4*>(&s_vs[64 + (ct >> 1) * 16 + 4 * quarter]);
-            const uint4& codes = x.v[ct >> 2];
-            const int at = ct & 3;
-            half8_t v = values_of(at == 0 ? codes.x : at == 1 ? codes.y : at == 2 ? codes.z : codes.w, sc, lo);
-            if (odd) v = within_fp16(v);
-#pragma unroll
-            for (int rt = 0; rt < RT; ++rt) acc[rt][ct] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, p[rt], acc[rt][ct], 0, 0, 0);
-        }
-        if ((bad0 | bad1) != 0) {  // rare: the rows that see such a node get its NaN, in the channels of its group
-#pragma unroll
-            for (int rt = 0; rt < RT; ++rt)
-                for (int t = 0; t < kBlock; ++t)
-#pragma unroll
-                    for (int g = 0; g < 4; ++g)
-                        if (((t & 1 ? bad1 : bad0) >> (16 * g + (t >> 1))) & 1u && (sees_block[rt] >> t) & 1u)
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) acc[rt][2 * g][i] = acc[rt][2 * g + 1][i] = __builtin_nanf("");
-        }
-        wave_sync();
-    };
-    bool there1 = false;
-    for (int blk = begin; blk < end; blk += 2) {
-        if (blk + 1 < end) there1 = fetch(x1);
-        work(x0, blk, there0);
-        if (blk + 1 >= end) break;
-        if (blk + 2 < end) there0 = fetch(x0);
-        work(x1, blk + 1, there1);
     }
 
+    // A value tile times the weights.
+    __device__ __forceinline__ void add(int ct, half8_t v, const half8_t* p) {
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-        float total = swap_sum16(l[rt], l[rt]);
-        total = swap_sum32(total, total);
-        const int at = rt * kTileRows + n, r = r0 + at, node = r / A.G;
-        if (r >= total_rows) continue;
-        if (record >= 0) {
-            const long rec = (long)record * kRows + at;
-            if (quarter == 0) A.stat[rec] = make_float2(m[rt], total);
-            float4_t* const dst = reinterpret_cast<float4_t*>(A.part + rec * kDim) + quarter;
+        for (int rt = 0; rt < RT; ++rt) acc[rt][ct] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, p[rt], acc[rt][ct], 0, 0, 0);
+    }
+
+    __device__ __forceinline__ void add_one(int ct, int rt, half8_t v, const half8_t* p) {
+        acc[rt][ct] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, p[rt], acc[rt][ct], 0, 0, 0);
+    }
+
+    // Rare: nodes whose values are no numbers (bad(g): the tokens of group g) were taken as zeros; the rows that see such a node
+    // get its NaN, in the channels of its group.
+    template <class Bad>
+    __device__ __forceinline__ void add_bad(const uint32_t* visible, Bad bad) {
 #pragma unroll
-            for (int ct = 0; ct < 8; ++ct) dst[4 * ct] = acc[rt][ct];
-        } else {
-            const float inv = total == 0.0f ? 0.0f : 1.0f / total;
-            uint2* const dst = reinterpret_cast<uint2*>(A.out + ((long)(rows.first + node) * A.Hq + hk * A.G + r - node * A.G) * kDim) + quarter;
+        for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-            for (int ct = 0; ct < 8; ++ct)
-                dst[4 * ct] = make_uint2(pack_halves(acc[rt][ct][0] * inv, acc[rt][ct][1] * inv), pack_halves(acc[rt][ct][2] * inv, acc[rt][ct][3] * inv));
+            for (int g = 0; g < 4; ++g)
+                if (visible[rt] & bad(g))
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) acc[rt][2 * g][i] = acc[rt][2 * g + 1][i] = __builtin_nanf("");
+    }
+
+    // Rows r0 .. of the chunk, to their record (of `chunk` rows) or out.
+    __device__ __forceinline__ void finish(const TreeArgs& A, const Rows& rows, int hk, int r0, int in_chunk, int chunk, int record, int lane) {
+        const int n = lane & 15, quarter = lane >> 4, all = rows.count * A.G;
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+            float total = swap_sum16(l[rt], l[rt]);
+            total = swap_sum32(total, total);
+            const int at = in_chunk + rt * kTileRows + n, r = r0 + rt * kTileRows + n, node = r / A.G;
+            if (r >= all) continue;
+            if (record >= 0) {
+                const long rec = (long)record * chunk + at;
+                if (quarter == 0) A.stat[rec] = make_float2(m[rt], total);
+                float4_t* const dst = reinterpret_cast<float4_t*>(A.part + rec * kDim) + quarter;
+#pragma unroll
+                for (int ct = 0; ct < 8; ++ct) dst[4 * ct] = acc[rt][ct];
+            } else {
+                const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+                uint2* const dst = reinterpret_cast<uint2*>(A.out + ((long)(rows.first + node) * A.Hq + hk * A.G + r - node * A.G) * kDim) + quarter;
+#pragma unroll
+                for (int ct = 0; ct < 8; ++ct)
+                    dst[4 * ct] = make_uint2(pack_results(acc[rt][ct][0] * inv, acc[rt][ct][1] * inv), pack_results(acc[rt][ct][2] * inv, acc[rt][ct][3] * inv));
+            }
         }
     }
+};
+
+// The blocks of a column one after the other: where they lie.  Page numbers come 64 at a time, one per lane, and a page's
+// address is worked out once.
+struct Walk {
+    int entry0, entry, inside, numbers;
+    bool there;
+    const char* at;  // the next block, where there is one
+    __device__ __forceinline__ void fetch(const TreeArgs& A, int s, int lane) {
+        numbers = A.pool.table[(long)s * A.pool.width + min(entry0 + lane, A.pool.width - 1)];
+    }
+    __device__ __forceinline__ void page(const TreeArgs& A, int hk) {
+        const char* const p = A.pool.in_page(__builtin_amdgcn_readlane(numbers, entry), inside, hk);
+        there = p != nullptr;
+        at = there ? p : A.pool.pages;
+    }
+    __device__ __forceinline__ void start(const TreeArgs& A, int s, int hk, int begin, int lane) {
+        entry0 = begin / A.pool.blocks;
+        entry = 0;
+        inside = begin - entry0 * A.pool.blocks;
+        fetch(A, s, lane);
+        page(A, hk);
+    }
+    __device__ __forceinline__ void next(const TreeArgs& A, int s, int hk, int lane) {
+        if (++inside < A.pool.blocks) {
+            if (there) at += kBlockBytes;
+            return;
+        }
+        inside = 0;
+        if (++entry == kWave) {
+            entry0 += kWave;
+            entry = 0;
+            fetch(A, s, lane);
+        }
+        page(A, hk);
+    }
+};
+
+// Loads of a block whose address is the same for all lanes: a lane has its offset, so that no address is worked out.
+struct BlockLoads {
+    __amdgpu_buffer_rsrc_t block;
+    __device__ __forceinline__ explicit BlockLoads(const char* p)
+        : block(__builtin_amdgcn_make_buffer_rsrc((void*)p, 0, kBlockBytes, 0x00020000)) {}
+    __device__ __forceinline__ uint4 b128(int lane, int at) const {
+        return __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(block, lane, at, 0));
+    }
+    __device__ __forceinline__ uint2 b64(int lane, int at) const {
+        return __builtin_bit_cast(uint2, __builtin_amdgcn_raw_buffer_load_b64(block, lane, at, 0));
+    }
+    __device__ __forceinline__ uint32_t b32(int lane, int at) const { return __builtin_amdgcn_raw_buffer_load_b32(block, lane, at, 0); }
+};
+
+// ---------------------------------------------------------------------------
+// few rows: a wave by itself
+// ---------------------------------------------------------------------------
+
+// One block as a lane takes it.
+struct TreeBlock {
+    uint4 k[2];      // tokens token_of(j), channels 8 quarter + [0, 8) of the four groups
+    uint32_t ks[2];  // their scale and low of group `quarter`
+    uint4 v[2];      // channels 16 (4 i + j) + lane % 16 (dword j), tokens 8 quarter + [0, 8)
+    uint32_t vs, vl; // scales and lowest values of group lane / 16, tokens 2 (lane % 16) + [0, 2)
+};
+__device__ __forceinline__ void load_block(TreeBlock& b, const char* p, int lane) {
+    const int n = lane & 15, quarter = lane >> 4;
+    const BlockLoads L(p);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        const int t = token_of(n, j);
+        b.k[j] = L.b128(16 * ((t >> 4) * 64 + quarter * 16 + (t & 15)), 0);
+        b.ks[j] = L.b32(4 * (((t >> 4) * 4 + quarter) * 16 + (t & 15)), kKScale);
+    }
+    b.v[0] = L.b128(16 * lane, kVCodes);
+    b.v[1] = L.b128(16 * lane, kVCodes + 1024);
+    b.vs = L.b32(4 * lane, kVScale);
+    b.vl = L.b32(4 * lane, kVLow);
+}
+__device__ __forceinline__ uint32_t dword(const uint4& x, int i) { return i == 0 ? x.x : i == 1 ? x.y : i == 2 ? x.z : x.w; }
+
+struct OneWave {  // LDS
+    alignas(16) uint16_t scale[4 * kBlock];
+    alignas(16) uint32_t vs[64], vl[64];
+};
+
+template <int RT>
+__device__ __forceinline__ void work_alone(const TreeArgs& A, OneWave& L, int s, int column, int begin, int end, int record) {
+    constexpr int kRows = RT * kTileRows;
+    const int lane = threadIdx.x, n = lane & 15, quarter = lane >> 4;
+    const Rows rows = A.rows(s);
+    const int chunks = A.chunks(s, kRows), hk = column / chunks, r0 = (column - hk * chunks) * kRows;
+    const int length = A.tokens(s), context = length - rows.count;
+    Walk at;
+    at.start(A, s, hk, begin, lane);
+    TreeBlock x0, x1;
+    // Block blk; behind the last one it is loaded again: a branch around the loads would have every wait for one of them wait for
+    // the next block's as well.
+    auto fetch = [&](TreeBlock& x, int blk) __attribute__((always_inline)) {
+        const bool there = at.there;
+        load_block(x, at.at, lane);
+        if (blk + 1 < end) at.next(A, s, hk, lane);
+        return there;
+    };
+    bool there0 = fetch(x0, begin), there1;  // before Q, so that the first block does not wait for it
+    RowState<RT> R;
+    R.start(A, rows, hk, r0, lane);
+    const Masks M;
+
+    auto work = [&](TreeBlock& x, int blk, bool there) __attribute__((always_inline)) {
+        // the two waves of a SIMD go first in turns: the older one would end long before the other, which is then alone
+        if ((blk ^ (int)blockIdx.x ^ ((int)blockIdx.x >> 10)) & 2) __builtin_amdgcn_s_setprio(1);
+        else __builtin_amdgcn_s_setprio(0);
+        if (!there) return;  // its tokens are not there
+        const int valid = min(kBlock, length - blk * kBlock), tree = context - blk * kBlock;  // tokens; where the nodes begin
+        if (valid < kBlock) {  // what lies behind the last token may be anything
+            const uint32_t keep = halves_below(2 * n, valid);
+            x.vs &= keep;
+            x.vl &= keep;
+        }
+        const bool odd = ballot(is_odd(x.vs)) != 0;
+        uint64_t bad0 = 0, bad1 = 0;  // nodes (even and odd tokens, 16 a group) whose values are no numbers
+        if (odd && tree < kBlock) {
+            const bool b0 = 2 * n >= tree && (x.vs & 0xFFFFu) >= 0x7C00u, b1 = 2 * n + 1 >= tree && x.vs >= 0x7C000000u;
+            bad0 = ballot(b0);
+            bad1 = ballot(b1);
+            const uint32_t keep = (b0 ? 0u : 0xFFFFu) | (b1 ? 0u : 0xFFFF0000u);
+            x.vs &= keep;
+            x.vl &= keep;
+        }
+        if (odd) {  // half of the values then, for twice the weights
+            const half2_t half = {(_Float16)0.5f, (_Float16)0.5f};
+            x.vs = __builtin_bit_cast(uint32_t, __builtin_bit_cast(half2_t, x.vs) * half);
+            x.vl = __builtin_bit_cast(uint32_t, __builtin_bit_cast(half2_t, x.vl) * half);
+        }
+#pragma unroll
+        for (int j = 0; j < 2; ++j) L.scale[quarter * kBlock + token_of(n, j)] = (uint16_t)x.ks[j];
+        L.vs[lane] = x.vs;
+        L.vl[lane] = x.vl;
+        wave_sync();
+        half8_t p[1][RT];
+        uint32_t visible[1][RT];
+        R.template weights<1, false>(p, visible, &valid, &tree, quarter,
+                              [&](int, int j, int g) __attribute__((always_inline)) { return operand(dword(x.k[j], g)); },
+                              [&](int, int g) __attribute__((always_inline)) { return reinterpret_cast<const uint4*>(L.scale)[4 * g + quarter]; },
+                              [&](int, int j) __attribute__((always_inline)) { return h2f((uint16_t)(x.ks[j] >> 16)); }, []() {}, [](int, int, int) {});
+        auto value = [&](int ct) __attribute__((always_inline)) {
+            const int of = 4 * (ct >> 1) + quarter;
+            return values_of(M, dword(x.v[ct >> 2], ct & 3), reinterpret_cast<const uint4*>(L.vs)[of], reinterpret_cast<const uint4*>(L.vl)[of]);
+        };
+        if (odd) {
+            const _Float16 two = (_Float16)2.0f;
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) p[0][rt] *= half8_t{two, two, two, two, two, two, two, two};
+        }
+#pragma unroll
+        for (int ct = 0; ct < 8; ++ct) R.add(ct, value(ct), p[0]);
+        if ((bad0 | bad1) != 0)
+            R.add_bad(visible[0], [&](int g) {
+                uint32_t bits = 0;
+                for (int t = 0; t < kBlock; ++t) bits |= (uint32_t)((t & 1 ? bad1 : bad0) >> (16 * g + (t >> 1)) & 1u) << t;
+                return bits;
+            });
+        wave_sync();
+    };
+    for (int blk = begin; blk < end; blk += 2) {
+        there1 = fetch(x1, blk + 1);
+        work(x0, blk, there0);
+        if (blk + 1 >= end) break;
+        there0 = fetch(x0, blk + 2);
+        work(x1, blk + 1, there1);
+    }
+    R.finish(A, rows, hk, r0, 0, kRows, record, lane);
     wave_sync();
 }
 
-template <int RT>
-__global__ void __launch_bounds__(kWave, kWavesPerSimd) tree_kernel(TreeArgs A) {
-    constexpr int kRows = RT * kTileRows;
-    __shared__ __align__(16) uint32_t s_ks[4 * kBlock], s_vs[128];
-    const int all = sum_units<kRows>(A, 0).all, run = run_length(A, all);
-    const int wave = blockIdx.x, start = wave * run;
+// ---------------------------------------------------------------------------
+// more rows: waves that share a block's operands
+// ---------------------------------------------------------------------------
+
+// A block as operands in the LDS: the codes of K as fp16 numbers, its scales and lowest values, and V in fp16.
+struct Operands {
+    uint4 k[2][4][kWave], v[8][kWave];
+    alignas(16) uint16_t scale[4 * kBlock];
+    float low[4 * kBlock];
+    uint32_t bad[4];  // tokens of a group whose values are no numbers, where nodes are
+};
+
+// A wave's share of that work: pieces of K and V.
+struct Share {
+    uint2 k;         // task t: tokens token_of(t / 2), groups 2 (t % 2) and the next
+    uint32_t ks;     // scale and low of token `lane` of group t
+    uint2 v;         // task t: channels 32 t + lane % 16 and 16 further on, tokens 8 quarter + [0, 8)
+    uint4 vs, vl;    // their scales and lowest values
+};
+
+// WAVES waves of 32 rows each take NB blocks per step; the blocks' four tasks each are shared out among the waves.  A block that
+// is not there counts as one without tokens.
+template <int WAVES, int NB>
+__device__ __forceinline__ void work_together(const TreeArgs& A, Operands (*L)[NB], int s, int column, int begin, int end, int record) {
+    constexpr int RT = 2, kWaveRows = RT * kTileRows, kRows = WAVES * kWaveRows, kItems = 4 * NB / WAVES;
+    const int lane = threadIdx.x & 63, n = lane & 15, quarter = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const Rows rows = A.rows(s);
+    const int chunks = A.chunks(s, kRows), hk = column / chunks, r0 = (column - hk * chunks) * kRows + wave * kWaveRows;
+    const int length = A.tokens(s), context = length - rows.count;
+    const bool active = r0 < rows.count * A.G;
+    Walk at;
+    at.start(A, s, hk, begin, lane);
+    Share x[kItems];
+    // the wave's shares of the blocks blk .. blk + NB - 1; which of them are there, as bits
+    auto fetch = [&](int blk) __attribute__((always_inline)) {
+        const char* found[NB];
+        uint32_t there = 0;
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            there |= (uint32_t)(at.there && blk + b < end) << b;
+            found[b] = at.at;
+            if (blk + b + 1 < end) at.next(A, s, hk, lane);
+        }
+#pragma unroll
+        for (int i = 0; i < kItems; ++i) {
+            const int item = wave + i * WAVES, task = item & 3, t = token_of(n, task >> 1), u = lane & 31;
+            const char* const p = NB == 1 || item < 4 ? found[0] : found[NB - 1];
+            const BlockLoads P(p);
+            x[i].k = P.b64(16 * ((t >> 4) * 64 + quarter * 16 + (t & 15)) + 8 * (task & 1), 0);
+            x[i].ks = P.b32(4 * (((u >> 4) * 4 + task) * 16 + (u & 15)), kKScale);
+            x[i].v = P.b64(16 * ((task >> 1) * 64 + lane) + 8 * (task & 1), kVCodes);
+            x[i].vs = P.b128(16 * (task * 4 + quarter), kVScale);
+            x[i].vl = P.b128(16 * (task * 4 + quarter), kVLow);
+        }
+        return there;
+    };
+    auto valid_of = [&](int blk, bool there) { return there ? min(kBlock, length - blk * kBlock) : 0; };
+    const Masks M;
+    auto stage = [&](Operands* O0, int blk0, uint32_t there) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < kItems; ++i) {
+            const int item = wave + i * WAVES, task = item & 3, b = item >> 2;
+            Operands& O = O0[b];
+            const int valid = valid_of(blk0 + b, there >> b & 1), tree = context - (blk0 + b) * kBlock;
+            O.k[task >> 1][2 * (task & 1)][lane] = __builtin_bit_cast(uint4, operand(x[i].k.x));
+            O.k[task >> 1][2 * (task & 1) + 1][lane] = __builtin_bit_cast(uint4, operand(x[i].k.y));
+            if (lane < kBlock) {
+                O.scale[task * kBlock + lane] = (uint16_t)x[i].ks;
+                O.low[task * kBlock + lane] = h2f((uint16_t)(x[i].ks >> 16));
+            }
+            uint32_t sc[4] = {x[i].vs.x, x[i].vs.y, x[i].vs.z, x[i].vs.w}, lo[4] = {x[i].vl.x, x[i].vl.y, x[i].vl.z, x[i].vl.w};
+            if (valid < kBlock) {  // what lies behind the last token may be anything
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const uint32_t keep = halves_below(8 * quarter + 2 * e, valid);
+                    sc[e] &= keep;
+                    lo[e] &= keep;
+                }
+            }
+            const bool odd = ballot(is_odd(pair_max(pair_max(sc[0], sc[1]), pair_max(sc[2], sc[3])))) != 0;
+            if (tree < kBlock) {
+                uint32_t bits = 0;  // of the lane's eight tokens
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int t = 8 * quarter + 2 * e;
+                    const bool b0 = t >= tree && (sc[e] & 0xFFFFu) >= 0x7C00u, b1 = t + 1 >= tree && sc[e] >= 0x7C000000u;
+                    bits |= (uint32_t)b0 << (2 * e) | (uint32_t)b1 << (2 * e + 1);
+                    const uint32_t keep = (b0 ? 0u : 0xFFFFu) | (b1 ? 0u : 0xFFFF0000u);
+                    sc[e] &= keep;
+                    lo[e] &= keep;
+                }
+                uint32_t all = 0;
+#pragma unroll
+                for (int q = 0; q < 4; ++q) all |= (uint32_t)__builtin_amdgcn_readlane((int)bits, 16 * q) << (8 * q);
+                if (lane == 0) O.bad[task] = all;
+            }
+            const uint4 s4 = make_uint4(sc[0], sc[1], sc[2], sc[3]), l4 = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+            half8_t v0 = values_of(M, x[i].v.x, s4, l4), v1 = values_of(M, x[i].v.y, s4, l4);
+            if (odd) {
+                v0 = within_fp16(v0);
+                v1 = within_fp16(v1);
+            }
+            O.v[2 * task][lane] = __builtin_bit_cast(uint4, v0);
+            O.v[2 * task + 1][lane] = __builtin_bit_cast(uint4, v1);
+        }
+    };
+    uint32_t there = fetch(begin), there_next = 0;
+    RowState<RT> R;
+    R.start(A, rows, hk, r0, lane);
+    stage(L[0], begin, there);
+    if (begin + NB < end) there_next = fetch(begin + NB);
+    __syncthreads();
+    int side = 0;
+    for (int blk = begin; blk < end; blk += NB) {
+        const Operands* const O = L[side];
+        side ^= 1;
+        const uint32_t here = there;
+        if (blk + NB < end) stage(L[side], blk + NB, there_next);
+        there = there_next;
+        if (blk + 2 * NB < end) there_next = fetch(blk + 2 * NB);
+        if (here && active) {
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                if (!(here >> b & 1)) continue;
+                const Operands& B = O[b];
+                const int valid = valid_of(blk + b, true), tree = context - (blk + b) * kBlock;
+                half8_t p[1][RT];
+                uint32_t visible[1][RT];
+                half8_t v[8];
+                R.template weights<1, true>(
+                    p, visible, &valid, &tree, quarter,
+                    [&](int, int j, int g) __attribute__((always_inline)) { return __builtin_bit_cast(half8_t, B.k[j][g][lane]); },
+                    [&](int, int g) __attribute__((always_inline)) { return reinterpret_cast<const uint4*>(B.scale)[4 * g + quarter]; },
+                    [&](int, int j) __attribute__((always_inline)) { return B.low[quarter * kBlock + token_of(n, j)]; },
+                    [&]() __attribute__((always_inline)) {  // on their way during the softmax
+#pragma unroll
+                        for (int ct = 0; ct < 8; ++ct) v[ct] = __builtin_bit_cast(half8_t, B.v[ct][lane]);
+                    },
+                    [&](int, int rt, int i) __attribute__((always_inline)) {  // the row tile's products between the next one's weights
+                        R.add_one(2 * i, rt, v[2 * i], p[0]);
+                        R.add_one(2 * i + 1, rt, v[2 * i + 1], p[0]);
+                    });
+#pragma unroll
+                for (int ct = 0; ct < 8; ++ct) { if (ct == 0) __builtin_amdgcn_s_setprio(1); R.add_one(ct, RT - 1, v[ct], p[0]); if (ct == 7) __builtin_amdgcn_s_setprio(0); }
+                if (tree < kBlock && (B.bad[0] | B.bad[1] | B.bad[2] | B.bad[3]) != 0)
+                    R.add_bad(visible[0], [&](int g) __attribute__((always_inline)) { return B.bad[g]; });
+            }
+        }
+        __syncthreads();
+    }
+    if (active) R.finish(A, rows, hk, r0, wave * kWaveRows, kRows, record, lane);
+}
+
+// A workgroup's run of blocks, column by column: work(sequence, column, first and last block, record or -1).
+template <class Work>
+__device__ __forceinline__ void run_of(const TreeArgs& A, int rows_each, Work work) {
+    const int all = sum_units(A, 0, rows_each).all, run = run_length(A, all);
+    const int group = blockIdx.x, start = group * run;
     int left = min(run, all - start);
     if (left <= 0) return;
-    const Item it = find_item(start, A.S, [&](int s) { return A.units<kRows>(s); });
+    const Item it = find_item(start, A.S, [&](int s) { return A.units(s, rows_each); });
     int s = it.seq;
     if (s < 0) return;
     int blocks = A.blocks(s), column = it.index / blocks, begin = it.index - column * blocks;
-    int columns = A.chunks<kRows>(s) * A.pool.heads;
+    int columns = A.chunks(s, rows_each) * A.pool.heads;
     for (bool first = true;; first = false) {
         const int count = min(left, blocks - begin);
-        work_on_column<RT>(A, s_ks, s_vs, s, column, begin, begin + count, count == blocks ? -1 : 2 * wave + !first);
+        work(s, column, begin, begin + count, count == blocks ? -1 : 2 * group + !first);
         left -= count;
         if (left <= 0) return;
         begin = 0;
@@ -384,111 +679,148 @@ __global__ void __launch_bounds__(kWave, kWavesPerSimd) tree_kernel(TreeArgs A) 
             do {
                 if (++s == A.S) return;
                 blocks = A.blocks(s);
-                columns = A.chunks<kRows>(s) * A.pool.heads;
+                columns = A.chunks(s, rows_each) * A.pool.heads;
             } while (blocks == 0 || columns == 0);
         }
     }
 }
 
-// Joins the records of columns that several waves worked on, two (node, query head) rows per wave and four channels per lane;
-// zeros for nodes that nobody worked on.
-constexpr int kMergeRows = 2 * (kThreads / kWave);
 template <int RT>
-__global__ void __launch_bounds__(kThreads) tree_merge_kernel(TreeArgs A) {
-    constexpr int kRows = RT * kTileRows;
-    const int lane = threadIdx.x & 63, half = lane >> 5;
-    const long row0 = ((long)blockIdx.x * (kThreads / kWave) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) * 2;
-    int first = 0, records = 0, r = 0;   // of the lane's row: its column's first wave, the waves, the row in its chunk
-    bool late = false, zero = false;     // the first wave's record is its last one; the row gets zeros
-    const long mine = row0 + half;
-    const bool there = mine < (long)A.N * A.Hq;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        const long row = row0 + h;
-        if (row >= (long)A.N * A.Hq) break;
-        const int at = (int)(row / A.Hq), head = (int)(row - (long)at * A.Hq);
-        // the sequence of row `at`
-        int s = -1, node = 0;
-        for (int s0 = 0; s0 < A.S && s < 0; s0 += kWave) {
-            const int i = s0 + lane;
-            const Rows q = i < A.S ? sequence_rows(A.offsets, i, A.N) : Rows{0, 0};
-            const uint64_t who = ballot(at >= q.first && at < q.first + q.count);
-            if (who == 0) continue;
-            const int of = __builtin_ctzll(who);
-            s = s0 + of;
-            node = at - __builtin_amdgcn_readlane(q.first, of);
+__global__ void __launch_bounds__(kWave, kWavesPerSimd) tree_alone_kernel(TreeArgs A) {
+    __shared__ OneWave L;
+    run_of(A, RT * kTileRows, [&](int s, int column, int begin, int end, int record) __attribute__((always_inline)) {
+        work_alone<RT>(A, L, s, column, begin, end, record);
+    });
+}
+template <int WAVES, int NB>
+__global__ void __launch_bounds__(WAVES * kWave, kWavesPerSimd) tree_together_kernel(TreeArgs A) {
+    __shared__ Operands L[2][NB];
+    run_of(A, WAVES * 2 * kTileRows, [&](int s, int column, int begin, int end, int record) __attribute__((always_inline)) {
+        work_together<WAVES, NB>(A, L, s, column, begin, end, record);
+    });
+}
+
+// Joins the records of columns that several workgroups worked on, ROWS rows of a sequence and KV head per workgroup: 16
+// threads a row, eight channels each, SPLIT such sets taking the records in turns, eight at a time.  Rows that nobody
+// worked on get zeros; the workgroups behind the last item take the rows of no sequence.
+template <int ROWS, int SPLIT>
+__global__ void __launch_bounds__(ROWS * 16 * SPLIT) tree_merge_kernel(TreeArgs A) {
+    constexpr int kSet = ROWS * 16, kAll = kSet * SPLIT;
+    __shared__ float s_top[SPLIT][ROWS], s_total[SPLIT][ROWS];
+    __shared__ float4 s_o[SPLIT > 1 ? SPLIT - 1 : 1][2][kSet];
+    const int hk = (int)(blockIdx.x % A.pool.heads), item = (int)(blockIdx.x / A.pool.heads), tid = threadIdx.x;
+    const Item it = find_item(item, A.S, [&](int s) { return (int)(((long)sequence_rows(A.offsets, s, A.N).count * A.G + ROWS - 1) / ROWS); });
+    if (it.seq < 0) {
+        if (!A.clear_rest) return;
+        const int spares = (int)(gridDim.x / A.pool.heads) - (item - it.index);
+        const int begin = min(max(A.offsets[0], 0), A.N), end = min(max(A.offsets[A.S], begin), A.N);
+        const long pieces = (long)A.G * (kDim / 8), rest = (begin + A.N - end) * pieces;
+        for (long i = (long)it.index * kAll + tid; i < rest; i += (long)spares * kAll) {
+            const long r = i / pieces, row = r < begin ? r : end + r - begin;
+            reinterpret_cast<uint4*>(A.out + (row * A.Hq + (long)hk * A.G) * kDim)[i - r * pieces] = make_uint4(0, 0, 0, 0);
         }
-        if (s < 0 || node >= A.max_nodes) {
-            if (half == h) zero = A.clear_rest;
-            continue;
-        }
-        const int blocks = A.blocks(s);
-        if (blocks == 0) {
-            if (half == h) zero = true;
-            continue;
-        }
-        const Sums sums = sum_units<kRows>(A, s);
-        const int run = run_length(A, sums.all), hk = head / A.G, in = node * A.G + head - hk * A.G;
-        const int start = sums.before + (hk * A.chunks<kRows>(s) + in / kRows) * blocks;
-        if (half == h) {
-            first = start / run;
-            records = (start + blocks - 1) / run - first + 1;
-            late = first * run != start;
-            r = in % kRows;
-        }
+        return;
     }
-    if (!there) return;
-    uint2* const out = reinterpret_cast<uint2*>(A.out + mine * kDim) + (lane & 31);
-    if (zero) *out = make_uint2(0, 0);
+    const int s = it.seq, set = tid / kSet, row = tid / 16 % ROWS, part = tid % 16;
+    const Rows rows = sequence_rows(A.offsets, s, A.N);
+    const int r = it.index * ROWS + row, node = r / A.G, blocks = A.blocks(s);
+    const bool real = r < rows.count * A.G, worked = node < A.max_nodes;
+    uint4* const out = reinterpret_cast<uint4*>(A.out + ((long)(rows.first + node) * A.Hq + hk * A.G + r - node * A.G) * kDim) + part;
+    if (real && set == 0 && (blocks == 0 || !worked) && (worked || A.clear_rest)) *out = make_uint4(0, 0, 0, 0);
+    if (blocks == 0 || it.index * ROWS >= A.max_nodes * A.G) return;
+    const Sums sums = sum_units(A, s, A.rows_of_chunk);
+    const int run = run_length(A, sums.all), in_chunk = r % A.rows_of_chunk;
+    const int start = sums.before + (hk * A.chunks(s, A.rows_of_chunk) + it.index * ROWS / A.rows_of_chunk) * blocks;
+    const int first = start / run, records = (start + blocks - 1) / run - first + 1;
     if (records <= 1) return;
-    auto record = [&](int i) { return (long)(2 * (first + i) + (i == 0 && late)) * kRows + r; };
-    float top = -__FLT_MAX__, total = 0.0f, o[4] = {};
-    for (int i0 = 0; i0 < records; i0 += 8) {
-        float4 x[8];
+    const bool late = first * run != start;  // the first workgroup's record is that of its last column
+    float top = -__FLT_MAX__, total = 0.0f;
+    float4 o0 = make_float4(0, 0, 0, 0), o1 = o0;
+    for (int i0 = set; i0 < records; i0 += 8 * SPLIT) {
+        float4 x[8][2];
         float2 ml[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            const long rec = record(min(i0 + j, records - 1));
-            x[j] = reinterpret_cast<const float4*>(A.part + rec * kDim)[lane & 31];
+            const int i = min(i0 + SPLIT * j, records - 1);
+            const long rec = (long)(2 * (first + i) + (i == 0 && late)) * A.rows_of_chunk + in_chunk;
+            const float4* const src = reinterpret_cast<const float4*>(A.part + rec * kDim) + 2 * part;
+            x[j][0] = src[0];
+            x[j][1] = src[1];
             ml[j] = A.stat[rec];
         }
         float most = top;
 #pragma unroll
         for (int j = 0; j < 8; ++j) most = fmaxf(most, ml[j].x);
         const float alpha = __builtin_amdgcn_exp2f(top - most);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) o[i] *= alpha;
+        o0.x *= alpha, o0.y *= alpha, o0.z *= alpha, o0.w *= alpha;
+        o1.x *= alpha, o1.y *= alpha, o1.z *= alpha, o1.w *= alpha;
         total *= alpha;
         top = most;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            if (i0 + j >= records || ml[j].y == 0.0f) continue;  // saw nothing (a NaN goes on)
+            if (i0 + SPLIT * j >= records || ml[j].y == 0.0f) continue;  // saw nothing (a NaN goes on)
             const float a = __builtin_amdgcn_exp2f(ml[j].x - top);
-            o[0] += a * x[j].x;
-            o[1] += a * x[j].y;
-            o[2] += a * x[j].z;
-            o[3] += a * x[j].w;
+            o0.x += a * x[j][0].x, o0.y += a * x[j][0].y, o0.z += a * x[j][0].z, o0.w += a * x[j][0].w;
+            o1.x += a * x[j][1].x, o1.y += a * x[j][1].y, o1.z += a * x[j][1].z, o1.w += a * x[j][1].w;
             total += a * ml[j].y;
         }
     }
+    if (SPLIT > 1) {
+        if (part == 0) {
+            s_top[set][row] = top;
+            s_total[set][row] = total;
+        }
+        if (set > 0) {
+            s_o[set - 1][0][tid % kSet] = o0;
+            s_o[set - 1][1][tid % kSet] = o1;
+        }
+        __syncthreads();
+        if (set > 0) return;
+        float most = top;
+#pragma unroll
+        for (int i = 1; i < SPLIT; ++i) most = fmaxf(most, s_top[i][row]);
+        const float alpha = __builtin_amdgcn_exp2f(top - most);
+        o0.x *= alpha, o0.y *= alpha, o0.z *= alpha, o0.w *= alpha;
+        o1.x *= alpha, o1.y *= alpha, o1.z *= alpha, o1.w *= alpha;
+        total *= alpha;
+#pragma unroll
+        for (int i = 1; i < SPLIT; ++i) {
+            if (s_total[i][row] == 0.0f) continue;
+            const float a = __builtin_amdgcn_exp2f(s_top[i][row] - most);
+            const float4 y0 = s_o[i - 1][0][tid], y1 = s_o[i - 1][1][tid];
+            o0.x += a * y0.x, o0.y += a * y0.y, o0.z += a * y0.z, o0.w += a * y0.w;
+            o1.x += a * y1.x, o1.y += a * y1.y, o1.z += a * y1.z, o1.w += a * y1.w;
+            total += a * s_total[i][row];
+        }
+    }
+    if (!real || !worked) return;
     const float inv = total == 0.0f ? 0.0f : 1.0f / total;
-    *out = make_uint2(pack_halves(o[0] * inv, o[1] * inv), pack_halves(o[2] * inv, o[3] * inv));
+    *out = make_uint4(pack_results(o0.x * inv, o0.y * inv), pack_results(o0.z * inv, o0.w * inv), pack_results(o1.x * inv, o1.y * inv),
+                      pack_results(o1.z * inv, o1.w * inv));
 }
 
-// Tiles of rows of a wave: what the widest tree brings, two at most.
-int tiles_of(int G, int max_nodes) { return G * max_nodes <= kTileRows ? 1 : 2; }
+// Rows of a workgroup: what the widest tree brings, 256 at most.
+int chunk_rows(int G, int max_nodes) {
+    const long rows = (long)G * max_nodes;
+    return rows <= 16 ? 16 : rows <= 64 ? 32 : rows <= 128 ? 128 : 256;
+}
+int waves_of(int rows) { return rows <= 32 ? 1 : rows / 32; }
 
 // Units when every sequence has the widest tree (offsets that fall may bring more than N rows in all).
 long most_units(int S, int Hk, int G, long max_length, int max_nodes) {
-    const long rows = tiles_of(G, max_nodes) * kTileRows, blocks = (max_length + kBlock - 1) / kBlock;
+    const long rows = chunk_rows(G, max_nodes), blocks = (max_length + kBlock - 1) / kBlock;
     return blocks * Hk * (((long)max_nodes * G + rows - 1) / rows) * S;
 }
-long tree_waves(int S, long N, int Hk, int G, long max_length, int max_nodes) {
-    const long rows = tiles_of(G, max_nodes) * kTileRows, blocks = (max_length + kBlock - 1) / kBlock;
+// Workgroups: as many as the chip holds at once, or one per unit when there are fewer.
+long tree_groups(int S, long N, int Hk, int G, long max_length, int max_nodes) {
+    const long rows = chunk_rows(G, max_nodes), blocks = (max_length + kBlock - 1) / kBlock;
     const long chunks = (N * G + rows - 1) / rows + S, widest = most_units(S, Hk, G, max_length, max_nodes);
-    const long units = blocks * Hk * chunks < widest ? blocks * Hk * chunks : widest;
-    return units < 1 ? 1 : units < kMostWaves ? units : kMostWaves;
+    const long units = blocks * Hk * chunks < widest ? blocks * Hk * chunks : widest, most = kMostWaves / waves_of(rows);
+    return units < 1 ? 1 : units < most ? units : most;
 }
+
+// Tiles of rows that S sequences of N rows in all can bring, and one that is always free.
+long merge_items(long N, long G, int S, int rows) { return N * G / rows + S + 1; }
 
 }  // namespace
 
@@ -497,7 +829,7 @@ extern "C" int64_t reskv_int4_tree_workspace_bytes(int S, int64_t N, int Hq, int
         max_nodes < 1 || max_nodes > kNodes || Hq / Hk >= (1 << 20))
         return 0;
     const int G = Hq / Hk;
-    return tree_waves(S, N, Hk, G, max_length, max_nodes) * 2 * tiles_of(G, max_nodes) * kTileRows * (kDim + 2) * 4;
+    return tree_groups(S, N, Hk, G, max_length, max_nodes) * 2 * chunk_rows(G, max_nodes) * (kDim + 2) * 4;
 }
 
 extern "C" int reskv_int4_tree_attention(const void* q, const void* pages, int64_t num_pages, int page_tokens,
@@ -517,10 +849,10 @@ extern "C" int reskv_int4_tree_attention(const void* q, const void* pages, int64
     if (max_length > most) max_length = most;
     const int G = Hq / Hk;
     // units and rows are counted in 32 bits; the last wave's run may end behind the last unit
-    RESKV_REQUIRE(most_units(S, Hk, G, max_length, max_nodes) < (1L << 30) && G < (1 << 20) && N * Hq < kLaunchThreads / kWave,
+    RESKV_REQUIRE(most_units(S, Hk, G, max_length, max_nodes) < (1L << 30) && G < (1 << 20) && merge_items(N, G, S, 16) * Hk < kLaunchThreads / kThreads,
                   "too many tokens: blocks of %d x KV heads x chunks of rows must stay below 2^30", kBlock);
     RESKV_REQUIRE(workspace && workspace_bytes >= reskv_int4_tree_workspace_bytes(S, N, Hq, Hk, max_length, max_nodes), "the workspace is too small");
-    const int tiles = tiles_of(G, max_nodes);
+    const int rows = chunk_rows(G, max_nodes);
     TreeArgs A{};
     A.pool = make_pool(pages, num_pages, page_tokens, Hk, table, table_width);
     A.q = (const uint16_t*)q;
@@ -532,17 +864,23 @@ extern "C" int reskv_int4_tree_attention(const void* q, const void* pages, int64
     A.N = (int)N;
     A.Hq = Hq;
     A.G = G;
-    A.waves = (int)tree_waves(S, N, Hk, G, max_length, max_nodes);
+    A.groups = (int)tree_groups(S, N, Hk, G, max_length, max_nodes);
     A.part = (float*)workspace;
-    A.stat = (float2*)(A.part + (long)A.waves * 2 * tiles * kTileRows * kDim);
+    A.stat = (float2*)(A.part + (long)A.groups * 2 * rows * kDim);
     A.max_length = (int)max_length;
     A.max_nodes = max_nodes;
+    A.rows_of_chunk = rows;
     A.clear_rest = clear_rest;
     A.c = scaling * 1.4426950408889634f;
-    hipLaunchKernelGGL(tiles == 1 ? tree_kernel<1> : tree_kernel<2>, dim3((unsigned)A.waves), dim3(kWave), 0, (hipStream_t)stream, A);
+    const auto kernel = rows == 16 ? tree_alone_kernel<1> : rows == 32 ? tree_alone_kernel<2> : rows == 128 ? tree_together_kernel<4, 2> : tree_together_kernel<8, 2>;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)A.groups), dim3(kWave * waves_of(rows)), 0, (hipStream_t)stream, A);
     if (reskv_host::check_launch("tree_kernel")) return 1;
-    const long rows = (long)N * Hq;
-    hipLaunchKernelGGL(tiles == 1 ? tree_merge_kernel<1> : tree_merge_kernel<2>, dim3((unsigned)((rows + kMergeRows - 1) / kMergeRows)),
-                       dim3(kThreads), 0, (hipStream_t)stream, A);
+    // The fewer the rows, the more threads take each one's records, which come from the whole chip then: 8 nodes of 32 heads after
+    // 20000 tokens (256 records a row) 32 us for both kernels with 16 sets and 46 with four, five trees of 1 to 61 nodes 129 with
+    // four and 139 with 16.
+    const long rows_all = (long)N * Hq;
+    const auto merge = rows_all <= 1024 ? tree_merge_kernel<4, 16> : rows_all <= 8192 ? tree_merge_kernel<16, 4> : tree_merge_kernel<16, 1>;
+    hipLaunchKernelGGL(merge, dim3((unsigned)(merge_items(N, G, S, rows_all <= 1024 ? 4 : 16) * Hk)), dim3(rows_all <= 8192 ? 1024 : 256), 0,
+                       (hipStream_t)stream, A);
     return reskv_host::check_launch("tree_merge_kernel");
 }

@@ -733,3 +733,20 @@ def test_append_rope_has_the_bits_of_the_decoder_steps():
     rows = qkv.view(b, -1, D)
     out = int4_append_rope(two, table, starts, rows[:, :hq], rows[:, hq: hq + hk], rows[:, hq + hk:], cos, sin)
     assert torch.equal(out, qr) and torch.equal(one, two)
+
+
+@pytest.mark.parametrize("nodes", [2, 40])
+def test_values_past_the_ends_of_fp16_mix(nodes):
+    """Tokens at both ends of fp16 in one block with ordinary ones, few rows and many: a row's result is their average."""
+    rng = np.random.default_rng(nodes)
+    m = 70 + nodes
+    v = rng.standard_normal((m, 1, D)).astype(np.float16)
+    v[40, :, ::2], v[40, :, 1::2] = 65504.0, -65504.0
+    v[41] = -v[40]
+    k = rng.standard_normal((m, 1, D)).astype(np.float16)
+    q = rng.standard_normal((nodes, 8, D)).astype(np.float16)
+    pool, table = empty_pages(4, 1, 32), i32([[2, 0, 1, 3]])
+    int4_append(pool, table, i32([0]), torch.from_numpy(k).cuda(), torch.from_numpy(v).cuda(), i32([0, m]))
+    (kd, ks), (vd, vs) = stored(k), stored(v)
+    out, bound = ref.tree_attention(q.astype(np.float64), kd, vd, np.tri(nodes, m, 70, dtype=bool), D ** -0.5, ks, vs)
+    within(int4_tree_attention(torch.from_numpy(q).cuda(), pool, table, i32([m]), i32([0, nodes])), out, bound)

@@ -123,22 +123,35 @@ __device__ __forceinline__ uint4 turned_piece(const Turn& R, const uint16_t* hea
     return make_uint4(out[0], out[1], out[2], out[3]);
 }
 
-// The rows' queries of KV head h: eight threads per (row, query head), 16 channels each.
-__device__ __forceinline__ void turn_queries(const RowArgs& A, const Turn& R, const Part& P, int h) {
-    const int at = 16 * ((int)threadIdx.x & 7);
-    for (int u = (int)threadIdx.x >> 3; u < (P.hi - P.lo) * R.G; u += kThreads / 8) {
+// Rows' queries of KV head h: eight threads per (row, query head), 16 channels each; a workgroup takes kQueries of a block's
+// (row, query head), two to a thread.
+constexpr int kQueries = 2 * kThreads / 8;
+__device__ __forceinline__ void turn_queries(const RowArgs& A, const Turn& R, const Part& P, int h, int set) {
+    const int at = 16 * ((int)threadIdx.x & 7), all = (P.hi - P.lo) * R.G;
+    uint4 x[2][2];
+    uint4* dst[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int u = set * kQueries + i * (kThreads / 8) + ((int)threadIdx.x >> 3);
+        dst[i] = nullptr;
+        if (u >= all) continue;
         const int t = u / R.G, head = h * R.G + u - t * R.G;
         const long row = P.row + t;
         const int position = R.positions ? R.positions[row] : P.block * kBlock + P.lo + t;
-        uint4* const dst = reinterpret_cast<uint4*>(R.q_out + (row * A.pool.heads * R.G + head) * kDim + at);
-        if (position >= 0 && position < R.rows) {
-            const uint16_t* const src = R.q + row * R.q_token + head * R.q_head;
-            const uint4 x0 = turned_piece(R, src, at, position), x1 = turned_piece(R, src, at + 8, position);
-            dst[0] = x0;
-            dst[1] = x1;
-        } else if (A.clear_rest) {
-            dst[0] = dst[1] = make_uint4(0, 0, 0, 0);
-        }
+        const bool in = position >= 0 && position < R.rows;
+        if (!in && !A.clear_rest) continue;
+        dst[i] = reinterpret_cast<uint4*>(R.q_out + (row * A.pool.heads * R.G + head) * kDim + at);
+        x[i][0] = x[i][1] = make_uint4(0, 0, 0, 0);
+        if (!in) continue;
+        const uint16_t* const src = R.q + row * R.q_token + head * R.q_head;
+        x[i][0] = turned_piece(R, src, at, position);
+        x[i][1] = turned_piece(R, src, at + 8, position);
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        if (!dst[i]) continue;
+        dst[i][0] = x[i][0];
+        dst[i][1] = x[i][1];
     }
 }
 
@@ -168,13 +181,16 @@ __global__ void __launch_bounds__(kThreads) append_kernel(RowArgs A, Turn R) {
     const int h = (int)blockIdx.x % A.pool.heads, item = (int)blockIdx.x / A.pool.heads;
     const Part P = row_part(A, item);
     if (P.seq < 0) {
-        if (TURN && A.clear_rest && R.q && A.offsets && P.block >= 0 && P.hi == 0) {
+        if (TURN && blockIdx.y == 0 && A.clear_rest && R.q && A.offsets && P.block >= 0 && P.hi == 0) {
             const int first = item - P.block;  // the number of items
             clear_queries(A, R, P.block, (int)gridDim.x / A.pool.heads - first, h);
         }
         return;
     }
-    if (TURN && R.q) turn_queries(A, R, P, h);
+    if (TURN && blockIdx.y > 0) {
+        turn_queries(A, R, P, h, (int)blockIdx.y - 1);
+        return;
+    }
     const int tid = threadIdx.x, token = tid >> 3, part = tid & 7, group = part >> 1;
     bool mine = token >= P.lo && token < P.hi;
     uint4 kw[2] = {}, vw[2] = {};
@@ -931,7 +947,9 @@ extern "C" int reskv_int4_append_rope(void* pages, int64_t num_pages, int page_t
     R.rows = rows;
     R.half = rotary / 2;
     R.interleaved = interleaved;
-    hipLaunchKernelGGL(append_kernel<true>, dim3((unsigned)items), dim3(kThreads), 0, (hipStream_t)stream, A, R);
+    const int sets = (kBlock * R.G + kQueries - 1) / kQueries;  // of a block's queries
+    RESKV_REQUIRE(items * (1 + sets) < kLaunchThreads / kThreads && sets < (1 << 15), "too many rows or sequences");
+    hipLaunchKernelGGL(append_kernel<true>, dim3((unsigned)items, (unsigned)(offsets || !q ? 1 + sets : 1 + (R.G + kQueries - 1) / kQueries)), dim3(kThreads), 0, (hipStream_t)stream, A, R);
     return reskv_host::check_launch("append_rope_kernel");
 }
 

@@ -89,6 +89,7 @@ def verify_drafts(logits, tokens, parents, offsets, accept=None, sample=None, *,
     _require(sequences >= 1, "offsets needs the start and the end of at least one sequence")
     temperature = float(temperature)
     _require(0.0 <= temperature < _INF, "temperature must be finite and not negative")
+    _require(temperature == 0.0 or temperature >= 1e-30, "a temperature that is not 0 must be 1e-30 or more")
     draft_stride = 0
     if temperature == 0.0:
         accept = sample = draft = None

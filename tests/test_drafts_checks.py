@@ -113,6 +113,7 @@ def verify(**changes):
     (dict(draft=torch.zeros(6, 49)), r"draft must be \[6, 50\]"),
     (dict(draft=torch.zeros(1, 50).expand(6, 50)), "draft must have contiguous rows"),
     (dict(temperature=-0.5), "temperature must be finite and not negative"),
+    (dict(temperature=1e-31), "must be 1e-30 or more"),
     (dict(temperature=float("inf")), "temperature must be finite and not negative"),
     (dict(temperature=float("nan")), "temperature must be finite and not negative"),
     (dict(), "every tensor must be a CUDA tensor"),

@@ -40,7 +40,10 @@ __global__ void __launch_bounds__(kWave) tree_masks_kernel(const int32_t* parent
 constexpr int kSegments = 64;         // of a row, at most: one per lane
 constexpr int kPiece = 8;             // elements that a thread takes at once
 constexpr double kSmall = 0x1p-20;    // of a row's sum: what is left of less is added up anew, as a difference has lost its bits
-constexpr int kStatThreads = 256, kWalkThreads = 1024, kWalkWaves = kWalkThreads / kWave;
+constexpr int kStatThreads = 256;
+// Of a walk: greedy, 16 waves take the statistics of 64 rows (24 trees 36 us in all, 38 with eight); else every barrier counts (32
+// chains with draft probabilities 33 us with eight waves, 37 with 16, 38 with four).
+constexpr int walk_threads(bool greedy) { return greedy ? 1024 : 512; }
 
 // A walk that waits for the sums of what a draft that was turned down leaves.
 struct WalkState {
@@ -261,7 +264,8 @@ __device__ __forceinline__ double less(double w, double scale, float q) {
 // over its row and the target's: the first one's is left to verify_rest_kernel, which has a workgroup per segment, and the walk
 // goes on in a second launch (RESUME); any further ones (siblings that were drawn) are done by the workgroup alone.
 template <class T, bool GREEDY, bool RESUME>
-__global__ void __launch_bounds__(kWalkThreads) verify_walk_kernel(VerifyArgs A) {
+__global__ void __launch_bounds__(walk_threads(GREEDY)) verify_walk_kernel(VerifyArgs A) {
+    constexpr int kWalkThreads = walk_threads(GREEDY), kWalkWaves = kWalkThreads / kWave;
     __shared__ double s_total[kNodes];  // of a node's row: sum of exp2((x - most) c)
     __shared__ float s_most[kNodes], s_logit[kNodes], s_q[kNodes], s_accept[kNodes];
     __shared__ int s_parent[kNodes], s_token[kNodes], s_best[kNodes], s_path[kNodes];
@@ -591,13 +595,13 @@ int verify(const VerifyArgs& A, int S, bool greedy, hipStream_t stream) {
                              : (A.pieces <= kStatThreads ? verify_stat_kernel<T, false, 1> : A.pieces <= 2 * kStatThreads ? verify_stat_kernel<T, false, 2> : verify_stat_kernel<T, false, 4>);
     hipLaunchKernelGGL(stat, grid, dim3(kStatThreads), 0, stream, A);
     if (reskv_host::check_launch("verify_stat_kernel")) return 1;
-    hipLaunchKernelGGL((greedy ? verify_walk_kernel<T, true, false> : verify_walk_kernel<T, false, false>), dim3((unsigned)S), dim3(kWalkThreads), 0,
+    hipLaunchKernelGGL((greedy ? verify_walk_kernel<T, true, false> : verify_walk_kernel<T, false, false>), dim3((unsigned)S), dim3(walk_threads(greedy)), 0,
                        stream, A);
     if (reskv_host::check_launch("verify_walk_kernel")) return 1;
     if (!A.draft) return 0;
     hipLaunchKernelGGL(verify_rest_kernel<T>, dim3((unsigned)((long)S * A.segments)), dim3(kStatThreads), 0, stream, A);
     if (reskv_host::check_launch("verify_rest_kernel")) return 1;
-    hipLaunchKernelGGL((verify_walk_kernel<T, false, true>), dim3((unsigned)S), dim3(kWalkThreads), 0, stream, A);
+    hipLaunchKernelGGL((verify_walk_kernel<T, false, true>), dim3((unsigned)S), dim3(walk_threads(false)), 0, stream, A);
     return reskv_host::check_launch("verify_walk_kernel");
 }
 
@@ -767,7 +771,7 @@ extern "C" int reskv_verify_drafts(const void* logits, int logits_fp32, int64_t 
     A.state = (WalkState*)(A.rest + (int64_t)S * A.segments);
     A.c = greedy ? 0.0 : 1.4426950408889634074 / temperature;
     A.N = (int)N;
-    RESKV_REQUIRE(N * A.segments < kLaunchThreads / kStatThreads && (int64_t)S * A.segments < kLaunchThreads / kStatThreads && S < kLaunchThreads / kWalkThreads,
+    RESKV_REQUIRE(N * A.segments < kLaunchThreads / kStatThreads && (int64_t)S * A.segments < kLaunchThreads / kStatThreads && S < kLaunchThreads / walk_threads(greedy),
                   "too many rows or sequences");
     return logits_fp32 ? verify<float>(A, S, greedy, (hipStream_t)stream) : verify<uint16_t>(A, S, greedy, (hipStream_t)stream);
 }

@@ -51,11 +51,13 @@ def _matrix(name, t, dtypes, shape):
     """t must be a matrix of the shape with contiguous rows that do not overlap; returns its row stride."""
     if t.dtype not in dtypes or t.dim() != 2:
         raise RuntimeError(f"{name} must be a matrix of {' or '.join(str(d)[6:] for d in dtypes)}")
-    if shape is not None and tuple(t.shape) != shape:
+    rows, columns = t.shape
+    if shape is not None and (rows, columns) != shape:
         raise RuntimeError(f"{name} must be [{shape[0]}, {shape[1]}]")
-    if not (t.stride(1) == 1 or t.shape[1] == 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
+    row, column = t.stride()
+    if not (column == 1 or columns == 1) or (rows > 1 and row < columns):
         raise RuntimeError(f"{name} must have contiguous rows")
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+    return row if rows > 1 else columns
 
 
 def verify_drafts(logits, tokens, parents, offsets, accept=None, sample=None, *, draft=None, temperature=1.0):
@@ -95,24 +97,24 @@ def verify_drafts(logits, tokens, parents, offsets, accept=None, sample=None, *,
         accept = sample = draft = None
     else:
         for name, t, count in (("accept", accept, n), ("sample", sample, sequences)):
-            _require(t is not None and t.dtype is torch.float32 and t.dim() == 1 and t.is_contiguous() and t.shape[0] == count,
-                     f"{name} must be a contiguous fp32 vector of {count} random numbers")
+            if t is None or t.dtype is not torch.float32 or t.dim() != 1 or t.shape[0] != count or not t.is_contiguous():
+                raise RuntimeError(f"{name} must be a contiguous fp32 vector of {count} random numbers")
         if draft is not None:
             draft_stride = _matrix("draft", draft, (torch.float32,), (n, vocab))
     index = _same_gpu(logits, tokens, parents, offsets, accept, sample, draft)
-    new = dict(device=logits.device)
-    path = torch.empty(sequences, TREE_NODES, dtype=torch.int32, **new)
-    counts = torch.empty(sequences, dtype=torch.int32, **new)
-    token = torch.empty(sequences, dtype=torch.int64, **new)
+    device = logits.device
+    path = torch.empty((sequences, TREE_NODES), dtype=torch.int32, device=device)
+    counts = torch.empty((sequences,), dtype=torch.int32, device=device)
+    token = torch.empty((sequences,), dtype=torch.int64, device=device)
     if n == 0:
         return path.fill_(-1), counts.zero_(), token.fill_(-1)
     if logits.data_ptr() & 15:
         logits = logits.detach().clone(memory_format=torch.contiguous_format)
         stride = vocab
     nbytes = _verify_workspace(sequences, n, vocab)
-    work = _workspace(nbytes, logits.device)
-    ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
+    work = _workspace(nbytes, device)
     _launch("reskv_verify_drafts", index, logits.data_ptr(), logits.dtype is torch.float32, stride, tokens.data_ptr(),
-            parents.data_ptr(), offsets.data_ptr(), ptr(accept), ptr(sample), ptr(draft), draft_stride, temperature, sequences, n,
-            vocab, path.data_ptr(), counts.data_ptr(), token.data_ptr(), work.data_ptr(), nbytes)
+            parents.data_ptr(), offsets.data_ptr(), None if accept is None else accept.data_ptr(),
+            None if sample is None else sample.data_ptr(), None if draft is None else draft.data_ptr(), draft_stride, temperature,
+            sequences, n, vocab, path.data_ptr(), counts.data_ptr(), token.data_ptr(), work.data_ptr(), nbytes)
     return path, counts, token

@@ -96,13 +96,15 @@ def int4_append(pages, table, starts, k, v, offsets=None):
 
 def _rotation(cos, sin):
     """(rows, rotated channels) of the tables."""
-    for name, t in (("cos", cos), ("sin", sin)):
-        if t.dtype is not torch.float32 or t.dim() != 2 or not t.is_contiguous():
-            raise RuntimeError(f"{name} must be a contiguous fp32 matrix [positions, half of the rotated channels]")
-    _require(cos.shape == sin.shape, "cos and sin must have the same shape")
-    _require(0 < cos.shape[0] < 1 << 31, "cos and sin must have a row for every position")
-    _require(cos.shape[1] in range(8, 65, 8), "the rotated channels must be a multiple of 16, up to 128")
-    return cos.shape[0], 2 * cos.shape[1]
+    if cos.dtype is not torch.float32 or cos.dim() != 2 or not cos.is_contiguous():
+        raise RuntimeError("cos must be a contiguous fp32 matrix [positions, half of the rotated channels]")
+    if sin.dtype is not torch.float32 or sin.dim() != 2 or not sin.is_contiguous():
+        raise RuntimeError("sin must be a contiguous fp32 matrix [positions, half of the rotated channels]")
+    rows, half = cos.shape
+    _require(sin.shape[0] == rows and sin.shape[1] == half, "cos and sin must have the same shape")
+    _require(0 < rows < 1 << 31, "cos and sin must have a row for every position")
+    _require(8 <= half <= 64 and half % 8 == 0, "the rotated channels must be a multiple of 16, up to 128")
+    return rows, 2 * half
 
 
 def int4_append_rope(pages, table, starts, q, k, v, cos, sin, offsets=None, *, positions=None, interleaved=False, out=None):
@@ -143,13 +145,14 @@ def int4_append_rope(pages, table, starts, q, k, v, cos, sin, offsets=None, *, p
         _require(out.shape[0] == n and out.is_contiguous(), "out must be contiguous and shaped like q")
     index = _same_gpu(pages, table, starts, k, v, cos, sin, q, offsets, positions, out)
     clear = out is None
-    if q is not None and clear:
-        out = _new(q, (n, q_heads, 128))
+    if q_heads and clear:
+        out = torch.empty((n, q_heads, 128), dtype=torch.float16, device=pages.device)
     if n == 0 or sequences == 0:
         return out.zero_() if clear and out is not None else out
     k, v = _kernel_rows(k), _kernel_rows(v)
-    q = k if q is None else _kernel_rows(q)
-    cos, sin = (t if not t.data_ptr() & 15 else t.detach().clone() for t in (cos, sin))
+    q = _kernel_rows(q) if q_heads else k
+    if (cos.data_ptr() | sin.data_ptr()) & 15:
+        cos, sin = cos.detach().clone(), sin.detach().clone()
     _launch("reskv_int4_append_rope", index, pages.data_ptr(), count, tokens, heads, table.data_ptr(), width, sequences,
             starts.data_ptr(), None if offsets is None else offsets.data_ptr(),
             None if positions is None else positions.data_ptr(), q.data_ptr() if q_heads else None, q_heads, k.data_ptr(),

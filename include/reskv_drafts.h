@@ -39,10 +39,10 @@ int reskv_draft_tree(const int32_t* parents, const int32_t* offsets, const int32
                      int32_t* positions, void* stream);
 
 /* Attention of the trees' nodes over the pages: sequence s has the rows [offsets[s], offsets[s+1]) of q fp16 [N, Hq, 128]
- * (contiguous), n of them, up to max_nodes <= RESKV_DRAFT_NODES; its first lengths[s] tokens count, the last n
- * of which are the nodes.  A node sees every token before them, and node j where bit j of seen[row] is set (seen NULL:
- * the nodes up to itself).  out [N, Hq, 128]: zeros where a node sees nothing; rows of no sequence and nodes from max_nodes on
- * are left as they are, or set to zero with clear_rest.  max_length as in reskv_int4_attention; scaling > 0. */
+ * (contiguous), n of them; its first lengths[s] tokens count, the last n of which are the nodes.  A node sees every token
+ * before them, and node j where bit j of seen[row] is set (seen NULL: the nodes up to itself).  out [N, Hq, 128]: zeros
+ * where a node sees nothing; rows of no sequence and nodes from max_nodes <= RESKV_DRAFT_NODES on are left as they are, or set
+ * to zero with clear_rest.  max_length as in reskv_int4_attention; scaling > 0. */
 int64_t reskv_int4_tree_workspace_bytes(int S, int64_t N, int Hq, int Hk, int64_t max_length, int max_nodes);
 int reskv_int4_tree_attention(const void* q, const void* pages, int64_t num_pages, int page_tokens, const int32_t* table,
                               int table_width, const int32_t* lengths, const int32_t* offsets, const uint64_t* seen, int S,
@@ -55,6 +55,7 @@ int reskv_int4_tree_attention(const void* q, const void* pages, int64_t num_page
  * token t was drawn from (draft[row], fp32 [N, V], draft_stride apart; draft NULL: all of it at t):
  *   accept[row] * q(t) < r(t) / sum r: x is reached, and r is its softmax;
  *   else r becomes max(r / sum r - q, 0), or stays where that leaves nothing.
+ * temperature is 0, or 1e-30 and more.
  * path[s] [RESKV_DRAFT_NODES] lists the nodes reached, the root first, and -1 behind them; counts[s] says how many;
  * token[s] is the first t with r(0) + .. + r(t) > sample[s] * sum r.  With temperature 0, r has one token, the
  * argmax (the lowest of equals), and accept, sample and draft are not read.  Sums are 64 bits.  A node whose token is outside the

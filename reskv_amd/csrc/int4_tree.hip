@@ -10,11 +10,27 @@
 // V's codes lie in a lane.  Softmax and its statistics are then a lane's own but for the maximum, and the weights are the B
 // operand of
 //   O^T [channel][row] += V^T P^T
-// as they are, without the LDS.  V = code * scale + low is rounded to fp16 once (the row that reskv_int4_gather gives): the
-// work of that is shared by the rows of a wave.
+// as they are, without the LDS.  V = code * scale + low is rounded to fp16 once (the row that reskv_int4_gather gives).
 //
-// Scores, softmax and sums are fp32.  Weights are 2^9 exp2(x - m), m at most 6 below the row's largest score so far, rounded
-// to fp16 for the product and summed as rounded: eleven bits down to 2^-23 of the largest weight.
+// Scores, softmax and sums are fp32.  Weights are 2^8 exp2(x - m), m at most 6 below the row's largest score so far, rounded
+// to fp16 for the product and summed as rounded: eleven bits down to 2^-22 of the largest weight.  With V and the weights rounded
+// to fp16, results differ from those of 64 bits by 2.8e-4 to 3.0e-4, of which their own rounding is 2.07e-4; V as codes with the
+// scales in the weights (int4.hip) would be 2.2e-4, and takes a rounding of every weight for each of the four groups instead of one.
+//
+// Up to 64 rows a wave works by itself on 16 or 32 of them and takes what it needs of a block from memory to registers; from
+// there on four or eight waves share the operands of two blocks at a time through the LDS, where the work of making them, as
+// much as that of 32 rows, is done once.  32 sequences of 4000 tokens, 32 / 8 heads, us by nodes a tree, as chosen / 32 rows a wave
+// alone / 128 and 256 rows together: 16: 93 / 93 / 117 / 144, 20: 121 / 125 / 121 / 146, 32: 130 / 151 / 132 / 150, 48: 200 / 199 /
+// 219 / 198.
+//
+// Bound: few rows by memory's latency and the vector ALU together (32 trees of up to 16 nodes after 2000 to 8192 tokens: 76 us and
+// 10 for the merge; 370 vector instructions per block and 32 rows, the ALU busy half of the time); many rows by the vector ALU (32
+// trees of 64 nodes after 8192 tokens: 380 us, 720 TFLOP/s; 140 vector instructions, 16 of them exponentials, and 36
+// matrix instructions per 32 rows and block, whose issue takes nine tenths of the time in which a workgroup multiplies, and that is
+// three quarters of all).
+// What made no difference there: the order of reads, products and sums in a wave by hand, one barrier per block or per two,
+// a third buffer with the barrier before the products.  One tile of rows a wave and four waves a SIMD (registers spill) 469 us
+// instead of 434, four waves and half the rows a workgroup 468, two 580.  A wave's priority while it multiplies: 410 to 393.
 #include "int4.h"
 #include "reskv_drafts.h"
 
@@ -45,7 +61,8 @@ struct TreeArgs {
 
     __device__ __forceinline__ int tokens(int s) const { return min(max(lengths[s], 0), max_length); }
     __device__ __forceinline__ int blocks(int s) const { return (tokens(s) + kBlock - 1) / kBlock; }
-    __device__ __forceinline__ Rows rows(int s) const {
+    __device__ __forceinline__ int nodes(int s) const { return sequence_rows(offsets, s, N).count; }  // all of them
+    __device__ __forceinline__ Rows rows(int s) const {                                               // that are worked on
         const Rows r = sequence_rows(offsets, s, N);
         return {r.first, min(r.count, max_nodes)};
     }
@@ -129,9 +146,9 @@ struct RowState {
 
     // Rows r0 .. of the sequence and KV head.  Each is brought to its own power of two, so that the sixteenth of an element,
     // which meets codes times 2^-20, keeps its bits.
-    __device__ __forceinline__ void start(const TreeArgs& A, const Rows& rows, int hk, int r0, int lane) {
+    __device__ __forceinline__ void start(const TreeArgs& A, const Rows& rows, int nodes, int hk, int r0, int lane) {
         const int n = lane & 15, quarter = lane >> 4, total = rows.count * A.G;
-        const uint64_t all = rows.count < 64 ? (1ull << rows.count) - 1 : ~0ull;
+        const uint64_t all = nodes < kNodes ? (1ull << nodes) - 1 : ~0ull;
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
             const int r = r0 + rt * kTileRows + n, node = r / A.G;
@@ -175,77 +192,73 @@ struct RowState {
         }
     }
 
-    // The weights of NB blocks, as operands.  key(b, j, g): the K operand of tile j and group g of block b; scale(b, g): the
-    // scales of the tokens 8 quarter .. + 7; low(b, j): the lowest value of the lane's K row and group.  Of block b valid[b] tokens
-    // are there, from tree[b] on they are nodes; `visible` gets the tokens that a row sees where some do not.
-    template <int NB, bool SHARED, class Key, class Scale, class Low, class Before, class Between>
-    __device__ __forceinline__ void weights(half8_t (*p)[RT], uint32_t (*visible)[RT], const int* valid, const int* tree, int quarter, Key key,
+    // The weights of a block, as operands.  key(j, g): the K operand of tile j and group g; scale(g): the scales of the tokens 8
+    // quarter .. + 7; low(j): the lowest value of the lane's K row and group.  `valid` tokens are there, from `tree` on they
+    // are nodes; `visible` gets the tokens that a row sees where some do not.  before_softmax() comes behind the scores, between(rt, i)
+    // in four places among the weights of the row tile behind rt.
+    template <bool SHARED, class Key, class Scale, class Low, class Before, class Between>
+    __device__ __forceinline__ void weights(half8_t* p, uint32_t* visible, int valid, int tree, int quarter, Key key,
                                             Scale scale, Low low, Before before_softmax, Between between) {
-        float4_t score[NB][RT][2];
+        float4_t score[RT][2];
         const float4_t zero = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (SHARED) __builtin_amdgcn_s_setprio(1);
+        float lows[2];
+        half8_t scales[4], keys[4][2];
+        auto read = [&](int g) __attribute__((always_inline)) {
 #pragma unroll
-        for (int b = 0; b < NB; ++b) {
-            if (SHARED) __builtin_amdgcn_s_setprio(1);
-            float lows[2];
-            half8_t scales[4], keys[4][2];
-            auto read = [&](int g) __attribute__((always_inline)) {
+            for (int j = 0; j < 2; ++j) keys[g][j] = key(j, g);
+            scales[g] = __builtin_bit_cast(half8_t, scale(g));
+        };
 #pragma unroll
-                for (int j = 0; j < 2; ++j) keys[g][j] = key(b, j, g);
-                scales[g] = __builtin_bit_cast(half8_t, scale(b, g));
-            };
+        for (int j = 0; j < 2; ++j) lows[j] = low(j);
+        read(0);
+        read(1);
+        float4_t d[2][2][RT];
+        auto multiply = [&](int g, int j, int rt) __attribute__((always_inline)) {
+            d[g & 1][j][rt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(keys[g][j], q[rt][g], zero, 0, 0, 0);
+        };
 #pragma unroll
-            for (int j = 0; j < 2; ++j) lows[j] = low(b, j);
-            read(0);
-            read(1);
-            float4_t d[2][2][RT];
-            auto multiply = [&](int g, int j, int rt) __attribute__((always_inline)) {
-                d[g & 1][j][rt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(keys[g][j], q[rt][g], zero, 0, 0, 0);
-            };
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) multiply(0, j, rt);
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            if (g < 2) read(g + 2);
 #pragma unroll
             for (int j = 0; j < 2; ++j)
 #pragma unroll
-                for (int rt = 0; rt < RT; ++rt) multiply(0, j, rt);
+                for (int rt = 0; rt < RT; ++rt) {
+                    if (g < 3) multiply(g + 1, j, rt);
 #pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                if (g < 2) read(g + 2);
-#pragma unroll
-                for (int j = 0; j < 2; ++j)
-#pragma unroll
-                    for (int rt = 0; rt < RT; ++rt) {
-                        if (g < 3) multiply(g + 1, j, rt);
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const float x = d[g & 1][j][rt][i], sc = (float)scales[g][4 * j + i];
-                            score[b][rt][j][i] = __builtin_fmaf(x, sc, g == 0 ? 0.0f : score[b][rt][j][i]);  // one instruction
-                        }
-                        if (g == 3) score[b][rt][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(lows[j], sum[rt], score[b][rt][j], 0, 0, 0);
+                    for (int i = 0; i < 4; ++i) {
+                        const float x = d[g & 1][j][rt][i], sc = (float)scales[g][4 * j + i];
+                        score[rt][j][i] = __builtin_fmaf(x, sc, g == 0 ? 0.0f : score[rt][j][i]);  // one instruction
                     }
-            }
+                    if (g == 3) score[rt][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(lows[j], sum[rt], score[rt][j], 0, 0, 0);
+                }
         }
         if (SHARED) __builtin_amdgcn_s_setprio(0);
         before_softmax();
+        if (tree < kBlock || valid < kBlock) {
 #pragma unroll
-        for (int b = 0; b < NB; ++b)
-            if (tree[b] < kBlock || valid[b] < kBlock) {
+            for (int rt = 0; rt < RT; ++rt) {
+                uint32_t bits = tree <= 0 ? (tree > -64 ? (uint32_t)(sees[rt] >> -tree) : 0u)
+                                          : tree < kBlock ? (uint32_t)(sees[rt] << tree) | ((1u << tree) - 1u) : ~0u;
+                if (valid < kBlock) bits &= (1u << valid) - 1u;
+                visible[rt] = bits;
+                const uint32_t mine = bits >> (8 * quarter);
 #pragma unroll
-                for (int rt = 0; rt < RT; ++rt) {
-                    uint32_t bits = tree[b] <= 0 ? (tree[b] > -64 ? (uint32_t)(sees[rt] >> -tree[b]) : 0u)
-                                                 : tree[b] < kBlock ? (uint32_t)(sees[rt] << tree[b]) | ((1u << tree[b]) - 1u) : ~0u;
-                    if (valid[b] < kBlock) bits &= (1u << valid[b]) - 1u;
-                    visible[b][rt] = bits;
-                    const uint32_t mine = bits >> (8 * quarter);
-#pragma unroll
-                    for (int e = 0; e < 8; ++e)
-                        if (!((mine >> e) & 1u)) score[b][rt][e >> 2][e & 3] = -INFINITY;
-                }
+                for (int e = 0; e < 8; ++e)
+                    if (!((mine >> e) & 1u)) score[rt][e >> 2][e & 3] = -INFINITY;
             }
+        }
         bool grow = false;
         float top[RT];
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
-            top[rt] = score[0][rt][0][0];
+            top[rt] = score[rt][0][0];
 #pragma unroll
-            for (int i = 1; i < 8 * NB; ++i) top[rt] = fmaxf(top[rt], score[i >> 3][rt][i >> 2 & 1][i & 3]);
+            for (int i = 1; i < 8; ++i) top[rt] = fmaxf(top[rt], score[rt][i >> 2][i & 3]);
             top[rt] *= back[rt];
             grow |= top[rt] > m[rt] + kSlack;
         }
@@ -263,22 +276,20 @@ struct RowState {
         }
         const half2_t ones = {(_Float16)1.0f, (_Float16)1.0f};
 #pragma unroll
-        for (int b = 0; b < NB; ++b)
+        for (int rt = 0; rt < RT; ++rt) {
+            const float shift = kWeightBits - m[rt];
+            float total = 0.0f;
 #pragma unroll
-            for (int rt = 0; rt < RT; ++rt) {
-                const float shift = kWeightBits - m[rt];
-                float total = 0.0f;
-#pragma unroll
-                for (int e = 0; e < 8; e += 2) {
-                    if (rt > 0) between(b, rt - 1, e >> 1);
-                    const half2_t w = {(_Float16)__builtin_amdgcn_exp2f(__builtin_fmaf(score[b][rt][e >> 2][e & 3], back[rt], shift)),
-                                       (_Float16)__builtin_amdgcn_exp2f(__builtin_fmaf(score[b][rt][e >> 2][(e & 3) + 1], back[rt], shift))};
-                    total = __builtin_amdgcn_fdot2(w, ones, total, false);
-                    p[b][rt][e] = w[0];
-                    p[b][rt][e + 1] = w[1];
-                }
-                l[rt] += total;
+            for (int e = 0; e < 8; e += 2) {
+                if (rt > 0) between(rt - 1, e >> 1);
+                const half2_t w = {(_Float16)__builtin_amdgcn_exp2f(__builtin_fmaf(score[rt][e >> 2][e & 3], back[rt], shift)),
+                                   (_Float16)__builtin_amdgcn_exp2f(__builtin_fmaf(score[rt][e >> 2][(e & 3) + 1], back[rt], shift))};
+                total = __builtin_amdgcn_fdot2(w, ones, total, false);
+                p[rt][e] = w[0];
+                p[rt][e + 1] = w[1];
             }
+            l[rt] += total;
+        }
     }
 
     // A value tile times the weights.
@@ -418,7 +429,7 @@ __device__ __forceinline__ void work_alone(const TreeArgs& A, OneWave& L, int s,
     const int lane = threadIdx.x, n = lane & 15, quarter = lane >> 4;
     const Rows rows = A.rows(s);
     const int chunks = A.chunks(s, kRows), hk = column / chunks, r0 = (column - hk * chunks) * kRows;
-    const int length = A.tokens(s), context = length - rows.count;
+    const int nodes = A.nodes(s), length = A.tokens(s), context = length - nodes;
     Walk at;
     at.start(A, s, hk, begin, lane);
     TreeBlock x0, x1;
@@ -432,7 +443,7 @@ __device__ __forceinline__ void work_alone(const TreeArgs& A, OneWave& L, int s,
     };
     bool there0 = fetch(x0, begin), there1;  // before Q, so that the first block does not wait for it
     RowState<RT> R;
-    R.start(A, rows, hk, r0, lane);
+    R.start(A, rows, nodes, hk, r0, lane);
     const Masks M;
 
     auto work = [&](TreeBlock& x, int blk, bool there) __attribute__((always_inline)) {
@@ -466,12 +477,12 @@ __device__ __forceinline__ void work_alone(const TreeArgs& A, OneWave& L, int s,
         L.vs[lane] = x.vs;
         L.vl[lane] = x.vl;
         wave_sync();
-        half8_t p[1][RT];
-        uint32_t visible[1][RT];
-        R.template weights<1, false>(p, visible, &valid, &tree, quarter,
-                              [&](int, int j, int g) __attribute__((always_inline)) { return operand(dword(x.k[j], g)); },
-                              [&](int, int g) __attribute__((always_inline)) { return reinterpret_cast<const uint4*>(L.scale)[4 * g + quarter]; },
-                              [&](int, int j) __attribute__((always_inline)) { return h2f((uint16_t)(x.ks[j] >> 16)); }, []() {}, [](int, int, int) {});
+        half8_t p[RT];
+        uint32_t visible[RT];
+        R.template weights<false>(p, visible, valid, tree, quarter,
+                                  [&](int j, int g) __attribute__((always_inline)) { return operand(dword(x.k[j], g)); },
+                                  [&](int g) __attribute__((always_inline)) { return reinterpret_cast<const uint4*>(L.scale)[4 * g + quarter]; },
+                                  [&](int j) __attribute__((always_inline)) { return h2f((uint16_t)(x.ks[j] >> 16)); }, []() {}, [](int, int) {});
         auto value = [&](int ct) __attribute__((always_inline)) {
             const int of = 4 * (ct >> 1) + quarter;
             return values_of(M, dword(x.v[ct >> 2], ct & 3), reinterpret_cast<const uint4*>(L.vs)[of], reinterpret_cast<const uint4*>(L.vl)[of]);
@@ -479,12 +490,12 @@ __device__ __forceinline__ void work_alone(const TreeArgs& A, OneWave& L, int s,
         if (odd) {
             const _Float16 two = (_Float16)2.0f;
 #pragma unroll
-            for (int rt = 0; rt < RT; ++rt) p[0][rt] *= half8_t{two, two, two, two, two, two, two, two};
+            for (int rt = 0; rt < RT; ++rt) p[rt] *= half8_t{two, two, two, two, two, two, two, two};
         }
 #pragma unroll
-        for (int ct = 0; ct < 8; ++ct) R.add(ct, value(ct), p[0]);
+        for (int ct = 0; ct < 8; ++ct) R.add(ct, value(ct), p);
         if ((bad0 | bad1) != 0)
-            R.add_bad(visible[0], [&](int g) {
+            R.add_bad(visible, [&](int g) {
                 uint32_t bits = 0;
                 for (int t = 0; t < kBlock; ++t) bits |= (uint32_t)((t & 1 ? bad1 : bad0) >> (16 * g + (t >> 1)) & 1u) << t;
                 return bits;
@@ -522,26 +533,28 @@ struct Share {
     uint4 vs, vl;    // their scales and lowest values
 };
 
-// WAVES waves of 32 rows each take NB blocks per step; the blocks' four tasks each are shared out among the waves.  A block that
+constexpr int kStep = 2;  // blocks
+
+// WAVES waves of 32 rows each take kStep blocks per step; the blocks' four tasks each are shared out among the waves.  A block that
 // is not there counts as one without tokens.
-template <int WAVES, int NB>
-__device__ __forceinline__ void work_together(const TreeArgs& A, Operands (*L)[NB], int s, int column, int begin, int end, int record) {
-    constexpr int RT = 2, kWaveRows = RT * kTileRows, kRows = WAVES * kWaveRows, kItems = 4 * NB / WAVES;
+template <int WAVES>
+__device__ __forceinline__ void work_together(const TreeArgs& A, Operands (*L)[kStep], int s, int column, int begin, int end, int record) {
+    constexpr int RT = 2, kWaveRows = RT * kTileRows, kRows = WAVES * kWaveRows, kItems = 4 * kStep / WAVES;
     const int lane = threadIdx.x & 63, n = lane & 15, quarter = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const Rows rows = A.rows(s);
     const int chunks = A.chunks(s, kRows), hk = column / chunks, r0 = (column - hk * chunks) * kRows + wave * kWaveRows;
-    const int length = A.tokens(s), context = length - rows.count;
+    const int nodes = A.nodes(s), length = A.tokens(s), context = length - nodes;
     const bool active = r0 < rows.count * A.G;
     Walk at;
     at.start(A, s, hk, begin, lane);
     Share x[kItems];
-    // the wave's shares of the blocks blk .. blk + NB - 1; which of them are there, as bits
+    // the wave's shares of the blocks blk .. blk + kStep - 1; which of them are there, as bits
     auto fetch = [&](int blk) __attribute__((always_inline)) {
-        const char* found[NB];
+        const char* found[kStep];
         uint32_t there = 0;
 #pragma unroll
-        for (int b = 0; b < NB; ++b) {
+        for (int b = 0; b < kStep; ++b) {
             there |= (uint32_t)(at.there && blk + b < end) << b;
             found[b] = at.at;
             if (blk + b + 1 < end) at.next(A, s, hk, lane);
@@ -549,7 +562,7 @@ __device__ __forceinline__ void work_together(const TreeArgs& A, Operands (*L)[N
 #pragma unroll
         for (int i = 0; i < kItems; ++i) {
             const int item = wave + i * WAVES, task = item & 3, t = token_of(n, task >> 1), u = lane & 31;
-            const char* const p = NB == 1 || item < 4 ? found[0] : found[NB - 1];
+            const char* const p = item < 4 ? found[0] : found[1];
             const BlockLoads P(p);
             x[i].k = P.b64(16 * ((t >> 4) * 64 + quarter * 16 + (t & 15)) + 8 * (task & 1), 0);
             x[i].ks = P.b32(4 * (((u >> 4) * 4 + task) * 16 + (u & 15)), kKScale);
@@ -611,44 +624,45 @@ __device__ __forceinline__ void work_together(const TreeArgs& A, Operands (*L)[N
     };
     uint32_t there = fetch(begin), there_next = 0;
     RowState<RT> R;
-    R.start(A, rows, hk, r0, lane);
+    R.start(A, rows, nodes, hk, r0, lane);
     stage(L[0], begin, there);
-    if (begin + NB < end) there_next = fetch(begin + NB);
+    if (begin + kStep < end) there_next = fetch(begin + kStep);
     __syncthreads();
     int side = 0;
-    for (int blk = begin; blk < end; blk += NB) {
+    for (int blk = begin; blk < end; blk += kStep) {
         const Operands* const O = L[side];
         side ^= 1;
         const uint32_t here = there;
-        if (blk + NB < end) stage(L[side], blk + NB, there_next);
+        if (blk + kStep < end) stage(L[side], blk + kStep, there_next);
         there = there_next;
-        if (blk + 2 * NB < end) there_next = fetch(blk + 2 * NB);
+        if (blk + 2 * kStep < end) there_next = fetch(blk + 2 * kStep);
         if (here && active) {
 #pragma unroll
-            for (int b = 0; b < NB; ++b) {
+            for (int b = 0; b < kStep; ++b) {
                 if (!(here >> b & 1)) continue;
                 const Operands& B = O[b];
                 const int valid = valid_of(blk + b, true), tree = context - (blk + b) * kBlock;
-                half8_t p[1][RT];
-                uint32_t visible[1][RT];
-                half8_t v[8];
-                R.template weights<1, true>(
-                    p, visible, &valid, &tree, quarter,
-                    [&](int, int j, int g) __attribute__((always_inline)) { return __builtin_bit_cast(half8_t, B.k[j][g][lane]); },
-                    [&](int, int g) __attribute__((always_inline)) { return reinterpret_cast<const uint4*>(B.scale)[4 * g + quarter]; },
-                    [&](int, int j) __attribute__((always_inline)) { return B.low[quarter * kBlock + token_of(n, j)]; },
+                half8_t p[RT], v[8];
+                uint32_t visible[RT];
+                R.template weights<true>(
+                    p, visible, valid, tree, quarter,
+                    [&](int j, int g) __attribute__((always_inline)) { return __builtin_bit_cast(half8_t, B.k[j][g][lane]); },
+                    [&](int g) __attribute__((always_inline)) { return reinterpret_cast<const uint4*>(B.scale)[4 * g + quarter]; },
+                    [&](int j) __attribute__((always_inline)) { return B.low[quarter * kBlock + token_of(n, j)]; },
                     [&]() __attribute__((always_inline)) {  // on their way during the softmax
 #pragma unroll
                         for (int ct = 0; ct < 8; ++ct) v[ct] = __builtin_bit_cast(half8_t, B.v[ct][lane]);
                     },
-                    [&](int, int rt, int i) __attribute__((always_inline)) {  // the row tile's products between the next one's weights
-                        R.add_one(2 * i, rt, v[2 * i], p[0]);
-                        R.add_one(2 * i + 1, rt, v[2 * i + 1], p[0]);
+                    [&](int rt, int i) __attribute__((always_inline)) {  // the row tile's products between the next one's weights
+                        R.add_one(2 * i, rt, v[2 * i], p);
+                        R.add_one(2 * i + 1, rt, v[2 * i + 1], p);
                     });
+                __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-                for (int ct = 0; ct < 8; ++ct) { if (ct == 0) __builtin_amdgcn_s_setprio(1); R.add_one(ct, RT - 1, v[ct], p[0]); if (ct == 7) __builtin_amdgcn_s_setprio(0); }
+                for (int ct = 0; ct < 8; ++ct) R.add_one(ct, RT - 1, v[ct], p);
+                __builtin_amdgcn_s_setprio(0);
                 if (tree < kBlock && (B.bad[0] | B.bad[1] | B.bad[2] | B.bad[3]) != 0)
-                    R.add_bad(visible[0], [&](int g) __attribute__((always_inline)) { return B.bad[g]; });
+                    R.add_bad(visible, [&](int g) __attribute__((always_inline)) { return B.bad[g]; });
             }
         }
         __syncthreads();
@@ -692,11 +706,11 @@ __global__ void __launch_bounds__(kWave, kWavesPerSimd) tree_alone_kernel(TreeAr
         work_alone<RT>(A, L, s, column, begin, end, record);
     });
 }
-template <int WAVES, int NB>
+template <int WAVES>
 __global__ void __launch_bounds__(WAVES * kWave, kWavesPerSimd) tree_together_kernel(TreeArgs A) {
-    __shared__ Operands L[2][NB];
+    __shared__ Operands L[2][kStep];
     run_of(A, WAVES * 2 * kTileRows, [&](int s, int column, int begin, int end, int record) __attribute__((always_inline)) {
-        work_together<WAVES, NB>(A, L, s, column, begin, end, record);
+        work_together<WAVES>(A, L, s, column, begin, end, record);
     });
 }
 
@@ -872,7 +886,7 @@ extern "C" int reskv_int4_tree_attention(const void* q, const void* pages, int64
     A.rows_of_chunk = rows;
     A.clear_rest = clear_rest;
     A.c = scaling * 1.4426950408889634f;
-    const auto kernel = rows == 16 ? tree_alone_kernel<1> : rows == 32 ? tree_alone_kernel<2> : rows == 128 ? tree_together_kernel<4, 2> : tree_together_kernel<8, 2>;
+    const auto kernel = rows == 16 ? tree_alone_kernel<1> : rows == 32 ? tree_alone_kernel<2> : rows == 128 ? tree_together_kernel<4> : tree_together_kernel<8>;
     hipLaunchKernelGGL(kernel, dim3((unsigned)A.groups), dim3(kWave * waves_of(rows)), 0, (hipStream_t)stream, A);
     if (reskv_host::check_launch("tree_kernel")) return 1;
     // The fewer the rows, the more threads take each one's records, which come from the whole chip then: 8 nodes of 32 heads after

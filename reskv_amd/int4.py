@@ -498,6 +498,7 @@ class Int4Cache:
         _int32("counts", counts, self.sequences)
         kept = counts.tolist()
         _require(all(0 <= k <= c for k, c in zip(kept, self._counts)), "a row keeps between none and all of the tokens reserved last")
+        _require(path.dim() == 2 and max(kept) <= path.shape[1], "path must list every token that is kept")
         int4_keep(self.pool, self.table, self.starts, path, counts)
         changed = []
         for s, (k, c) in enumerate(zip(kept, self._counts)):

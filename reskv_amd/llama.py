@@ -584,9 +584,10 @@ class GreedyDecoder:
               "parents must name a node before it for every draft")
         for name, t, shape in (("accept", accept, (self.batch, m + 1)), ("sample", sample, (self.batch,)),
                                ("draft", draft, (self.batch, m + 1, self.model.shape.vocab))):
-            _need(t is None or tuple(t.shape) == shape, f"{name} must be {list(shape)}")
+            _need(t is None or (tuple(t.shape) == shape and t.dtype == torch.float32), f"{name} must be fp32 {list(shape)}")
+        _need(temperature == 0.0 or 1e-30 <= temperature < math.inf, "temperature must be 0, or 1e-30 and more")
         _need(temperature == 0.0 or (accept is not None and sample is not None), "sampling needs random numbers")
-        _on_gpu(drafts)
+        _on_gpu(drafts, accept, sample, draft)
         with torch.cuda.device(self.x.device):
             return self._nodes(torch.cat([self.tok[:, None], drafts], dim=1), parents, temperature, accept, sample, draft, None)
 
@@ -618,11 +619,12 @@ class GreedyDecoder:
             x.addmm_(fused_silu_mul(F.linear(h, p["wgu"]), act), p["wd"].t())
         logits = F.linear(fused_rmsnorm(x, self.model.norm, s.rms_eps, h), self.model.lm_head)
         path, counts, token = verify_drafts(logits, ids.reshape(-1), above, offsets, None if accept is None else accept.reshape(-1),
-                                            sample, draft=None if draft is None else draft.flatten(0, 1),
-                                            temperature=temperature)
-        kept = self.pages.keep(path, counts)
+                                            None if sample is None else sample.contiguous(),
+                                            draft=None if draft is None else draft.flatten(0, 1), temperature=temperature)
         if bool((token < 0).any()):
+            self.pages.keep(path, torch.zeros_like(counts))
             raise RuntimeError("the model's logits hold a NaN or an infinity")
+        kept = self.pages.keep(path, counts)
         self.tok.copy_(token)
         self.x.copy_(self.model.embed[self.tok])
         self.pos = max(self.pages._lengths)

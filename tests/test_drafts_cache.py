@@ -59,6 +59,15 @@ def test_more_than_was_reserved_is_refused(moved, counts):
     assert not moved and cache.lengths.tolist() == [13, 11]
 
 
+def test_a_path_shorter_than_what_is_kept_is_refused(moved):
+    cache = Int4Cache(1, 1, 2, 200, device="cpu")
+    cache.reserve(5)
+    for bad in (torch.zeros(2, 3, **i32), torch.zeros(128, **i32)):
+        with pytest.raises(RuntimeError, match="path must list every token that is kept"):
+            cache.keep(bad, torch.tensor([4, 1], **i32))
+    assert not moved and cache.lengths.tolist() == [5, 5]
+
+
 def test_forked_rows_are_refused(moved):
     cache = Int4Cache(1, 1, 2, 200, device="cpu")
     cache.reserve([10, 10])
@@ -99,9 +108,12 @@ def decoder():
     (dict(parents=[0, 2, 1]), "a node before it for every draft"),
     (dict(parents=[-1, 0, 0]), "a node before it for every draft"),
     (dict(temperature=1.0), "sampling needs random numbers"),
-    (dict(temperature=1.0, accept=torch.zeros(2, 3), sample=torch.zeros(2)), r"accept must be \[2, 4\]"),
-    (dict(temperature=1.0, accept=torch.zeros(2, 4), sample=torch.zeros(4)), r"sample must be \[2\]"),
-    (dict(temperature=1.0, accept=torch.zeros(2, 4), sample=torch.zeros(2), draft=torch.zeros(2, 4, 49)), r"draft must be \[2, 4, 50\]"),
+    (dict(temperature=1.0, accept=torch.zeros(2, 3), sample=torch.zeros(2)), r"accept must be fp32 \[2, 4\]"),
+    (dict(temperature=1.0, accept=torch.zeros(2, 4, dtype=torch.float64), sample=torch.zeros(2)), r"accept must be fp32 \[2, 4\]"),
+    (dict(temperature=-1.0, accept=torch.zeros(2, 4), sample=torch.zeros(2)), "temperature must be 0, or"),
+    (dict(temperature=float("nan"), accept=torch.zeros(2, 4), sample=torch.zeros(2)), "temperature must be 0, or"),
+    (dict(temperature=1.0, accept=torch.zeros(2, 4), sample=torch.zeros(4)), r"sample must be fp32 \[2\]"),
+    (dict(temperature=1.0, accept=torch.zeros(2, 4), sample=torch.zeros(2), draft=torch.zeros(2, 4, 49)), r"draft must be fp32 \[2, 4, 50\]"),
     (dict(), "every tensor must be a CUDA tensor"),
 ])
 def test_step_drafts_checks(decoder, kw, match):

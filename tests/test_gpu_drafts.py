@@ -339,8 +339,8 @@ def test_rows_of_no_sequence_and_nodes_past_the_last():
     kept = torch.full_like(q, 3.0)
     assert int4_tree_attention(**more, out=kept) is kept
     assert (kept[0] == 3).all() and (kept[-2:] == 3).all() and torch.equal(kept[1:-2], got[1:-2])
-    few = int4_tree_attention(**more, max_nodes=4)  # six rows of the first sequence, of which four are nodes: the last 4 tokens
-    assert (few[5:7] == 0).all()
+    few = int4_tree_attention(**more, max_nodes=4)  # six rows of the first sequence, of which four are worked on
+    assert (few[5:7] == 0).all() and torch.equal(few[1:5], got[1:5]) and torch.equal(few[7:], got[7:])
     # lengths that are nothing, or more than the table holds
     none = int4_tree_attention(**dict(more, lengths=i32([-3, 24])))
     assert (none[:7] == 0).all() and torch.equal(none[7:-2], got[7:-2])
@@ -750,3 +750,67 @@ def test_values_past_the_ends_of_fp16_mix(nodes):
     (kd, ks), (vd, vs) = stored(k), stored(v)
     out, bound = ref.tree_attention(q.astype(np.float64), kd, vd, np.tri(nodes, m, 70, dtype=bool), D ** -0.5, ks, vs)
     within(int4_tree_attention(torch.from_numpy(q).cuda(), pool, table, i32([m]), i32([0, nodes])), out, bound)
+
+
+def test_pages_past_32_bits_of_bytes():
+    """A pool of more than 4 GB, its last pages in use: appended, attended, read back and moved where they are."""
+    heads, page, count = 8, 64, 56000
+    pool = torch.zeros(count, heads, page * 160, dtype=torch.uint8, device="cuda")
+    assert pool.numel() > 1 << 32
+    table, small = i32([[count - 1, count - 3], [count - 2, 5]]), i32([[0, 1], [2, 3]])
+    other = empty_pages(4, heads, page)
+    rng = np.random.default_rng(6)
+    n, starts, offsets = 70, i32([10, 40]), i32([0, 60, 70])
+    q, k, v = (torch.from_numpy(rng.standard_normal((n, h, D)).astype(np.float16)).cuda() for h in (16, heads, heads))
+    cos, sin = (torch.from_numpy(x).cuda() for x in tables(200, 128))
+    got = []
+    for p, t in ((pool, table), (other, small)):
+        turned = int4_append_rope(p, t, starts, q, k, v, cos, sin, offsets)
+        out = int4_tree_attention(turned, p, t, i32([70, 50]), offsets)
+        int4_keep(p, t, starts, i32([[0, 3, 59], [2, 9, -1]]), i32([3, 2]))
+        got.append([turned, out, *int4_gather(p, t, starts, offsets, n)])
+    for a, b in zip(*got):
+        assert torch.equal(a, b)
+    assert not pool[6: count - 3].any()
+
+
+def test_logits_past_32_bits_of_elements():
+    n, vocab = 17000, 128256
+    logits = torch.full((n, vocab), -5.0, dtype=torch.float16, device="cuda")
+    assert logits.numel() > 1 << 31
+    logits[n - 2, 77], logits[n - 1, vocab - 1] = 9.0, 8.0
+    tokens = torch.zeros(n, dtype=torch.int64, device="cuda")
+    tokens[n - 1] = 77
+    parents, offsets = i32([-1] * (n - 1) + [0]), i32([0, n - 2, n])
+    u = torch.zeros(n, device="cuda")
+    for args in (dict(temperature=0), dict(accept=u, sample=torch.tensor([0.5, 0.9999999], device="cuda"))):
+        path, counts, token = verify_drafts(logits, tokens, parents, offsets, **args)
+        assert path[1, :3].tolist() == [0, 1, -1] and counts[1] == 2 and token[1] == vocab - 1
+
+
+def test_calls_on_two_streams_at_once():
+    """Calls that overlap share nothing: each stream's results are those of a call alone."""
+    cases = [attention_case(s, [900, 333], [40, 7], 2, 4, 64)[0] for s in (1, 2)]
+    new = [12, 12, 12]
+    checks = [verify_case(s, new, 20011, 1.0, True)[0] for s in (3, 4)]
+    alone = [(int4_tree_attention(**a), verify_drafts(**c)) for a, c in zip(cases, checks)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    both = [[], []]
+    for _ in range(5):
+        for i, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                both[i].append((int4_tree_attention(**cases[i]), verify_drafts(**checks[i])))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for out, found in both[i]:
+            assert torch.equal(out, alone[i][0]) and all(torch.equal(a, b) for a, b in zip(found, alone[i][1]))
+
+
+def test_results_do_not_change_from_run_to_run():
+    args, _, _ = attention_case(12, [3000, 100, 7], [33, 64, 2], 2, 4, 64)
+    check = verify_case(5, [30, 30], 9001, 1.0, True)[0]
+    first, found = int4_tree_attention(**args), verify_drafts(**check)
+    for _ in range(5):
+        assert torch.equal(first, int4_tree_attention(**args))
+        assert all(torch.equal(a, b) for a, b in zip(found, verify_drafts(**check)))

@@ -168,6 +168,10 @@ __device__ __forceinline__ double wave_scan_double(double v, int lane) {
 
 // Each row's segments: the largest logit and the sum of exp2((x - largest) c) in 64 bits, or where the largest is.  A thread
 // keeps its own maximum and brings its sum down when that moves; PIECES of them are under way at once.
+//
+// Bound: greedy by memory (558 rows of 128256: 32 us, 4.5 TB/s), else by the 64-bit exponentials (192 rows of 32003: 10 us, where
+// the bytes alone would take 2.6; 14 with a branch per element and the series in 64 bits throughout).  In 32 bits the sums would turn a
+// sampled token now and then: a token's share of a wide vocabulary is 1e-5 and less.
 template <class T, bool GREEDY, int PIECES>
 __global__ void __launch_bounds__(kStatThreads) verify_stat_kernel(VerifyArgs A) {
     __shared__ float s_most[kStatThreads / kWave];
@@ -263,6 +267,9 @@ __device__ __forceinline__ double less(double w, double scale, float q) {
 // segments.  The token at the end costs a pass over one segment.  A draft that was turned down costs, with `draft`, a pass
 // over its row and the target's: the first one's is left to verify_rest_kernel, which has a workgroup per segment, and the walk
 // goes on in a second launch (RESUME); any further ones (siblings that were drawn) are done by the workgroup alone.
+//
+// Bound: trips to memory and barriers (8 nodes 8 us, 24 greedy trees of up to 64 nodes 6).  The pass over a row by the walk's own
+// workgroup made 32 chains of a vocabulary of 32003 55 us, where the four kernels now take 35.
 template <class T, bool GREEDY, bool RESUME>
 __global__ void __launch_bounds__(walk_threads(GREEDY)) verify_walk_kernel(VerifyArgs A) {
     constexpr int kWalkThreads = walk_threads(GREEDY), kWalkWaves = kWalkThreads / kWave;

@@ -24,13 +24,14 @@
 // 219 / 198.
 //
 // Bound: few rows by memory's latency and the vector ALU together (32 trees of up to 16 nodes after 2000 to 8192 tokens: 76 us and
-// 10 for the merge; 370 vector instructions per block and 32 rows, the ALU busy half of the time); many rows by the vector ALU (32
-// trees of 64 nodes after 8192 tokens: 380 us, 720 TFLOP/s; 140 vector instructions, 16 of them exponentials, and 36
-// matrix instructions per 32 rows and block, whose issue takes nine tenths of the time in which a workgroup multiplies, and that is
-// three quarters of all).
+// 10 for the merge; 370 vector instructions per block and 32 rows, the ALU issuing in half of the cycles); many rows by the vector
+// ALU and the matrix cores one after the other (32 trees of 64 nodes after 8192 tokens: 352 us, 780 TFLOP/s; 190 vector instructions,
+// 16 of them exponentials, and 36 products per block and 32 rows: the ALU issues in 58% of the cycles, the matrix cores are busy in
+// 34%, and little of that is at the same time).
 // What made no difference there: the order of reads, products and sums in a wave by hand, one barrier per block or per two,
-// a third buffer with the barrier before the products.  One tile of rows a wave and four waves a SIMD (registers spill) 469 us
-// instead of 434, four waves and half the rows a workgroup 468, two 580.  A wave's priority while it multiplies: 410 to 393.
+// a third buffer with the barrier before the products.  One tile of rows a wave and four waves a SIMD (registers spill) took 469 us
+// where this took 434, four waves and half the rows a workgroup 468, two 580; a wave's priority while it multiplies brought 410 to
+// 393, the lowest values' share in two fp16 parts instead of one fp32 product 388 to 362.
 #include "int4.h"
 #include "reskv_drafts.h"
 

@@ -68,7 +68,7 @@ struct VerifyArgs {
     int N, segments, pieces;  // pieces of a segment
 };
 
-// 2^y for finite y <= 0, to 2^-38 of itself: the series of 2^f for a fraction f of at most a half (its coefficients are ln(2)^k /
+// 2^y for -2000 <= y <= 0, to 2^-38 of itself: the series of 2^f for a fraction f of at most a half (its coefficients are ln(2)^k /
 // k!), from the fifth power on, where it is below 2^-14, in 32 bits.  A NaN goes on.
 __device__ __forceinline__ double exp2_of(double y) {
     constexpr double l = 0.69314718055994530942, l2 = l * l, l4 = l2 * l2, l8 = l4 * l4;
@@ -87,10 +87,10 @@ __device__ __forceinline__ double exp2_of(double y) {
     p = __builtin_fma(p, f, 1.0);
     return __builtin_ldexp(p, (int)whole);  // 0 where it is below 2^-1074
 }
-// The weight of a logit x against the largest: 0 for minus infinity, without a branch.
+// The weight of a logit x against the largest, without a branch: 0 for minus infinity, also where there is nothing else.
 __device__ __forceinline__ double weight_of(float x, float most, double c) {
-    const double y = ((double)x - (double)most) * c;
-    return exp2_of(x == -INFINITY ? -2000.0 : y);
+    const double y = ((double)x - (double)fmaxf(most, -__FLT_MAX__)) * c;
+    return exp2_of(y < -2000.0 ? -2000.0 : y);
 }
 
 template <class T>

@@ -814,3 +814,36 @@ def test_results_do_not_change_from_run_to_run():
     for _ in range(5):
         assert torch.equal(first, int4_tree_attention(**args))
         assert all(torch.equal(a, b) for a, b in zip(found, verify_drafts(**check)))
+
+
+def test_rows_past_the_last_node():
+    """A sequence of more than 64 rows: its first 64 are nodes, the rest get zeros, and the tokens keep their places."""
+    contexts, n = 40, 70
+    args, _, _ = attention_case(13, [contexts], [64], 1, 2, 32, chain=True)
+    q = torch.cat([args["q"], args["q"][:6]])
+    table, pages = i32([[3, 0, 2, 1]]), empty_pages(4, 1, 32)
+    rng = np.random.default_rng(1)
+    k, v = (torch.from_numpy(rng.standard_normal((contexts + n, 1, D)).astype(np.float16)).cuda() for _ in range(2))
+    int4_append(pages, table, i32([0]), k, v, i32([0, contexts + n]))
+    got = int4_tree_attention(q, pages, table, i32([contexts + n]), i32([0, n]))
+    want = int4_tree_attention(q[:64], pages, table, i32([contexts + 64]), i32([0, 64]))
+    assert torch.equal(got[:64], want) and (got[64:] == 0).all()
+    parents = [-1] + list(range(n - 1))
+    seen, positions = draft_tree(i32(parents), i32([0, n]))
+    assert seen[:64].tolist() == signed(ref.masks(parents[:64])).tolist() and (seen[64:] == 0).all() and (positions[64:] == 0).all()
+    logits = torch.zeros(n, 33, dtype=torch.float16, device="cuda")
+    logits[:, 5] = 1.0
+    tokens = torch.full((n,), 5, dtype=torch.int64, device="cuda")
+    path, counts, token = verify_drafts(logits, tokens, i32(parents), i32([0, n]), temperature=0)
+    assert path[0].tolist() == list(range(64)) and counts.tolist() == [64] and token.tolist() == [5]
+    u = torch.zeros(n, device="cuda")
+    path, counts, token = verify_drafts(logits, tokens, i32(parents), i32([0, n]), u, u[:1])
+    assert path[0].tolist() == list(range(64)) and counts.tolist() == [64] and token.tolist() == [0]
+
+
+def test_nothing_but_rows_without_tokens():
+    """Lengths that the nodes themselves pass: node i is token length - n + i, and what lies before token 0 is not there."""
+    args, _, _ = attention_case(2, [0], [9], 1, 4, 32, chain=True)
+    got = int4_tree_attention(**dict(args, lengths=i32([4])))  # nodes 5 .. 8 are tokens 0 .. 3
+    few = int4_tree_attention(**dict(args, q=args["q"][5:].contiguous(), lengths=i32([4]), offsets=i32([0, 4])))
+    assert (got[:5] == 0).all() and torch.equal(got[5:], few)

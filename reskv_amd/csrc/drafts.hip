@@ -585,15 +585,17 @@ __global__ void __launch_bounds__(kStatThreads) verify_rest_kernel(VerifyArgs A)
     if (tid == 0) A.rest[(long)s * A.segments + segment] = (s_sum[0] + s_sum[1]) + (s_sum[2] + s_sum[3]);
 }
 
-// Elements of a segment: 8192, less while the rows are few, more where a row would have too many segments.
+// Elements of a segment: 2048, up to 8192 while there are rows enough, more where a row would have more segments than lanes.  A row's
+// first and last piece may hold one element each, so that V elements lie in up to (V + 14) / 8 pieces.
 constexpr long kSegment = kStatThreads * kPiece;
+long segments_at(long size, long V) { return ((V + 2 * (kPiece - 1)) / kPiece + size / kPiece - 1) / (size / kPiece); }
 long segment_of(long N, long V) {
     long size = kSegment;
     while (size < 4 * kSegment && N * (V / (2 * size)) >= 1024) size *= 2;
-    while (V / size + 1 > kSegments) size *= 2;
+    while (segments_at(size, V) > kSegments) size *= 2;
     return size;
 }
-int segments_of(long N, long V) { return (int)((V / kPiece + 2 + segment_of(N, V) / kPiece - 1) / (segment_of(N, V) / kPiece)); }
+int segments_of(long N, long V) { return (int)segments_at(segment_of(N, V), V); }
 
 template <class T>
 int verify(const VerifyArgs& A, int S, bool greedy, hipStream_t stream) {
@@ -769,7 +771,8 @@ extern "C" int reskv_verify_drafts(const void* logits, int logits_fp32, int64_t 
     A.path = path;
     A.counts = counts;
     A.token = token;
-    A.segments = segments_of(N, V);
+    A.segments = segments_of(N, V);  // one per lane of the walk
+    RESKV_REQUIRE(A.segments <= kSegments, "a row has %d segments, more than %d", A.segments, kSegments);
     A.pieces = (int)(segment_of(N, V) / kPiece);
     A.sum = (double*)workspace;
     A.most = (float*)(A.sum + N * A.segments);

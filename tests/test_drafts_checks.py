@@ -279,3 +279,14 @@ def test_no_gradient_is_recorded(library):
     wide = torch.zeros(6, 4, 256, **f16, requires_grad=True)[..., ::2]  # copied first
     assert not append(q=wide).requires_grad and not attend(q=wide).requires_grad
     verify(logits=torch.zeros(6, 50, requires_grad=True))
+
+
+@pytest.mark.parametrize("rows", [1, 7, 33, 34, 100, 558, 1000, 5000])
+def test_a_row_has_a_segment_for_every_lane_at_most(rows):
+    """The walk of verify_drafts takes a row's segments one per lane of a wave: 64, whatever the vocabulary is.  The workspace
+    holds 16 bytes per row and segment, 8 per sequence and segment, and 24 per sequence."""
+    size = _lib.lib().reskv_verify_workspace_bytes
+    around = [(64 << k) + i for k in range(10, 23) for i in range(-20, 21)] + [(1 << k) + i for k in range(21) for i in range(-9, 10)]
+    for vocab in {v for v in around if v > 0} | set(range(1, 200000, 97)):
+        segments = (size(3, rows, vocab) - 3 * 24) / (16 * rows + 3 * 8)
+        assert segments == int(segments) and 1 <= segments <= 64, vocab

@@ -788,6 +788,37 @@ def test_logits_past_32_bits_of_elements():
         assert path[1, :3].tolist() == [0, 1, -1] and counts[1] == 2 and token[1] == vocab - 1
 
 
+@pytest.mark.parametrize("vocab", [2041, 2048, 2049, 16383, 131058, 131064, 131071, 131072, 262143])
+@pytest.mark.parametrize("drawn", [False, True])
+@pytest.mark.parametrize("fp32", [False, True])
+def test_verify_at_the_ends_of_segments(vocab, drawn, fp32):
+    """The probability lies on a row's first and last tokens and on both sides of multiples of 2048, in rows at every place relative
+    to 16 bytes; siblings are turned down there.  Every token at the end of a row may be the largest."""
+    for padding in (0, 1):
+        rng = np.random.default_rng(1000 * padding + 2 * drawn + fp32)
+        new = [4, 5]
+        args, (logits, tokens, parents, accept, sample, q) = verify_case(vocab + padding, new, vocab, 1.0, drawn, fp32, padding=padding)
+        at = 2048 * rng.integers(1, vocab // 2048 + 2, 4)[:, None] + np.arange(-8, 3)
+        at = np.unique(np.concatenate([at.reshape(-1), np.arange(4), vocab - 1 - np.arange(9)]))
+        at = at[(at >= 0) & (at < vocab)]
+        logits[:, at] = (np.log(vocab) + 6 + rng.standard_normal((sum(new), at.size))).astype(logits.dtype)
+        share = np.mean([ref.softmax(row, 1.0)[at].sum() for row in logits])
+        assert share > 0.5
+        tokens[:] = rng.choice(at, sum(new))
+        if drawn:  # half of each draft's distribution on these tokens, the other as it was
+            q *= 0.5
+            q[:, at] += (0.5 * rng.dirichlet(np.ones(at.size), sum(new))).astype(np.float32)
+            args["draft"].copy_(torch.from_numpy(q))
+        args["logits"].copy_(torch.from_numpy(logits))
+        args["tokens"].copy_(torch.from_numpy(tokens))
+        check_verify(args, (logits, tokens, parents, accept, sample, q), new)
+        logits[np.arange(sum(new)), vocab - 1 - np.arange(sum(new)) % 9] = 100.0
+        args["logits"].copy_(torch.from_numpy(logits))
+        tokens[:] = np.argmax(logits, axis=1)[np.maximum(parents, 0) + np.repeat(sums(new)[:-1], new)]
+        args["tokens"].copy_(torch.from_numpy(tokens))
+        check_verify({**args, "temperature": 0.0}, (logits, tokens, parents, accept, sample, q), new)
+
+
 def test_calls_on_two_streams_at_once():
     """Calls that overlap share nothing: each stream's results are those of a call alone."""
     cases = [attention_case(s, [900, 333], [40, 7], 2, 4, 64)[0] for s in (1, 2)]

@@ -500,6 +500,11 @@ class Int4Cache:
         _require(all(0 <= k <= c for k, c in zip(kept, self._counts)), "a row keeps between none and all of the tokens reserved last")
         _require(path.dim() == 2 and max(kept) <= path.shape[1], "path must list every token that is kept")
         int4_keep(self.pool, self.table, self.starts, path, counts)
+        self._cut(kept)
+        return kept
+
+    def _cut(self, kept):
+        """Of the tokens reserved last, row s has its first ``kept[s]``; pages behind them are free."""
         changed = []
         for s, (k, c) in enumerate(zip(kept, self._counts)):
             self._lengths[s] += k - c
@@ -511,7 +516,6 @@ class Int4Cache:
         self._counts = kept
         self._publish(changed)
         self._publish_lengths()
-        return kept
 
     def gather(self, layer, *, reserved=True):
         """(k, v, offsets): the stored values of all tokens, packed (``int4_gather``), as

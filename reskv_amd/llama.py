@@ -592,11 +592,27 @@ class GreedyDecoder:
             return self._nodes(torch.cat([self.tok[:, None], drafts], dim=1), parents, temperature, accept, sample, draft, None)
 
     def _nodes(self, ids, parents, temperature, accept, sample, draft, events):
-        s, dev = self.model.shape, self.model.device
         n = ids.shape[1]
         if max(self.pages._lengths) + n > self.max_pos:
             raise RuntimeError("decoder capacity exhausted")
         self.pages.reserve(n)
+        try:
+            path, counts, token, out = self._checked(ids, parents, temperature, accept, sample, draft, events)
+            x = self.model.embed[token]
+            kept = self.pages.keep(path, counts)
+        except BaseException:  # the cache is what it was: the next step must not attend tokens that nobody accepted
+            self.pages._cut([0] * self.batch)
+            raise
+        self.tok.copy_(token)
+        self.x.copy_(x)
+        self.pos = max(self.pages._lengths)
+        return out, kept
+
+    def _checked(self, ids, parents, temperature, accept, sample, draft, events):
+        """The nodes' way through the model and their verification, in the tokens that are reserved for them: ``verify_drafts``'
+        results and the new tokens."""
+        s, dev = self.model.shape, self.model.device
+        n = ids.shape[1]
         offsets = torch.arange(0, (self.batch + 1) * n, n, dtype=torch.int32, device=dev)
         above = torch.tensor([-1, *parents] * self.batch, dtype=torch.int32).to(dev)
         seen, positions = draft_tree(above, offsets, self.pages.starts)
@@ -622,15 +638,9 @@ class GreedyDecoder:
                                             None if sample is None else sample.contiguous(),
                                             draft=None if draft is None else draft.flatten(0, 1), temperature=temperature)
         if bool((token < 0).any()):
-            self.pages.keep(path, torch.zeros_like(counts))
             raise RuntimeError("the model's logits hold a NaN or an infinity")
-        kept = self.pages.keep(path, counts)
-        self.tok.copy_(token)
-        self.x.copy_(self.model.embed[self.tok])
-        self.pos = max(self.pages._lengths)
         # the accepted drafts are the path's nodes behind the root
         place = torch.arange(1, n + 1, device=dev)
         accepted = torch.gather(ids, 1, path[:, 1: n].clamp(min=0).long())
         out = torch.cat([accepted, token[:, None]], dim=1)
-        out = torch.where(place == counts[:, None], token[:, None], torch.where(place < counts[:, None], out, -1))
-        return out, kept
+        return path, counts, token, torch.where(place == counts[:, None], token[:, None], torch.where(place < counts[:, None], out, -1))

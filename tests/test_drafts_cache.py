@@ -1,9 +1,11 @@
 """Int4Cache.keep and GreedyDecoder.step_drafts on the host: lengths, pages and refusals, with the launches left out."""
 
+import contextlib
+
 import pytest
 import torch
 
-from reskv_amd import int4
+from reskv_amd import int4, llama
 from reskv_amd.int4 import Int4Cache
 from reskv_amd.llama import GreedyDecoder, LlamaShape, RandomLlama
 
@@ -126,3 +128,29 @@ def test_drafts_need_the_paged_cache():
     dec = GreedyDecoder(RandomLlama(SHAPE, "cpu", seed=3), 2, 6, 4, "dense")
     with pytest.raises(ValueError, match="drafts need the 4-bit cache"):
         dec.step_drafts(torch.zeros(2, 3, dtype=torch.int64))
+
+
+@pytest.mark.parametrize("fails", ["draft_tree", "fused_rmsnorm", "verify_drafts"])
+def test_a_failed_step_leaves_nothing_reserved(monkeypatch, fails):
+    """Whatever raises between the reservation and the accepted tokens, rows and pages are what they were."""
+    def stop(*args, **kw):
+        raise MemoryError("no room")
+
+    nodes = 4 * 2  # what stands in for the GPU's operators returns tensors of their shapes
+    monkeypatch.setattr(llama, "_on_gpu", lambda *t: None)
+    monkeypatch.setattr(torch.cuda, "device", lambda d: contextlib.nullcontext())
+    monkeypatch.setattr(llama, "draft_tree", lambda *a: (torch.zeros(nodes, dtype=torch.int64), torch.zeros(nodes, dtype=torch.int32)))
+    monkeypatch.setattr(llama, "fused_rmsnorm", lambda x, *a: x)
+    monkeypatch.setattr(llama, "fused_silu_mul", lambda x, out: out.zero_())
+    monkeypatch.setattr(Int4Cache, "append_rope", lambda self, li, q, *a, **kw: q)
+    monkeypatch.setattr(Int4Cache, "attend_tree", lambda self, li, q, *a, **kw: q.contiguous())
+    monkeypatch.setattr(llama, fails, stop)
+    decoder = GreedyDecoder(RandomLlama(SHAPE, "cpu", seed=3), 2, 6, 140, "int4")
+    pages = decoder.pages
+    pages.reserve([5, 62])  # the second row's nodes need another page
+    free, state = pages.free_pages, (pages.lengths.tolist(), pages.table.tolist(), decoder.tok.tolist(), decoder.pos)
+    for _ in range(2):
+        with pytest.raises(MemoryError, match="no room"):
+            decoder.step_drafts(torch.zeros(2, 3, dtype=torch.int64))
+        assert (pages.lengths.tolist(), pages.table.tolist(), decoder.tok.tolist(), decoder.pos) == state
+        assert pages.free_pages == free and pages.starts.tolist() == [5, 62] and [pages.get_seq_length(s) for s in range(2)] == [5, 62]

@@ -3,6 +3,7 @@
 import pytest
 import torch
 
+from reskv_amd import llama
 from reskv_amd.llama import GreedyDecoder, LlamaShape, RandomLlama
 
 pytestmark = pytest.mark.gpu
@@ -114,3 +115,21 @@ def test_capacity(setting, plain):
     assert counts == [4, 4, 4] and dec.pos == 49
     with pytest.raises(RuntimeError, match="capacity exhausted"):
         dec.step()
+
+
+def test_a_failed_step_changes_nothing(setting, plain, monkeypatch):
+    """Drafts that a failed step has appended are not there for the next one, captured (rows of one length) or not."""
+    dec = start(setting)
+    for uneven in (False, True):
+        if uneven:
+            drafts = plain[:, 2:5].clone()
+            drafts[1] = -1
+            assert dec.step_drafts(drafts)[1] == [4, 1, 4]
+        have = [n - 41 + 1 for n in dec.pages.lengths.tolist()]
+        with monkeypatch.context() as m:
+            m.setattr(llama, "verify_drafts", lambda *a, **kw: 1 / 0)
+            with pytest.raises(ZeroDivisionError):
+                dec.step_drafts(torch.zeros(3, 5, dtype=torch.int64, device="cuda"))
+        assert [n - 41 + 1 for n in dec.pages.lengths.tolist()] == have and dec.pages.starts.tolist() == dec.pages.lengths.tolist()
+        step = dec.step()
+        assert [int(step[s]) for s in range(3)] == [int(plain[s, h]) for s, h in enumerate(have)]

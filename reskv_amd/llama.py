@@ -588,6 +588,14 @@ class GreedyDecoder:
         _need(temperature == 0.0 or 1e-30 <= temperature < math.inf, "temperature must be 0, or 1e-30 and more")
         _need(temperature == 0.0 or (accept is not None and sample is not None), "sampling needs random numbers")
         _on_gpu(drafts, accept, sample, draft)
+        if temperature == 0.0:
+            accept = sample = draft = None
+        else:
+            accept, sample = accept.contiguous().view(-1), sample.contiguous()
+        if draft is not None:
+            draft = draft.flatten(0, 1)
+            if draft.stride(1) != 1 or draft.stride(0) < draft.shape[1]:  # verify_drafts takes rows, apart from each other
+                draft = draft.contiguous()
         with torch.cuda.device(self.x.device):
             return self._nodes(torch.cat([self.tok[:, None], drafts], dim=1), parents, temperature, accept, sample, draft, None)
 
@@ -634,9 +642,7 @@ class GreedyDecoder:
             fused_rmsnorm(x, p["n2"], s.rms_eps, h)
             x.addmm_(fused_silu_mul(F.linear(h, p["wgu"]), act), p["wd"].t())
         logits = F.linear(fused_rmsnorm(x, self.model.norm, s.rms_eps, h), self.model.lm_head)
-        path, counts, token = verify_drafts(logits, ids.reshape(-1), above, offsets, None if accept is None else accept.reshape(-1),
-                                            None if sample is None else sample.contiguous(),
-                                            draft=None if draft is None else draft.flatten(0, 1), temperature=temperature)
+        path, counts, token = verify_drafts(logits, ids.reshape(-1), above, offsets, accept, sample, draft=draft, temperature=temperature)
         if bool((token < 0).any()):
             raise RuntimeError("the model's logits hold a NaN or an infinity")
         # the accepted drafts are the path's nodes behind the root

@@ -133,3 +133,22 @@ def test_a_failed_step_changes_nothing(setting, plain, monkeypatch):
         assert [n - 41 + 1 for n in dec.pages.lengths.tolist()] == have and dec.pages.starts.tolist() == dec.pages.lengths.tolist()
         step = dec.step()
         assert [int(step[s]) for s in range(3)] == [int(plain[s, h]) for s, h in enumerate(have)]
+
+
+def test_random_numbers_and_distributions_of_any_strides(setting):
+    """accept, sample and draft as views: the results are those of contiguous tensors."""
+    gen = torch.Generator("cuda").manual_seed(2)
+    accept, sample = torch.rand(3, 4, 2, device="cuda", generator=gen), torch.rand(3, 2, device="cuda", generator=gen)
+    q = torch.softmax(torch.randn(3, 4, TINY.vocab, 2, device="cuda", generator=gen), dim=2)
+    one = torch.softmax(torch.randn(TINY.vocab, device="cuda", generator=gen), dim=0)
+    wide = torch.zeros(3, 4, TINY.vocab + 5, device="cuda")
+    wide[..., :TINY.vocab] = q[..., 0]
+    drafts = torch.randint(TINY.vocab, (3, 3), device="cuda", generator=gen)
+    for draft in (q[..., 0], one.expand(3, 4, TINY.vocab), wide[..., :TINY.vocab], q[..., 1].transpose(0, 1).contiguous().transpose(0, 1), None):
+        runs = []
+        for same in (lambda t: t, lambda t: t.contiguous()):
+            dec = start(setting)
+            for _ in range(2):
+                runs.append(dec.step_drafts(drafts, temperature=5.0, accept=same(accept[..., 0]), sample=same(sample[:, 0]),
+                                            draft=None if draft is None else same(draft)))
+        assert all(torch.equal(a[0], b[0]) and a[1] == b[1] for a, b in zip(runs[:2], runs[2:]))

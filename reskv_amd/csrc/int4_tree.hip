@@ -871,8 +871,17 @@ extern "C" int reskv_int4_tree_attention(const void* q, const void* pages, int64
     if (max_length > most) max_length = most;
     const int G = Hq / Hk;
     // units and rows are counted in 32 bits; the last wave's run may end behind the last unit
-    RESKV_REQUIRE(most_units(S, Hk, G, max_length, max_nodes) < (1L << 30) && G < (1 << 20) && merge_items(N, G, S, 16) * Hk < kLaunchThreads / kThreads,
+    RESKV_REQUIRE(most_units(S, Hk, G, max_length, max_nodes) < (1L << 30) && G < (1 << 20),
                   "too many tokens: blocks of %d x KV heads x chunks of rows must stay below 2^30", kBlock);
+    // The fewer the rows, the more threads of the merge take each one's records, which come from the whole chip then: 8 nodes of 32 heads
+    // after 20000 tokens (256 records a row) 32 us for both kernels with 16 sets and 46 with four, five trees of 1 to 61 nodes 129 with
+    // four and 139 with 16.
+    const long rows_all = (long)N * Hq;
+    const auto merge = rows_all <= 1024 ? tree_merge_kernel<4, 16> : rows_all <= 8192 ? tree_merge_kernel<16, 4> : tree_merge_kernel<16, 1>;
+    const int merge_threads = rows_all <= 8192 ? 1024 : 256;
+    const long merge_groups = merge_items(N, G, S, rows_all <= 1024 ? 4 : 16) * Hk;
+    RESKV_REQUIRE(merge_groups < kLaunchThreads / merge_threads, "too many tokens: %ld nodes of %d sequences for %d KV heads pass a launch's 2^32 threads",
+                  (long)N, S, Hk);
     RESKV_REQUIRE(workspace && workspace_bytes >= reskv_int4_tree_workspace_bytes(S, N, Hq, Hk, max_length, max_nodes), "the workspace is too small");
     const int rows = chunk_rows(G, max_nodes);
     TreeArgs A{};
@@ -897,12 +906,6 @@ extern "C" int reskv_int4_tree_attention(const void* q, const void* pages, int64
     const auto kernel = rows == 16 ? tree_alone_kernel<1> : rows == 32 ? tree_alone_kernel<2> : rows == 128 ? tree_together_kernel<4> : tree_together_kernel<8>;
     hipLaunchKernelGGL(kernel, dim3((unsigned)A.groups), dim3(kWave * waves_of(rows)), 0, (hipStream_t)stream, A);
     if (reskv_host::check_launch("tree_kernel")) return 1;
-    // The fewer the rows, the more threads take each one's records, which come from the whole chip then: 8 nodes of 32 heads after
-    // 20000 tokens (256 records a row) 32 us for both kernels with 16 sets and 46 with four, five trees of 1 to 61 nodes 129 with
-    // four and 139 with 16.
-    const long rows_all = (long)N * Hq;
-    const auto merge = rows_all <= 1024 ? tree_merge_kernel<4, 16> : rows_all <= 8192 ? tree_merge_kernel<16, 4> : tree_merge_kernel<16, 1>;
-    hipLaunchKernelGGL(merge, dim3((unsigned)(merge_items(N, G, S, rows_all <= 1024 ? 4 : 16) * Hk)), dim3(rows_all <= 8192 ? 1024 : 256), 0,
-                       (hipStream_t)stream, A);
+    hipLaunchKernelGGL(merge, dim3((unsigned)merge_groups), dim3((unsigned)merge_threads), 0, (hipStream_t)stream, A);
     return reskv_host::check_launch("tree_merge_kernel");
 }

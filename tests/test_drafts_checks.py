@@ -290,3 +290,19 @@ def test_a_row_has_a_segment_for_every_lane_at_most(rows):
     for vocab in {v for v in around if v > 0} | set(range(1, 200000, 97)):
         segments = (size(3, rows, vocab) - 3 * 24) / (16 * rows + 3 * 8)
         assert segments == int(segments) and 1 <= segments <= 64, vocab
+
+
+@pytest.mark.parametrize("sequences,rows,heads,per_head,refused", [
+    (1 << 21, 4, 4, 2, True),        # few rows: 1024 threads for every four of them, or every sequence
+    ((1 << 21) - 4, 4, 4, 2, False),
+    (1 << 21, 2048, 4, 2, True),     # 1024 threads for every 16 rows
+    (1 << 22, 257, 4, 4, True),
+    (1 << 22, 8192, 4, 2, False),    # 256 threads
+    (1 << 23, 8192, 4, 2, True),
+])
+def test_a_launch_of_the_merge_has_fewer_than_2_to_the_32_threads(sequences, rows, heads, per_head, refused):
+    """Looked at before anything is launched; a workspace that is too small stops the calls that pass."""
+    p = ctypes.c_void_p(16)
+    said = err(_lib.lib().reskv_int4_tree_attention(p, p, 3, 64, p, 1, p, p, None, sequences, rows, heads, heads // per_head, 1.0, 64, 1, 1, p, p,
+                                                    0, None))
+    assert ("pass a launch's 2^32 threads" if refused else "workspace is too small") in said

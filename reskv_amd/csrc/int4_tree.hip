@@ -4,9 +4,9 @@
 // tiles.  For 32 tokens and each of the four groups g of 32 channels, on v_mfma_f32_16x16x32_f16,
 //   S_g^T [token][row] = K_g Q_g^T, codes as fp16 by masking alone (see int4.hip), and
 //   S^T = low q-sum^T + sum_g scale[token, g] S_g^T,
-// the first term on v_mfma_f32_16x16x16_f16 (its inner dimension is the four groups, with q-sum in two fp16 parts, to 2^-25 of a sum
-// of at most 2^-4), the others as one mixed fp32 / fp16 multiply-add per score and group, so that keys are not rounded.  The rows of the K operand are taken in an order of
-// tokens that leaves lane (quarter q, row n) with the scores of the tokens 8 q .. 8 q + 7: the order in which
+// the first term on v_mfma_f32_16x16x16_f16 (its inner dimension is the four groups, with q-sum in three fp16 parts: see lowest), the
+// others as one mixed fp32 / fp16 multiply-add per score and group, so that keys are not rounded.  The rows of the K operand are taken
+// in an order of tokens that leaves lane (quarter q, row n) with the scores of the tokens 8 q .. 8 q + 7: the order in which
 // V's codes lie in a lane.  Softmax and its statistics are then a lane's own but for the maximum, and the weights are the B
 // operand of
 //   O^T [channel][row] += V^T P^T
@@ -134,8 +134,16 @@ __device__ __forceinline__ uint32_t pair_max(uint32_t a, uint32_t b) {
 // Scales of 2^12 and more, NaN and infinity among them: values may pass fp16's largest.
 __device__ __forceinline__ bool is_odd(uint32_t scales) { return (scales & 0xFFFFu) >= 0x6C00u || scales >= 0x6C000000u; }
 
-// The lowest value of a K scaling, twice.
-__device__ __forceinline__ uint32_t twice(uint32_t scaling) { return __builtin_amdgcn_perm(scaling, scaling, 0x03020302u); }
+// The lowest value of a K scaling against the parts of a sum of q: itself for the first two, 2^-10 of it for the third.  With q's
+// largest element at 2^14 and codes at 2^-24 a sum is at most 2^-4, and what its first two parts leave is up to 2^-25, fp16 numbers
+// having no smaller steps there than 2^-24.  2^10 times that is rounded to 2^-25 again, and the lowest value to 2^-25 or its eleven bits:
+// the share is off by at most 2^-25 of |lowest| and 2^-30, times the largest element of q, where an fp32 sum's own rounding is 2^-24 of it.
+constexpr float kThird = 1024.0f;
+__device__ __forceinline__ uint2 lowest(uint32_t scaling) {
+    const uint32_t low = __builtin_amdgcn_perm(scaling, scaling, 0x03020302u);
+    const half2_t third = {(_Float16)(1.0f / kThird), (_Float16)0.0f};
+    return make_uint2(low, __builtin_bit_cast(uint32_t, __builtin_bit_cast(half2_t, low) * third));
+}
 // Two results in fp16; one past fp16's largest is that largest, as a value may be (a NaN goes on).
 __device__ __forceinline__ float within(float x) { return x > 65504.0f ? 65504.0f : x < -65504.0f ? -65504.0f : x; }
 __device__ __forceinline__ uint32_t pack_results(float a, float b) { return pack_halves(within(a), within(b)); }
@@ -144,7 +152,7 @@ __device__ __forceinline__ uint32_t pack_results(float a, float b) { return pack
 template <int RT>
 struct RowState {
     half8_t q[RT][4];        // lane (row n, quarter): channels 32 g + 8 quarter + [0, 8) of each group
-    half4_t sum[RT];         // sum of group `quarter`'s channels, as two fp16 numbers
+    half4_t sum[RT];         // sum of group `quarter`'s channels, as three fp16 numbers
     float back[RT];          // what brings the row's scores back
     uint64_t sees[RT];       // the row's nodes
     float4_t acc[RT][8];     // channels 16 ct + 4 quarter + i of row n
@@ -189,8 +197,9 @@ struct RowState {
                 part[g] = swap_sum32(part[g], part[g]);
             }
             const float mine = (quarter == 0 ? part[0] : quarter == 1 ? part[1] : quarter == 2 ? part[2] : part[3]) * (up * 0x1p-24f);
-            const _Float16 high = (_Float16)mine, none = (_Float16)0.0f;  // (an infinity's rest is a NaN)
-            sum[rt] = half4_t{high, (_Float16)(mine - (float)high), none, none};
+            const _Float16 first = (_Float16)mine, second = (_Float16)(mine - (float)first);  // (an infinity's rest is a NaN)
+            const float rest = (mine - (float)first) - (float)second;
+            sum[rt] = half4_t{first, second, (_Float16)(rest * kThird), (_Float16)0.0f};
             back[rt] = A.c * (0x1p24f / up);
             sees[rt] = !real ? 0 : (A.seen ? A.seen[rows.first + node] : (2ull << node) - 1) & all;
             m[rt] = -__FLT_MAX__;
@@ -201,7 +210,7 @@ struct RowState {
     }
 
     // The weights of a block, as operands.  key(j, g): the K operand of tile j and group g; scale(g): the scales of the tokens 8
-    // quarter .. + 7; low(j): the lowest value of the lane's K row and group.  `valid` tokens are there, from `tree` on they
+    // quarter .. + 7; low(j): lowest() of the lane's K row and group.  `valid` tokens are there, from `tree` on they
     // are nodes; `visible` gets the tokens that a row sees where some do not.  before_softmax() comes behind the scores, between(rt, i)
     // in four places among the weights of the row tile behind rt.
     template <bool SHARED, class Key, class Scale, class Low, class Before, class Between>
@@ -218,7 +227,7 @@ struct RowState {
             scales[g] = __builtin_bit_cast(half8_t, scale(g));
         };
 #pragma unroll
-        for (int j = 0; j < 2; ++j) lows[j] = __builtin_bit_cast(half4_t, make_uint2(low(j), 0));
+        for (int j = 0; j < 2; ++j) lows[j] = __builtin_bit_cast(half4_t, low(j));
         read(0);
         read(1);
         float4_t d[2][2][RT];
@@ -490,7 +499,7 @@ __device__ __forceinline__ void work_alone(const TreeArgs& A, OneWave& L, int s,
         R.template weights<false>(p, visible, valid, tree, quarter,
                                   [&](int j, int g) __attribute__((always_inline)) { return operand(dword(x.k[j], g)); },
                                   [&](int g) __attribute__((always_inline)) { return reinterpret_cast<const uint4*>(L.scale)[4 * g + quarter]; },
-                                  [&](int j) __attribute__((always_inline)) { return twice(x.ks[j]); }, []() {}, [](int, int) {});
+                                  [&](int j) __attribute__((always_inline)) { return lowest(x.ks[j]); }, []() {}, [](int, int) {});
         auto value = [&](int ct) __attribute__((always_inline)) {
             const int of = 4 * (ct >> 1) + quarter;
             return values_of(M, dword(x.v[ct >> 2], ct & 3), reinterpret_cast<const uint4*>(L.vs)[of], reinterpret_cast<const uint4*>(L.vl)[of]);
@@ -529,7 +538,7 @@ __device__ __forceinline__ void work_alone(const TreeArgs& A, OneWave& L, int s,
 struct Operands {
     uint4 k[2][4][kWave], v[8][kWave];
     alignas(16) uint16_t scale[4 * kBlock];
-    uint32_t low[4 * kBlock];
+    uint2 low[4 * kBlock];
     uint32_t bad[4];  // tokens of a group whose values are no numbers, where nodes are
 };
 
@@ -592,7 +601,7 @@ __device__ __forceinline__ void work_together(const TreeArgs& A, Operands (*L)[k
             O.k[task >> 1][2 * (task & 1) + 1][lane] = __builtin_bit_cast(uint4, operand(x[i].k.y));
             if (lane < kBlock) {
                 O.scale[task * kBlock + lane] = (uint16_t)x[i].ks;
-                O.low[task * kBlock + lane] = twice(x[i].ks);
+                O.low[task * kBlock + lane] = lowest(x[i].ks);
             }
             uint32_t sc[4] = {x[i].vs.x, x[i].vs.y, x[i].vs.z, x[i].vs.w}, lo[4] = {x[i].vl.x, x[i].vl.y, x[i].vl.z, x[i].vl.w};
             if (valid < kBlock) {  // what lies behind the last token may be anything

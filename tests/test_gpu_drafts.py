@@ -373,6 +373,38 @@ def test_queries_and_keys_of_other_sizes(power):
     within(got, out, bound)
 
 
+@pytest.mark.parametrize("nodes", [2, 40])
+@pytest.mark.parametrize("power", [-9, 0, 15])
+def test_scores_of_keys_whose_groups_are_level(nodes, power):
+    """Every key's channels of a group are equal, so that scores are sums of q times lowest values alone, and two groups' sums of q cancel
+    but for a 2^-15 of them.
+
+    In fp32 a sum of q takes up to ten roundings (four elements that are not zero, the lanes' shares), the products of two groups
+    in three parts six, the scaling and the exponent two; a third part is off by 2^-25 of q's largest element and the lowest value: fewer
+    than 32 half steps of 2^-24 of the terms' sum, which a weight is off by twice.  The rest as in drafts_reference.tree_attention."""
+    rng = np.random.default_rng(100 + nodes + power)
+    m, heads = 40 + nodes, 4
+    sign = rng.choice([-1.0, 1.0], (m, 1, 1))
+    k = np.zeros((m, 1, D))
+    k[..., :64] = sign * 2.0 ** power * (1 + rng.integers(0, 900, (m, 1, 1)) / 1024)
+    v = (sign * (1 + 0.1 * rng.standard_normal((m, 1, D)))).astype(np.float16)
+    q = np.zeros((nodes, heads, D))
+    q[..., 0], q[..., 32] = 1.0, -1.0
+    for at in (1, 33):
+        q[..., at: at + 3] = rng.uniform(-1, 1, (nodes, heads, 3)) * 2.0 ** -15
+    q, k = (q * 2.0 ** min(15, 15 - power)).astype(np.float16), k.astype(np.float16)
+    pool, table = empty_pages(4, 1, 32), i32([[2, 0, 1, 3]])
+    int4_append(pool, table, i32([0]), torch.from_numpy(k).cuda(), torch.from_numpy(v).cuda(), i32([0, m]))
+    (kd, ks), (vd, vs) = stored(k), stored(v)
+    assert np.array_equal(kd, k)
+    visible = np.tri(nodes, m, 40, dtype=bool)
+    out, _ = ref.tree_attention(q.astype(np.float64), kd, vd, visible, D ** -0.5, ks, vs)
+    spread, _ = ref.tree_attention(q.astype(np.float64), kd, np.abs(vs), visible, D ** -0.5, ks, vs)
+    delta = 32 * 2.0 ** -24 * D ** -0.5 * np.abs(q.astype(np.float64)).sum(-1).max() * np.abs(kd).max()
+    bound = spread * (2 * 2.0 ** -11 + 2 * delta + 2.0 ** -20) * 1.01 + 2.0 ** -34 * vs.sum(0) + 2.0 ** -24 + 2.0 ** -11 * np.abs(out) * 1.01
+    within(int4_tree_attention(torch.from_numpy(q).cuda(), pool, table, i32([m]), i32([0, nodes])), out, bound)
+
+
 def test_long_context():
     """More blocks than waves, with a tree that is split over many of them; 64 bits on the GPU."""
     gen = torch.Generator("cuda").manual_seed(1)

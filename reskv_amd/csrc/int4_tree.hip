@@ -116,22 +116,20 @@ __device__ __forceinline__ half8_t values_of(const Masks& M, uint32_t d, const u
     return half8_t{r0[0], r0[1], r1[0], r1[1], r2[0], r2[1], r3[0], r3[1]};
 }
 
-// A value past fp16's largest, which code * scale + low can reach by the rounding of the scale, is that largest (a NaN
-// goes on).
-__device__ __forceinline__ half8_t within_fp16(half8_t v) {
-    const _Float16 top = (_Float16)65504.0f;
-    const half8_t most = {top, top, top, top, top, top, top, top};
-    return __builtin_elementwise_maximum(__builtin_elementwise_minimum(v, most), -most);
-}
-
 // Tokens t0 and t0 + 1 of a dword: the halves of those below `valid`.
 __device__ __forceinline__ uint32_t halves_below(int t0, int valid) { return (t0 < valid ? 0xFFFFu : 0u) | (t0 + 1 < valid ? 0xFFFF0000u : 0u); }
+// Half of two numbers in a dword.
+__device__ __forceinline__ uint32_t halves_of(uint32_t w) {
+    const half2_t half = {(_Float16)0.5f, (_Float16)0.5f};
+    return __builtin_bit_cast(uint32_t, __builtin_bit_cast(half2_t, w) * half);
+}
 // The larger of each of two numbers in a dword, not negative in fp16.
 __device__ __forceinline__ uint32_t pair_max(uint32_t a, uint32_t b) {
     typedef unsigned short ushort2_t __attribute__((ext_vector_type(2)));
     return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(ushort2_t, a), __builtin_bit_cast(ushort2_t, b)));
 }
-// Scales of 2^12 and more, NaN and infinity among them: values may pass fp16's largest.
+// Scales of 2^12 and more, NaN and infinity among them: values may pass fp16's largest, by the rounding of the scale.  Half of the
+// values are made then, and counted twice.
 __device__ __forceinline__ bool is_odd(uint32_t scales) { return (scales & 0xFFFFu) >= 0x6C00u || scales >= 0x6C000000u; }
 
 // The lowest value of a K scaling against the parts of a sum of q: itself for the first two, 2^-10 of it for the third.  With q's
@@ -484,10 +482,9 @@ __device__ __forceinline__ void work_alone(const TreeArgs& A, OneWave& L, int s,
             x.vs &= keep;
             x.vl &= keep;
         }
-        if (odd) {  // half of the values then, for twice the weights
-            const half2_t half = {(_Float16)0.5f, (_Float16)0.5f};
-            x.vs = __builtin_bit_cast(uint32_t, __builtin_bit_cast(half2_t, x.vs) * half);
-            x.vl = __builtin_bit_cast(uint32_t, __builtin_bit_cast(half2_t, x.vl) * half);
+        if (odd) {
+            x.vs = halves_of(x.vs);
+            x.vl = halves_of(x.vl);
         }
 #pragma unroll
         for (int j = 0; j < 2; ++j) L.scale[quarter * kBlock + token_of(n, j)] = (uint16_t)x.ks[j];
@@ -540,6 +537,8 @@ struct Operands {
     alignas(16) uint16_t scale[4 * kBlock];
     uint2 low[4 * kBlock];
     uint32_t bad[4];  // tokens of a group whose values are no numbers, where nodes are
+    int odd[4];       // groups whose values are halves, where they have the number of the step (its first block's, from 1)
+    int any_odd;      // of a step's first block: that number, where the step has any
 };
 
 // A wave's share of that work: pieces of K and V.
@@ -632,16 +631,24 @@ __device__ __forceinline__ void work_together(const TreeArgs& A, Operands (*L)[k
             const uint4 s4 = make_uint4(sc[0], sc[1], sc[2], sc[3]), l4 = make_uint4(lo[0], lo[1], lo[2], lo[3]);
             half8_t v0 = values_of(M, x[i].v.x, s4, l4), v1 = values_of(M, x[i].v.y, s4, l4);
             if (odd) {
-                v0 = within_fp16(v0);
-                v1 = within_fp16(v1);
+                const uint4 s2 = make_uint4(halves_of(sc[0]), halves_of(sc[1]), halves_of(sc[2]), halves_of(sc[3]));
+                const uint4 l2 = make_uint4(halves_of(lo[0]), halves_of(lo[1]), halves_of(lo[2]), halves_of(lo[3]));
+                v0 = values_of(M, x[i].v.x, s2, l2);
+                v1 = values_of(M, x[i].v.y, s2, l2);
+                if (lane == 0) O.odd[task] = O0->any_odd = blk0 + 1;
             }
             O.v[2 * task][lane] = __builtin_bit_cast(uint4, v0);
             O.v[2 * task + 1][lane] = __builtin_bit_cast(uint4, v1);
         }
     };
     uint32_t there = fetch(begin), there_next = 0;
+    if (threadIdx.x < 2 * kStep) {
+        Operands& O = L[threadIdx.x / kStep][threadIdx.x % kStep];
+        O.any_odd = O.odd[0] = O.odd[1] = O.odd[2] = O.odd[3] = 0;
+    }
     RowState<RT> R;
     R.start(A, rows, nodes, hk, r0, lane);
+    __syncthreads();
     stage(L[0], begin, there);
     if (begin + kStep < end) there_next = fetch(begin + kStep);
     __syncthreads();
@@ -649,11 +656,13 @@ __device__ __forceinline__ void work_together(const TreeArgs& A, Operands (*L)[k
     for (int blk = begin; blk < end; blk += kStep) {
         const Operands* const O = L[side];
         side ^= 1;
+        const int any_odd = O->any_odd;
         const uint32_t here = there;
         if (blk + kStep < end) stage(L[side], blk + kStep, there_next);
         there = there_next;
         if (blk + 2 * kStep < end) there_next = fetch(blk + 2 * kStep);
         if (here && active) {
+            const bool odd = __builtin_amdgcn_readfirstlane(any_odd) == blk + 1;
 #pragma unroll
             for (int b = 0; b < kStep; ++b) {
                 if (!(here >> b & 1)) continue;
@@ -678,8 +687,14 @@ __device__ __forceinline__ void work_together(const TreeArgs& A, Operands (*L)[k
 #pragma unroll
                 for (int ct = 0; ct < 8; ++ct) R.add_one(ct, RT - 1, v[ct], p);
                 __builtin_amdgcn_s_setprio(0);
-                if (tree < kBlock && (B.bad[0] | B.bad[1] | B.bad[2] | B.bad[3]) != 0)
-                    R.add_bad(visible, [&](int g) __attribute__((always_inline)) { return B.bad[g]; });
+                if (tree < kBlock || odd) {  // (rare)
+                    if (odd)  // the products again of values that are halves
+#pragma unroll
+                        for (int ct = 0; ct < 8; ++ct)
+                            if (__builtin_amdgcn_readfirstlane(B.odd[ct >> 1]) == blk + 1) R.add(ct, __builtin_bit_cast(half8_t, B.v[ct][lane]), p);
+                    if (tree < kBlock && (B.bad[0] | B.bad[1] | B.bad[2] | B.bad[3]) != 0)
+                        R.add_bad(visible, [&](int g) __attribute__((always_inline)) { return B.bad[g]; });
+                }
             }
         }
         __syncthreads();

@@ -784,6 +784,26 @@ def test_values_past_the_ends_of_fp16_mix(nodes):
     within(int4_tree_attention(torch.from_numpy(q).cuda(), pool, table, i32([m]), i32([0, nodes])), out, bound)
 
 
+@pytest.mark.parametrize("nodes,heads", [(1, 1), (2, 4), (9, 4), (24, 4), (40, 4)])
+def test_values_past_the_ends_of_fp16_do_not_depend_on_the_rows(nodes, heads):
+    """A step of 8736 (131008 / 15 in fp16) takes the largest code to 65536: two tokens of one weight at opposite ends have the average
+    16 in every channel, with every sum exact, however many rows there are; blocks before and behind have no such tokens."""
+    v = torch.full((110 + nodes, 1, D), 65504.0, dtype=torch.float16, device="cuda")
+    v[:, :, ::2] = -65504.0
+    v[33] = -v[33]
+    k = torch.zeros_like(v)
+    k[:32] = k[34:110] = -1.0
+    v[:32] = v[64:110] = 0.0
+    held = stored(v[32:34].cpu().numpy())[0]
+    assert (held.max(axis=-1) == 65536.0).all() and (held.mean(axis=0) == 16.0).all()
+    pool, table = empty_pages(5, 1, 32), i32([[2, 0, 1, 3, 4]])
+    int4_append(pool, table, i32([0]), k, v, i32([0, 110 + nodes]))
+    q = torch.full((nodes, heads, D), 8.0, dtype=torch.float16, device="cuda")  # the other tokens' weights are exp(-90): nothing
+    hidden = torch.zeros(nodes, dtype=torch.int64, device="cuda")
+    got = int4_tree_attention(q, pool, table, i32([110 + nodes]), i32([0, nodes]), hidden)
+    assert (got == 16.0).all()
+
+
 def test_pages_past_32_bits_of_bytes():
     """A pool of more than 4 GB, its last pages in use: appended, attended, read back and moved where they are."""
     heads, page, count = 8, 64, 56000

@@ -372,10 +372,10 @@ __global__ void __launch_bounds__(walk_threads(GREEDY)) verify_walk_kernel(Verif
         return w;
     };
     auto sum_segments = [&]() __attribute__((always_inline)) { return wave_sum_double(lane < A.segments ? s_segment[lane] : 0.0); };
-    // The segments' sums of r; returns their sum.
-    auto measure = [&]() __attribute__((always_inline)) {
+    // The sums of r of segments g0 .. g1 - 1; returns that of all.
+    auto measure = [&](int g0, int g1) __attribute__((always_inline)) {
         const Row<T> R(A, rows.first + here);
-        for (int g = 0; g < A.segments; ++g) {
+        for (int g = g0; g < g1; ++g) {
             const int last = min((g + 1) * A.pieces, R.pieces());
             double sum = 0.0;
             for (int p = g * A.pieces + tid; p < last; p += kWalkThreads) {
@@ -389,7 +389,7 @@ __global__ void __launch_bounds__(walk_threads(GREEDY)) verify_walk_kernel(Verif
             if (lane == 0) s_part[g][wave] = sum;
         }
         __syncthreads();
-        if (tid < A.segments) {
+        if (tid >= g0 && tid < g1) {
             double sum = 0.0;
 #pragma unroll
             for (int v = 0; v < kWalkWaves; ++v) sum += s_part[tid][v];
@@ -441,8 +441,8 @@ __global__ void __launch_bounds__(walk_threads(GREEDY)) verify_walk_kernel(Verif
         ++down;
         // without a distribution only one token goes; where that is nearly all, the rest is added up anew
         double rest = left - w;
-        if (A.draft || !(rest > kSmall * s_total[here])) {
-            rest = measure();
+        if (A.draft || !whole || !(rest > kSmall * s_total[here])) {
+            rest = measure(0, A.segments);
             whole = false;
         }
         if (rest > 0.0) {
@@ -465,21 +465,34 @@ __global__ void __launch_bounds__(walk_threads(GREEDY)) verify_walk_kernel(Verif
     const Row<T> R(A, rows.first + here);
     if (whole) {
         if ((A.draft && down > 0) || !(left > kSmall * s_total[here])) {
-            measure();
+            measure(0, A.segments);
         } else {
             // from the row's statistics, without the tokens turned down
             if (tid < A.segments) {
                 const long at = (long)(rows.first + here) * A.segments + tid;
                 const double sum = A.sum[at];
-                s_segment[tid] = sum == 0.0 ? 0.0 : sum * weight_of(A.most[at], s_most[here], A.c);
+                s_segment[tid] = s_part[tid][0] = sum == 0.0 ? 0.0 : sum * weight_of(A.most[at], s_most[here], A.c);
             }
             __syncthreads();
+            auto segment_of = [&](int d) __attribute__((always_inline)) { return (s_token[s_down[d]] + R.shift) / kPiece / A.pieces; };
             if (tid == 0)
                 for (int d = 0; d < down; ++d) {
-                    const int g = (s_token[s_down[d]] + R.shift) / kPiece / A.pieces;
+                    const int g = segment_of(d);
                     const double rest = s_segment[g] - weight_of(s_logit[s_down[d]], s_most[here], A.c);
                     s_segment[g] = rest > 0.0 ? rest : 0.0;
                 }
+            // what is left of nearly all of a segment may be roundings, with no token behind them: that segment is added up anew
+            if (down > 0) {
+                __syncthreads();
+                uint64_t again = 0;
+                for (int d = 0; d < down; ++d) {
+                    const int g = segment_of(d);
+                    if (s_segment[g] > 0.0 && !(s_segment[g] > kSmall * s_part[g][0])) again |= 1ull << g;
+                }
+                again = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(again >> 32)) << 32 | (uint32_t)__builtin_amdgcn_readfirstlane((int)again);
+                __syncthreads();  // before measure writes what others may still read
+                for (; again != 0; again &= again - 1) measure(__builtin_ctzll(again), __builtin_ctzll(again) + 1);
+            }
         }
     }
     __syncthreads();

@@ -543,6 +543,24 @@ def test_verify_where_nothing_is_left():
         assert got[1].tolist() == [1] and got[2].tolist() == [want]
 
 
+@pytest.mark.parametrize("fp32", [False, True])
+def test_verify_where_all_of_a_segment_is_turned_down(fp32):
+    """The siblings that were turned down are all that the row has among its first tokens: what rounding leaves of their sum is no
+    token, and a walk that samples at 0 ends with the first of the others."""
+    rng = np.random.default_rng(3)
+    count, vocab = 60, 9001
+    logits = np.full((4 * count, vocab), -np.inf, np.float32 if fp32 else np.float16)
+    logits[0::4, 8000] = logits[0::4, 8999] = 0.0
+    for at in (3, 70, 900):
+        logits[0::4, at] = rng.uniform(-4, 1, count)
+    logits[:, 8000] = 0.0
+    tokens = torch.tensor([0, 3, 70, 900] * count, device="cuda")
+    accept = torch.tensor([0.0, 0.999, 0.9995, 0.9999] * count, device="cuda")
+    path, counts, token = verify_drafts(torch.from_numpy(logits).cuda(), tokens, i32([-1, 0, 0, 0] * count), i32(list(range(0, 4 * count + 1, 4))),
+                                        accept, torch.zeros(count, device="cuda"))
+    assert (counts == 1).all() and (token == 8000).all()
+
+
 def test_verify_rows_without_a_distribution():
     rng = np.random.default_rng(0)
     good = rng.standard_normal((6, 4000)).astype(np.float16)

@@ -39,7 +39,7 @@ __global__ void __launch_bounds__(kWave) tree_masks_kernel(const int32_t* parent
 
 constexpr int kSegments = 64;         // of a row, at most: one per lane
 constexpr int kPiece = 8;             // elements that a thread takes at once
-constexpr double kSmall = 0x1p-20;    // of a row's sum: what is left of less is added up anew, as a difference has lost its bits
+constexpr double kSmall = 0x1p-20;    // of a row's or a segment's sum: what is left of less is added up anew, as a difference has lost its bits
 constexpr int kStatThreads = 256;
 // Of a walk: greedy, 16 waves take the statistics of 64 rows (24 trees 36 us in all, 38 with eight); else every barrier counts (32
 // chains with draft probabilities 33 us with eight waves, 37 with 16, 38 with four).

@@ -10,28 +10,30 @@
 // V's codes lie in a lane.  Softmax and its statistics are then a lane's own but for the maximum, and the weights are the B
 // operand of
 //   O^T [channel][row] += V^T P^T
-// as they are, without the LDS.  V = code * scale + low is rounded to fp16 once (the row that reskv_int4_gather gives).
+// as they are, without the LDS.  V = code * scale + low is rounded to fp16 once (the row that reskv_int4_gather gives; half of it where a
+// scale is so large that it may pass fp16's end, twice).
 //
 // Scores, softmax and sums are fp32.  Weights are 2^8 exp2(x - m), m at most 6 below the row's largest score so far, rounded
 // to fp16 for the product and summed as rounded: eleven bits down to 2^-22 of the largest weight.  With V and the weights rounded
-// to fp16, results differ from those of 64 bits by 2.8e-4 to 3.0e-4, of which their own rounding is 2.07e-4; V as codes with the
-// scales in the weights (int4.hip) would be 2.2e-4, and takes a rounding of every weight for each of the four groups instead of one.
+// to fp16, results differ from those of 64 bits by 2.8e-4 to 2.9e-4 (1 to 64 nodes after 23 to 65001 tokens, keys with outlier channels), of
+// which their own rounding is 2.07e-4; V as codes with the scales in the weights (int4.hip) would be 2.2e-4, and takes a rounding of every weight for each of the four groups instead of one.
 //
 // Up to 64 rows a wave works by itself on 16 or 32 of them and takes what it needs of a block from memory to registers; from
 // there on four or eight waves share the operands of two blocks at a time through the LDS, where the work of making them, as
-// much as that of 32 rows, is done once.  32 sequences of 4000 tokens, 32 / 8 heads, us by nodes a tree, as chosen / 32 rows a wave
-// alone / 128 and 256 rows together: 16: 93 / 93 / 117 / 144, 20: 121 / 125 / 121 / 146, 32: 130 / 151 / 132 / 150, 48: 200 / 199 /
-// 219 / 198.
+// much as that of 32 rows, is done once.  32 sequences of 4000 tokens, 32 / 8 heads, us by nodes a tree, 32 rows a wave alone / 128
+// and 256 rows together, with a star as chosen: 16: 93* / 114 / 136, 20: 114 / 115* / 136, 32: 137 / 123* / 140, 48: 205 / 211 / 182*,
+// 64: 246 / 217 / 187*.
 //
-// Bound: few rows by memory's latency and the vector ALU together (32 trees of up to 16 nodes after 2000 to 8192 tokens: 76 us and
+// Bound: few rows by memory's latency and the vector ALU together (32 trees of up to 16 nodes after 2000 to 8192 tokens: 77 us and
 // 10 for the merge; 370 vector instructions per block and 32 rows, the ALU issuing in half of the cycles); many rows by the vector
-// ALU and the matrix cores one after the other (32 trees of 64 nodes after 8192 tokens: 352 us, 780 TFLOP/s; 190 vector instructions,
+// ALU and the matrix cores one after the other (32 trees of 64 nodes after 8192 tokens: 370 us with the merge's 10, 745 TFLOP/s; 190 vector instructions,
 // 16 of them exponentials, and 36 products per block and 32 rows: the ALU issues in 58% of the cycles, the matrix cores are busy in
 // 34%, and little of that is at the same time).
 // What made no difference there: the order of reads, products and sums in a wave by hand, one barrier per block or per two,
 // a third buffer with the barrier before the products.  One tile of rows a wave and four waves a SIMD (registers spill) took 469 us
 // where this took 434, four waves and half the rows a workgroup 468, two 580; a wave's priority while it multiplies brought 410 to
-// 393, the lowest values' share in two fp16 parts instead of one fp32 product 388 to 362.
+// 393, the lowest values' share in fp16 parts instead of one fp32 product 388 to 362 (the third part, and the check for values past
+// fp16's end, made that 370).
 #include "int4.h"
 #include "reskv_drafts.h"
 

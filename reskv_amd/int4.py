@@ -252,11 +252,11 @@ def int4_tree_attention(q, pages, table, lengths, offsets, seen=None, *, scaling
     infinities included; a node that sees nothing gives zeros.
 
     Hq is any multiple of the pool's KV heads.  ``max_length`` bounds the lengths as in ``int4_attention``; ``max_nodes``
-    (up to 64) bounds the nodes of a sequence: both steer how the work is split.  Returns fp16 [N, Hq, 128], ``out``
+    (up to 64) bounds the nodes of a sequence: both steer how the work is split, so pass what is known.  Returns fp16 [N, Hq, 128], ``out``
     when given (contiguous); rows of no sequence and nodes from ``max_nodes`` on are zero, or left as they are in ``out``.
 
-    Scores, softmax and sums are fp32; V is rounded to fp16 (what ``int4_gather`` gives) and so are the softmax weights, for
-    their product.
+    Scores, softmax and sums are fp32; V is rounded to fp16 (what ``int4_gather`` gives, but that a value which its scale's rounding
+    takes past fp16's largest stays a number) and so are the softmax weights, for their product.
     """
     count, tokens, kv_heads = _pool(pages)
     sequences, width = _table(table)
